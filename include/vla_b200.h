@@ -173,6 +173,41 @@ VLAB200_API int32_t vlab200_denoise_attn_loop_static(const vlab200_kv_store *st,
 VLAB200_API int32_t vlab200_denoise_attn_loop_host(const vlab200_kv_store *st, const vlab200_denoise_attn_args *a,
                                                    void *x_stage, void *out_host, void *stream);
 
+/* --------------------------------------------- a prefix cache whose observations differ in length */
+
+/* Angles per position of the rotated pairs of a head, and the factor on their cosines and sines (host only; needs no GPU).
+ * freqs_host: double [rot_dim/2].  scaling 0 = none: f_i = base^(-2i/rot_dim); 1 = linear: f_i / factor; 2 = NTK-aware:
+ * base * factor^(rot_dim/(rot_dim-2)); 3 = YaRN: pairs that turn more than 32 times within original_len positions keep f_i, those that
+ * turn less than once get f_i / factor, a linear ramp over the pairs in between, and *mscale_host = 0.1 ln(factor) + 1 (1 otherwise).
+ * factor >= 1; original_len is read with scaling 3 only.  The reference knows the unscaled form (src/models/smolvla.cpp:759-766). */
+VLAB200_API int32_t vlab200_rope_freqs(double *freqs_host, float *mscale_host, int32_t rot_dim, double base, int32_t scaling,
+                                       double factor, int32_t original_len);
+
+/* Per-head RMSNorm of q and k, rotation at given positions, and the append of K / V, over a projection's rows in one pass:
+ *   y = x * rsqrt(mean over the head of x^2 + eps) * norm[head_dim]       (q, k; left out where the norm vector is NULL)
+ *   columns [0, rot_dim) of every q and k head turned by pos * freqs[i]: pairs (i, i + rot_dim/2), or (2i, 2i + 1) if interleaved;
+ *   cosines and sines times mscale; the other columns of the head stay; one rounding to bf16.  V is rounded only.
+ * Token t of observation b is row b * S + t of x; its K and V go to row row0[b] + t of the pages of `layer` and are left out where that
+ * row is not in [0, cap).  Angles are formed in 64 bits: positions up to 2^31 - 1 keep float32 accuracy.
+ * A token with t >= n_tok[b] is padding: its x is not read, its q is written as zero, nothing of it is stored in the pages.
+ * The reference's suffix has one prefix length for all rows and neither norms nor a choice of layout (src/models/pi0.cpp:170-201). */
+typedef struct {
+    const void *x;        /* [n_obs * S] rows of q heads | k heads | v heads (with_kv == 0: q heads), bf16 or float32, 16-byte aligned */
+    int64_t x_stride;     /* elements between rows, a multiple of 16 bytes, at least the row's width */
+    const float *q_norm;  /* [head_dim] or NULL */
+    const float *k_norm;
+    const double *freqs;  /* [rot_dim/2] (device): vlab200_rope_freqs */
+    const int32_t *pos;   /* [n_obs * S] or NULL: the page row, row0[b] + t */
+    const int32_t *row0;  /* [n_obs] or NULL: the store's prefix_len */
+    const int32_t *n_tok; /* [n_obs] or NULL: S */
+    void *q_out;          /* bf16 [n_obs][n_q][S][head_dim] */
+    int32_t S, n_q, rot_dim, interleaved, x_is_f32, with_kv;
+    float eps, mscale;
+} vlab200_qk_norm_rope_args;
+
+VLAB200_API int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, const vlab200_qk_norm_rope_args *a,
+                                                void *stream);
+
 /* ------------------------------------------------------------- whole denoise loop (engine) */
 
 /* Shape of a flow-matching policy's action expert (fields follow vla_config of include/vla.h:59-96

@@ -31,7 +31,9 @@ from .api import (  # noqa: F401
     node_norm,
     node_scale,
     node_unary,
+    qk_norm_rope_append,
     qkv_rope_append,
+    rope_freqs,
     rope_table,
     selftest_bounded_wait,
     set_gemm_tiling,

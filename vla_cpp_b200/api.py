@@ -77,6 +77,7 @@ EXPORTS = [
     "vlab200_qkv_rope_append",
     "vlab200_attention", "vlab200_denoise_attn_loop", "vlab200_denoise_attn_loop_host",
     "vlab200_denoise_attn_loop_static",
+    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append",
     "vlab200_engine_create", "vlab200_engine_free", "vlab200_engine_set_prefix", "vlab200_engine_denoise",
     "vlab200_engine_denoise_host", "vlab200_engine_run_stage", "vlab200_engine_set_prefix_len",
     "vlab200_engine_loop_phases", "vlab200_loop_kernel_phases",
@@ -256,6 +257,102 @@ def attention(store, layer, q, S, n_q, kv_len, mask_mode, pad_ranges=None, out=N
     _check(lib().vlab200_attention(C.byref(store.c), layer, _ptr(q), _ptr(out), S, n_q, kv_len, mask_mode,
                                    _ptr(pad_ranges), _stream()), "vlab200_attention")
     return out
+
+
+def _need(ok, what):
+    if not ok:
+        raise VlaB200Error(ERR_ARG, what)
+
+
+def _need_tensor(t, name, dtype, shape, dev):
+    """t is a contiguous tensor of this type and shape on cuda device `dev` (an index).  A call makes half a dozen of these checks, so the
+    text of an error is put together only where there is one."""
+    import torch
+
+    if not isinstance(t, torch.Tensor):
+        raise VlaB200Error(ERR_ARG, f"{name}: a tensor is needed, not {type(t).__name__}")
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise VlaB200Error(ERR_ARG, f"{name}: a contiguous {dtype} tensor {tuple(shape)} on cuda:{dev} is needed, not {t.dtype} "
+                                    f"{tuple(t.shape)} (strides {t.stride()}) on {t.device}")
+
+
+def _call_on(dev, fn, what, *args):
+    """fn(*args, stream) with cuda device `dev` (an index) current, on its current stream."""
+    import torch
+
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    if rc != OK:
+        raise VlaB200Error(rc, what)
+
+
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def rope_freqs(rot_dim, base=10000.0, scaling="none", factor=1.0, original_len=0, device="cuda"):
+    """-> (float64 [rot_dim/2] on `device`: angle per position of every rotated pair, factor on cosines and sines)."""
+    import torch
+
+    _need(scaling in ROPE_SCALING, f"scaling: {scaling!r} is not one of {sorted(ROPE_SCALING)}")
+    _need(int(rot_dim) > 0 and int(rot_dim) % 2 == 0, "rot_dim: an even number is needed")
+    f, m = (C.c_double * (int(rot_dim) // 2))(), C.c_float()
+    _check(lib().vlab200_rope_freqs(f, C.byref(m), int(rot_dim), C.c_double(base), ROPE_SCALING[scaling], C.c_double(factor),
+                                    int(original_len)), "vlab200_rope_freqs")
+    return torch.tensor(list(f), dtype=torch.float64, device=device), m.value
+
+
+class _QkNormRopeArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64)] + [(n, C.c_void_p) for n in (
+        "q_norm", "k_norm", "freqs", "pos", "row0", "n_tok", "q_out")] + [(n, C.c_int32) for n in (
+            "S", "n_q", "rot_dim", "interleaved", "x_is_f32", "with_kv")] + [("eps", C.c_float), ("mscale", C.c_float)]
+
+
+def qk_norm_rope_append(store, layer, x, S, n_q, freqs=None, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, mscale=1.0,
+                        pos=None, row0=None, n_tok=None, with_kv=True, q_out=None):
+    """Per-head norms of q and k, rotation and append to the pages over a projection's rows.
+
+    x: cuda [n_obs * S, >= (n_q + 2 n_kv) hd] bf16 or f32 (rows may be strided); freqs: rope_freqs(...)[0] (its length says how many
+    columns of a head are rotated; None: none); q_norm, k_norm: f32 [hd] or None; pos: int32 [n_obs, S] or None (the page row);
+    row0: int32 [n_obs], the page row of every observation's first token, or None (prefix_len); n_tok: int32 [n_obs] or None (S).
+    Returns q: bf16 [n_obs, n_q, S, hd]; K / V land in the store (with_kv=False: x holds q heads only)."""
+    import torch
+
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float32):
+        raise VlaB200Error(ERR_ARG, "x: a bf16 or f32 cuda tensor is needed")
+    dev, B, hd, f32, i32 = x.get_device(), store.n_obs, store.head_dim, torch.float32, torch.int32
+    width = (n_q + (2 * store.n_kv if with_kv else 0)) * hd
+    if store.k.get_device() != dev:
+        raise VlaB200Error(ERR_ARG, f"the store is on {store.k.device}, x on {x.device}")
+    if S < 0 or n_q <= 0 or x.dim() != 2 or x.shape[0] != B * S or x.shape[1] < width or x.stride(1) != 1:
+        raise VlaB200Error(ERR_ARG, f"x: [{B * S}, >= {width}] with adjacent columns is needed, not {tuple(x.shape)}")
+    if freqs is not None:
+        _need_tensor(freqs, "freqs", torch.float64, (freqs.numel(),), dev)
+    if q_norm is not None:
+        _need_tensor(q_norm, "q_norm", f32, (hd,), dev)
+    if k_norm is not None:
+        _need_tensor(k_norm, "k_norm", f32, (hd,), dev)
+    if pos is not None:
+        _need_tensor(pos, "pos", i32, (B, S), dev)
+    if row0 is not None:
+        _need_tensor(row0, "row0", i32, (B,), dev)
+    if n_tok is not None:
+        _need_tensor(n_tok, "n_tok", i32, (B,), dev)
+    if q_out is None:
+        q_out = torch.empty((B, n_q, S, hd), dtype=torch.bfloat16, device=x.device)
+    else:
+        _need_tensor(q_out, "q_out", torch.bfloat16, (B, n_q, S, hd), dev)
+    if B * S == 0:
+        return q_out
+    a = _QkNormRopeArgs(x.data_ptr(), x.stride(0) if B * S > 1 else width, q_norm.data_ptr() if q_norm is not None else None,
+                        k_norm.data_ptr() if k_norm is not None else None, freqs.data_ptr() if freqs is not None else None,
+                        pos.data_ptr() if pos is not None else None, row0.data_ptr() if row0 is not None else None,
+                        n_tok.data_ptr() if n_tok is not None else None, q_out.data_ptr(), S, n_q,
+                        2 * freqs.numel() if freqs is not None else 0, bool(interleaved), x.dtype is f32, bool(with_kv), eps, mscale)
+    _call_on(dev, lib().vlab200_qk_norm_rope_append, "vlab200_qk_norm_rope_append", C.byref(store.c), layer, C.byref(a))
+    return q_out
 
 
 class _DenoiseAttnArgs(C.Structure):
