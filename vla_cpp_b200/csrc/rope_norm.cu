@@ -1,15 +1,15 @@
 // Per-head RMSNorm of q and k, rotary positions and the append of K / V to the pages, in one pass over a projection's rows:
 //
 //   y = x / sqrt(mean(x^2) + eps) * w            (a head's columns; 32 bits; left out where there is no w)
-//   a_i = pos * f_i                              (64 bits, brought into half a turn before it is rounded to 32)
+//   a_i = pos * f_i                              (64 bits, whole turns taken out before it is rounded to 32)
 //   (y_u, y_v) -> (y_u c - y_v s, y_v c + y_u s) with c = m cos a_i, s = m sin a_i;  half layout: u, v = i, i + r / 2;
 //                                                 interleaved: u, v = 2 i, 2 i + 1;  columns from r on stay
 //   one rounding to bf16; V is rounded only.
 //
 // The op reads and writes every element once and does some ten operations on it: HBM bounds it.  A warp takes a token and walks its
-// heads, 8 columns (16 bytes of bf16) per lane, so the token's cosines and sines stay in registers (every lane computes
-// r / 64 of them, they are exchanged through shared memory once per token) and a head's partner columns come by
-// shuffle.  Loads of two steps are in flight per warp.  Few tokens: a token's heads are dealt over several warps.
+// heads, 16 columns per lane, so the token's cosines and sines stay in registers (every lane computes r / 64 of them, they
+// are exchanged through shared memory once per token).  In the half layout a lane holds columns 8 j .. 8 j + 7 and their partners r / 2
+// further on, so the rotation needs no exchange.  Few tokens: a token's heads are dealt over several warps.
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -28,28 +28,55 @@ struct RopeNormParams {
     const double *freqs;
     const int32_t *pos, *row0, *n_tok;
     __nv_bfloat16 *q_out, *k, *v;  // k, v: pages of the layer
-    long long M;                   // n_obs * S rows
+    unsigned M;                    // n_obs * S rows
     int S, n_q, n_kv, n_heads, cap, prefix_len, rot, parts;  // n_heads: heads of a row; parts: warps that share a token
     float eps, mscale;
 };
 
 enum : int { ROPE_PAIRS = 0, ROPE_HALF_LANES = 1, ROPE_HALF_ANY = 2 };
 
-// 8 columns of a lane as float32
+// Two float32 per register pair: one instruction of the FMA pipe serves both.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f2_get(F2 a, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ uint32_t f2_bf16(F2 a) {
+    float lo, hi;
+    f2_get(a, lo, hi);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 8 columns of a lane
 template <bool F32>
 struct RnChunk;
 template <>
 struct RnChunk<false> {
     uint4 r;
     __device__ __forceinline__ void load(const void *x, long long i) { r = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(x) + i); }
-    __device__ __forceinline__ void get(float (&f)[8]) {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            f[2 * e] = __uint_as_float(w[e] << 16);
-            f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        }
+    __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(F2 (&f)[4]) {
+        f[0] = f2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u));
+        f[1] = f2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u));
+        f[2] = f2(__uint_as_float(r.z << 16), __uint_as_float(r.z & 0xffff0000u));
+        f[3] = f2(__uint_as_float(r.w << 16), __uint_as_float(r.w & 0xffff0000u));
     }
+    __device__ __forceinline__ uint4 as_bf16() { return r; }
 };
 template <>
 struct RnChunk<true> {
@@ -59,177 +86,292 @@ struct RnChunk<true> {
         a = s[0];
         b = s[1];
     }
-    __device__ __forceinline__ void get(float (&f)[8]) {
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void get(F2 (&f)[4]) {
+        f[0] = f2(a.x, a.y);
+        f[1] = f2(a.z, a.w);
+        f[2] = f2(b.x, b.y);
+        f[3] = f2(b.z, b.w);
+    }
+    __device__ __forceinline__ uint4 as_bf16() {
+        F2 f[4];
+        get(f);
+        return make_uint4(f2_bf16(f[0]), f2_bf16(f[1]), f2_bf16(f[2]), f2_bf16(f[3]));
     }
 };
 
+// What a warp needs to know of a token before it works on it; fetched while it works on the one before.
+struct RnToken {
+    long long row, pos;
+    unsigned m;
+    int obs, t;
+    bool exists, live;
+};
+__device__ __forceinline__ void rn_fetch_token(RnToken &k, const RopeNormParams &p) {
+    k.exists = k.m < p.M;
+    k.live = k.exists && (p.n_tok == nullptr || k.t < p.n_tok[k.obs]);
+    k.row = (k.live && p.row0 ? (long long)p.row0[k.obs] : (long long)p.prefix_len) + k.t;
+    k.pos = k.live && p.pos ? (long long)p.pos[k.m] : k.row;
+}
+__device__ __forceinline__ void lds_f2x4(F2 (&f)[4], const float *s) {  // 8 floats, 16-byte aligned
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(s), b = *reinterpret_cast<const ulonglong2 *>(s + 4);
+    f[0].v = a.x;
+    f[1].v = a.y;
+    f[2].v = b.x;
+    f[3].v = b.y;
+}
+
 template <int HD, int MODE, bool F32>
-__global__ void __launch_bounds__(RN_WARPS * 32) qk_norm_rope_kernel(const RopeNormParams p) {
-    constexpr int LH = HD / 8;         // lanes per head
+__global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const RopeNormParams p) {
+    constexpr int LH = HD / 16;        // lanes per head: two chunks of 8 columns each
     constexpr int HPW = 32 / LH;       // heads per warp and step
-    constexpr int DEPTH = F32 ? 2 : 4; // steps whose loads are in flight
+    constexpr int DEPTH = F32 ? 1 : 2; // steps whose loads are in flight beside the one being worked on
     __shared__ __align__(16) float s_cos[RN_WARPS][HD / 2], s_sin[RN_WARPS][HD / 2], s_w[2][HD];
-    __shared__ float s_y[MODE == ROPE_HALF_ANY ? RN_WARPS : 1][MODE == ROPE_HALF_ANY ? 256 : 1];
+    __shared__ long long s_turn[HD / 2];  // turns per position in units of 2^-64
+    __shared__ float s_y[MODE == ROPE_HALF_ANY ? RN_WARPS : 1][MODE == ROPE_HALF_ANY ? 512 : 1];
     pdl_launch_dependents();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long task = (long long)blockIdx.x * RN_WARPS + warp;
-    const long long m = task / p.parts;
-    const int part = (int)(task % p.parts);
-    const int obs = (int)(m / p.S), t = (int)(m % p.S);
-    const bool exists = m < p.M;
-    const bool live = exists && (p.n_tok == nullptr || t < p.n_tok[obs]);
-    const int jl = lane % LH, c0 = jl * 8;
-    const int n_steps = (p.n_heads + HPW - 1) / HPW, hstep = p.parts * HPW;
-    const int head0 = part * HPW + lane / LH;
-    const long long x_row = m * p.x_stride + c0;
-    RnChunk<F32> ring[DEPTH];
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int half = p.rot >> 1;
+    // This lane's two chunks start at columns cu and cv.  Half layout with rot % 16 == 0: the two columns of every pair are in one lane
+    // (columns from rot on: two chunks side by side); otherwise 16 columns side by side.
+    const int jl = lane % LH, lh = lane / LH;
+    const bool across = MODE == ROPE_HALF_LANES && jl < (p.rot >> 4);
+    const int cu = across ? jl * 8 : jl * 16, cv = across ? half + jl * 8 : jl * 16 + 8;
+    const bool turned = MODE == ROPE_HALF_LANES ? across : cu < p.rot;
+    // a token's steps: those of its q heads, then of its k heads, then of its v heads, HPW heads each; this warp takes every parts-th
+    const int nsq = (p.n_q + HPW - 1) / HPW, nsk = p.n_heads > p.n_q ? (p.n_kv + HPW - 1) / HPW : 0, n_steps = nsq + 2 * nsk;
+    const unsigned n_warps = gridDim.x * RN_WARPS, task = blockIdx.x * RN_WARPS + warp;
+    const int part = (int)(task % (unsigned)p.parts);
+    const int my_steps = (n_steps - part + p.parts - 1) / p.parts;
+    const int my_slots = (my_steps + DEPTH - 1) / DEPTH * DEPTH;  // a token starts at slot 0 of the ring
+    RnToken tok, nxt;
+    tok.m = task / (unsigned)p.parts;
+    tok.obs = (int)(tok.m / (unsigned)p.S);
+    tok.t = (int)(tok.m - (unsigned)tok.obs * (unsigned)p.S);
+    rn_fetch_token(tok, p);
+    // a warp has more than one token only where parts == 1
+    const int d_obs = (int)(n_warps / (unsigned)p.S), d_t = (int)(n_warps - (unsigned)d_obs * (unsigned)p.S);
+    RnChunk<F32> ru[DEPTH], rv[DEPTH];
+    auto fetch = [&](int d, const RnToken &k, int i) {  // this lane's columns in the warp's i-th step of a token
+        const int s = part + i * p.parts;
+        const int h = (s < nsq ? s : s < nsq + nsk ? s - nsq : s - nsq - nsk) * HPW + lh;  // among its kind
+        if (k.live && s < n_steps && h < (s < nsq ? p.n_q : p.n_kv)) {
+            const long long at = (long long)k.m * p.x_stride + (h + (s < nsq ? 0 : s < nsq + nsk ? p.n_q : p.n_q + p.n_kv)) * HD;
+            ru[d].load(p.x, at + cu);
+            rv[d].load(p.x, at + cv);
+        }
+    };
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-        if (live && head0 + d * hstep < p.n_heads) ring[d].load(p.x, x_row + (long long)(head0 + d * hstep) * HD);
+    for (int d = 0; d < DEPTH; ++d) {
+        ru[d].zero();
+        rv[d].zero();
+        fetch(d, tok, d);
+    }
     for (int i = threadIdx.x; i < 2 * HD; i += RN_WARPS * 32) {
         const float *w = i < HD ? p.q_norm : p.k_norm;
         s_w[0][i] = w ? w[i < HD ? i : i - HD] : 1.0f;
     }
+    if (threadIdx.x < half) {
+        const double turns = p.freqs[threadIdx.x] * 0.15915494309189533577;
+        s_turn[threadIdx.x] = __double2ll_rn((turns - rint(turns)) * 18446744073709551616.0);
+    }
     __syncthreads();
-    if (!exists) return;
-    if (!live) {  // a padding token: q is zero, its row of the pages stays as it is
-        for (int head = head0; head < p.n_q; head += hstep)
-            *reinterpret_cast<uint4 *>(p.q_out + (((long long)obs * p.n_q + head) * p.S + t) * HD + c0) = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    const long long row = (p.row0 ? (long long)p.row0[obs] : (long long)p.prefix_len) + t;
-    const double pos = p.pos ? (double)p.pos[m] : (double)row;
-    const int half = p.rot >> 1;
-    for (int i = lane; i < half; i += 32) {
-        // whole turns go before the rounding to 32 bits: a position of 10^6 would otherwise lose 0.06 of a radian
-        double turns = pos * p.freqs[i] * 0.15915494309189533577;
-        turns -= rint(turns);
-        float sn, cs;
-        sincospif(2.0f * (float)turns, &sn, &cs);
-        s_cos[warp][i] = cs * p.mscale;
-        s_sin[warp][i] = sn * p.mscale;
-    }
-    __syncwarp();
-    constexpr int NCS = MODE == ROPE_PAIRS ? 4 : 8;
-    float cs[NCS], sn[NCS];  // of this lane's columns: 1 and 0 where they are not rotated
-    int partner = lane;      // ROPE_HALF_LANES: the lane with the other column of every pair
-#pragma unroll
-    for (int e = 0; e < NCS; ++e) {
-        cs[e] = 1.0f;
-        sn[e] = 0.0f;
-        if (MODE == ROPE_PAIRS) {
-            const int i = c0 / 2 + e;
-            if (i < half) {
-                cs[e] = s_cos[warp][i];
-                sn[e] = s_sin[warp][i];
-            }
-        } else {
-            const int c = c0 + e;
-            if (c < p.rot) {
-                const int i = c < half ? c : c - half;
-                cs[e] = s_cos[warp][i];
-                sn[e] = c < half ? -s_sin[warp][i] : s_sin[warp][i];  // y_u c - y_v s, y_v c + y_u s
-            }
+    const int q_head = p.S * HD, kv_head = p.cap * HD;
+    for (; tok.exists; tok = nxt) {
+        nxt.m = tok.m + n_warps;
+        nxt.obs = tok.obs + d_obs;
+        nxt.t = tok.t + d_t;
+        if (nxt.t >= p.S) {
+            nxt.t -= p.S;
+            ++nxt.obs;
         }
-    }
-    const bool turned = c0 < p.rot;
-    if (MODE == ROPE_HALF_LANES && turned) partner = c0 < half ? lane + half / 8 : lane - half / 8;
-    const bool row_ok = row >= 0 && row < p.cap;
-    float w[8];
-    int w_of = -1;  // whose norm weights w holds: 0 q, 1 k
-    int head = head0;
-    for (int step = part; step < n_steps; step += p.parts * DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d, head += hstep) {
-            if (step + d * p.parts >= n_steps) break;  // the same for every lane
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-            if (head < p.n_heads) ring[d].get(y);
-            if (head + DEPTH * hstep < p.n_heads) ring[d].load(p.x, x_row + (long long)(head + DEPTH * hstep) * HD);
-            const bool is_q = head < p.n_q, is_v = head >= p.n_q + p.n_kv;
-            float ss = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-#pragma unroll
-            for (int off = LH / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-            const bool normed = !is_v && (is_q ? p.q_norm != nullptr : p.k_norm != nullptr);
-            const float inv = normed ? 1.0f / sqrtf(ss * (1.0f / HD) + p.eps) : 1.0f;
-            if (!is_v && w_of != (is_q ? 0 : 1)) {
-                w_of = is_q ? 0 : 1;
-                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(&s_w[w_of][c0]);
-                *reinterpret_cast<float4 *>(w + 4) = *reinterpret_cast<const float4 *>(&s_w[w_of][c0 + 4]);
+        rn_fetch_token(nxt, p);
+        __nv_bfloat16 *const q_dst = p.q_out + ((long long)tok.obs * p.n_q * p.S + tok.t) * HD;
+        if (!tok.live) {  // a padding token: q is zero, its row of the pages stays as it is
+            for (int s = part; s < nsq; s += p.parts) {
+                const int h = s * HPW + lh;
+                if (h >= p.n_q) break;
+                *reinterpret_cast<uint4 *>(q_dst + (long long)h * q_head + cu) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(q_dst + (long long)h * q_head + cv) = make_uint4(0, 0, 0, 0);
             }
-            float o[8];
-            if (MODE == ROPE_PAIRS) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = y[e] * inv * w[e];
-                if (turned) {
+            for (int d = 0; d < DEPTH; ++d) fetch(d, nxt, d);
+            continue;
+        }
+        const bool row_ok = tok.row >= 0 && tok.row < p.cap;
+        const long long kv0 = (long long)tok.obs * p.n_kv * kv_head + tok.row * HD;
+        __syncwarp();
+        for (int i = lane; i < half; i += 32) {
+            // The angle in units of 2^-64 turns: whole turns drop out of the product, which would otherwise cost a float32 angle 0.06 of
+            // a radian at position 10^6.  What is left lies within half a turn, where the fast sine and cosine are off by 2^-21 at
+            // most: 2^-13 of the rounding to bf16 that follows.
+            const unsigned long long a = (unsigned long long)tok.pos * (unsigned long long)s_turn[i];
+            const float rad = (float)(int)(a >> 32) * 1.4629180792671596e-9f;  // 2 pi 2^-32
+            s_cos[warp][i] = __cosf(rad) * p.mscale;
+            s_sin[warp][i] = __sinf(rad) * p.mscale;
+        }
+        __syncwarp();
+        // half layout:  out_u = scale (y_u au - y_v bv),  out_v = scale (y_v av + y_u bu): norm weights times cosine (a) and sine (b)
+        // interleaved:  the same within a chunk, with the pair's two products side by side
+        F2 au[4], av[4], bu[4], bv[4];
+        int kind = -1;  // whose norm weights they hold: 0 q, 1 k
+        for (int i0 = 0; i0 < my_slots; i0 += DEPTH) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                RnChunk<F32> xu = ru[d], xv = rv[d];
+                const bool more = i0 + DEPTH < my_slots;
+                fetch(d, more ? tok : nxt, more ? i0 + d + DEPTH : d);
+                const int s = part + (i0 + d) * p.parts;
+                if (s >= n_steps) continue;
+                const int now = s < nsq ? 0 : s < nsq + nsk ? 1 : 2;
+                const int h = (now == 0 ? s : now == 1 ? s - nsq : s - nsq - nsk) * HPW + lh;
+                uint4 du, dv;
+                if (now == 2) {
+                    du = xu.as_bf16();
+                    dv = xv.as_bf16();
+                } else {
+                    if (kind != now) {
+                        kind = now;
+                        const float *w = s_w[kind], *ct = s_cos[warp], *st = s_sin[warp];
+                        if (MODE == ROPE_HALF_LANES) {
+                            lds_f2x4(au, w + cu);
+                            lds_f2x4(av, w + cv);
+                            if (across) {
+                                F2 c[4], sn[4];
+                                lds_f2x4(c, ct + cu);
+                                lds_f2x4(sn, st + cu);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    bu[e] = f2_mul(au[e], sn[e]);
+                                    bv[e] = f2_mul(f2_mul(av[e], sn[e]), f2(-1.0f, -1.0f));
+                                    au[e] = f2_mul(au[e], c[e]);
+                                    av[e] = f2_mul(av[e], c[e]);
+                                }
+                            }
+                        } else if (MODE == ROPE_PAIRS) {
+                            lds_f2x4(au, w + cu);
+                            lds_f2x4(av, w + cv);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int iu = (cu >> 1) + e, iv = (cv >> 1) + e;
+                                const float cc = iu < half ? ct[iu] : 1.0f, ss = iu < half ? st[iu] : 0.0f;
+                                const float dc = iv < half ? ct[iv] : 1.0f, ds = iv < half ? st[iv] : 0.0f;
+                                float lo, hi;
+                                f2_get(au[e], lo, hi);
+                                bu[e] = f2(-(hi * ss), lo * ss);
+                                f2_get(av[e], lo, hi);
+                                bv[e] = f2(-(hi * ds), lo * ds);
+                                au[e] = f2_mul(au[e], f2(cc, cc));
+                                av[e] = f2_mul(av[e], f2(dc, dc));
+                            }
+                        } else {
+                            auto a_of = [&](int x) { return x < p.rot ? w[x] * ct[x < half ? x : x - half] : w[x]; };
+                            auto b_of = [&](int x) { return x >= p.rot ? 0.0f : x < half ? -(w[x + half] * st[x]) : w[x - half] * st[x - half]; };
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int c = 2 * e;
+                                au[e] = f2(a_of(cu + c), a_of(cu + c + 1));
+                                av[e] = f2(a_of(cv + c), a_of(cv + c + 1));
+                                bu[e] = f2(b_of(cu + c), b_of(cu + c + 1));
+                                bv[e] = f2(b_of(cv + c), b_of(cv + c + 1));
+                            }
+                        }
+                    }
+                    F2 yu[4], yv[4], ou[4], ov[4];
+                    xu.get(yu);
+                    xv.get(yv);
+                    F2 s2 = f2_mul(yu[0], yu[0]), s3 = f2_mul(yv[0], yv[0]);
+#pragma unroll
+                    for (int e = 1; e < 4; ++e) {
+                        s2 = f2_fma(yu[e], yu[e], s2);
+                        s3 = f2_fma(yv[e], yv[e], s3);
+                    }
+                    float sa, sb, sc, sd;
+                    f2_get(s2, sa, sb);
+                    f2_get(s3, sc, sd);
+                    float ss = (sa + sb) + (sc + sd);
+#pragma unroll
+                    for (int off = LH / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float a = o[2 * e], b = o[2 * e + 1];
-                        o[2 * e] = a * cs[e] - b * sn[e];
-                        o[2 * e + 1] = b * cs[e] + a * sn[e];
+                        ou[e] = f2_mul(yu[e], au[e]);
+                        ov[e] = f2_mul(yv[e], av[e]);
                     }
-                }
-            } else if (MODE == ROPE_HALF_LANES) {
+                    if (MODE == ROPE_HALF_LANES) {
+                        if (turned) {  // columns that are not rotated stay clear of the others' infinities
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float a = y[e] * inv * w[e];
-                    const float b = __shfl_sync(0xffffffffu, a, partner);
-                    o[e] = turned ? a * cs[e] + b * sn[e] : a;
-                }
-            } else {
-                float *sy = s_y[warp] + (lane / LH) * HD;
+                            for (int e = 0; e < 4; ++e) {
+                                ou[e] = f2_fma(yv[e], bv[e], ou[e]);
+                                ov[e] = f2_fma(yu[e], bu[e], ov[e]);
+                            }
+                        }
+                    } else if (MODE == ROPE_PAIRS) {
+                        if (turned) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    o[e] = y[e] * inv * w[e];
-                    sy[c0 + e] = o[e];
-                }
-                __syncwarp();
+                            for (int e = 0; e < 4; ++e) {
+                                float lo, hi;
+                                f2_get(yu[e], lo, hi);
+                                if (cu + 2 * e < p.rot) ou[e] = f2_fma(f2(hi, lo), bu[e], ou[e]);
+                                f2_get(yv[e], lo, hi);
+                                if (cv + 2 * e < p.rot) ov[e] = f2_fma(f2(hi, lo), bv[e], ov[e]);
+                            }
+                        }
+                    } else {  // partners in the middle of other lanes' chunks: through shared memory
+                        float *sy = s_y[warp] + lh * HD;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int c = c0 + e;
-                    if (c < p.rot) o[e] = o[e] * cs[e] + sy[c < half ? c + half : c - half] * sn[e];
+                        for (int e = 0; e < 4; ++e) {
+                            f2_get(yu[e], sy[cu + 2 * e], sy[cu + 2 * e + 1]);
+                            f2_get(yv[e], sy[cv + 2 * e], sy[cv + 2 * e + 1]);
+                        }
+                        __syncwarp();
+                        auto z_of = [&](int x) { return x >= p.rot ? 0.0f : sy[x < half ? x + half : x - half]; };
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            ou[e] = f2_fma(f2(z_of(cu + 2 * e), z_of(cu + 2 * e + 1)), bu[e], ou[e]);
+                            ov[e] = f2_fma(f2(z_of(cv + 2 * e), z_of(cv + 2 * e + 1)), bv[e], ov[e]);
+                        }
+                        __syncwarp();
+                    }
+                    const bool normed = (now == 0 ? p.q_norm : p.k_norm) != nullptr;
+                    const float inv = normed ? rsqrtf(ss * (1.0f / HD) + p.eps) : 1.0f;
+                    const F2 inv2 = f2(inv, inv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        ou[e] = f2_mul(ou[e], inv2);
+                        ov[e] = f2_mul(ov[e], inv2);
+                    }
+                    du = make_uint4(f2_bf16(ou[0]), f2_bf16(ou[1]), f2_bf16(ou[2]), f2_bf16(ou[3]));
+                    dv = make_uint4(f2_bf16(ov[0]), f2_bf16(ov[1]), f2_bf16(ov[2]), f2_bf16(ov[3]));
                 }
-                __syncwarp();
+                if (now == 0 ? h < p.n_q : h < p.n_kv && row_ok) {
+                    __nv_bfloat16 *dst = now == 0 ? q_dst + (long long)h * q_head : (now == 1 ? p.k : p.v) + kv0 + (long long)h * kv_head;
+                    *reinterpret_cast<uint4 *>(dst + cu) = du;
+                    *reinterpret_cast<uint4 *>(dst + cv) = dv;
+                }
             }
-            uint32_t r[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 h = is_v ? __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]) : __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
-                r[e] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-            __nv_bfloat16 *dst = nullptr;
-            if (is_q)
-                dst = p.q_out + (((long long)obs * p.n_q + head) * p.S + t) * HD + c0;
-            else if (head < p.n_heads && row_ok)
-                dst = (is_v ? p.v : p.k) + (((long long)obs * p.n_kv + head - p.n_q - (is_v ? p.n_kv : 0)) * p.cap + row) * HD + c0;
-            if (dst) *reinterpret_cast<uint4 *>(dst) = make_uint4(r[0], r[1], r[2], r[3]);
         }
     }
 }
 
 template <int HD, int MODE, bool F32>
 static int launch_rope_norm(RopeNormParams &p, cudaStream_t stream) {
-    constexpr int HPW = 32 / (HD / 8);
-    const int n_steps = (p.n_heads + HPW - 1) / HPW;
+    constexpr int HPW = 32 / (HD / 16);
+    const int n_steps = (p.n_q + HPW - 1) / HPW + (p.n_heads > p.n_q ? 2 * ((p.n_kv + HPW - 1) / HPW) : 0);
     // a warp per token once the tokens alone fill the machine (16 warps on every SM); fewer tokens: their heads over as many warps
-    const long long fill = 16LL * sm_count();
-    long long parts = p.M >= fill ? 1 : (fill + p.M - 1) / p.M;
-    p.parts = (int)(parts < n_steps ? parts : n_steps);
-    const long long blocks = (p.M * p.parts + RN_WARPS - 1) / RN_WARPS;
-    if (blocks > 0x7fffffffLL) return VLAB200_ERR_UNSUPPORTED;
+    const unsigned fill = 16u * (unsigned)sm_count();
+    const unsigned parts = p.M >= fill ? 1 : (fill + p.M - 1) / p.M;
+    p.parts = (int)parts < n_steps ? (int)parts : n_steps;
+    // persistent: two blocks on every SM.  One part: any number of blocks is a multiple of it; more: a token's warps are all there is.
+    unsigned blocks = (p.M * (unsigned)p.parts + RN_WARPS - 1) / RN_WARPS;  // M < 2^12, or parts == 1
+    if (p.parts == 1 && blocks > 2u * (unsigned)sm_count()) blocks = 2u * (unsigned)sm_count();
     return launch_pdl(qk_norm_rope_kernel<HD, MODE, F32>, dim3((unsigned)blocks), dim3(RN_WARPS * 32), 0, stream, p);
 }
 
 template <int HD, bool F32>
 static int dispatch_rope_norm(RopeNormParams &p, int interleaved, cudaStream_t stream) {
     if (interleaved) return launch_rope_norm<HD, ROPE_PAIRS, F32>(p, stream);
-    // partner columns 8 r' apart sit in the same place of another lane's 8
+    // chunks of 8 columns and the chunks of their partners
     if (p.rot % 16 == 0) return launch_rope_norm<HD, ROPE_HALF_LANES, F32>(p, stream);
     return launch_rope_norm<HD, ROPE_HALF_ANY, F32>(p, stream);
 }
@@ -279,8 +421,14 @@ int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, c
                          (a->with_kv ? reinterpret_cast<uintptr_t>(st->k_pages) | reinterpret_cast<uintptr_t>(st->v_pages) : 0);
     if (al & 15) return VLAB200_ERR_ARG;
     vb::RopeNormParams p;
-    p.M = (long long)st->n_obs * a->S;
-    if (p.M == 0) return VLAB200_OK;
+    const long long rows = (long long)st->n_obs * a->S;
+    if (rows == 0) return VLAB200_OK;
+    if (rows > 0x7fffffffLL || (long long)a->S * hd > 0x7fffffffLL || (long long)n_heads * hd > 0x7fffffffLL ||
+        (long long)st->cap * hd > 0x7fffffffLL) {
+        vb::set_last_error("qk_norm_rope_append: more than 2^31 - 1 rows, columns of a row or elements of a page");
+        return VLAB200_ERR_UNSUPPORTED;
+    }
+    p.M = (unsigned)rows;
     const long long page0 = (long long)layer * st->n_obs * st->n_kv * st->cap * hd;
     p.x = a->x;
     p.x_stride = a->x_stride;
