@@ -208,6 +208,17 @@ typedef struct {
 VLAB200_API int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, const vlab200_qk_norm_rope_args *a,
                                                 void *stream);
 
+/* The attention weight that every cached row of `layer` got from a call's query tokens, accumulated over calls: for rows j < lens[b]
+ *   mass_out[b][h][j] = decay * mass_in[b][h][j] + sum over the n_q / n_kv heads of kv head h and the S tokens of exp(scale q . k_j - lse)
+ * q: bf16 [n_obs][n_q][S][head_dim] and lse: float32 [n_obs][n_q][S] as vlab200_cross_attention takes and returns them (a query row whose
+ * lse is -inf saw nothing and weighs nothing).  mass_in, mass_out: float32 [n_obs][n_kv][cap]; mass_in NULL or decay 0: not read, no
+ * earlier weight; mass_in may be mass_out.  lens: int32 [n_obs], taken into [0, max_len], or NULL (max_len for all);
+ * 0 <= max_len <= cap bounds the work.  pad_ranges (optional, int32 [n_obs][2]): rows [lo, hi) are hidden, their sum is 0.  Rows from
+ * lens[b] on are neither read nor written.  scale 0 = 1 / sqrt(head_dim).  Same bits from run to run.  No counterpart in the reference. */
+VLAB200_API int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, const void *q, const float *lse, const float *mass_in,
+                                     float *mass_out, int32_t S, int32_t n_q, const int32_t *lens, int32_t max_len,
+                                     const int32_t *pad_ranges, float scale, float decay, void *stream);
+
 /* ------------------------------------------------------------- whole denoise loop (engine) */
 
 /* Shape of a flow-matching policy's action expert (fields follow vla_config of include/vla.h:59-96

@@ -25,6 +25,7 @@ from .api import (  # noqa: F401
     bitvla_norm_quant,
     device_status,
     fold_norm_weight,
+    key_mass,
     lib,
     node_bin,
     node_mul_mat,

@@ -77,7 +77,7 @@ EXPORTS = [
     "vlab200_qkv_rope_append",
     "vlab200_attention", "vlab200_denoise_attn_loop", "vlab200_denoise_attn_loop_host",
     "vlab200_denoise_attn_loop_static",
-    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append",
+    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append", "vlab200_key_mass",
     "vlab200_engine_create", "vlab200_engine_free", "vlab200_engine_set_prefix", "vlab200_engine_denoise",
     "vlab200_engine_denoise_host", "vlab200_engine_run_stage", "vlab200_engine_set_prefix_len",
     "vlab200_engine_loop_phases", "vlab200_loop_kernel_phases",
@@ -353,6 +353,50 @@ def qk_norm_rope_append(store, layer, x, S, n_q, freqs=None, q_norm=None, k_norm
                         2 * freqs.numel() if freqs is not None else 0, bool(interleaved), x.dtype is f32, bool(with_kv), eps, mscale)
     _call_on(dev, lib().vlab200_qk_norm_rope_append, "vlab200_qk_norm_rope_append", C.byref(store.c), layer, C.byref(a))
     return q_out
+
+
+def _ragged_args(store, q, lens, max_len, pad_ranges):
+    """What calls over ragged observations check of their arguments -> (device index, S, n_q, max_len)."""
+    import torch
+
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 4:
+        raise VlaB200Error(ERR_ARG, "q: a cuda tensor [n_obs, n_q, S, head_dim] is needed")
+    dev, B = q.get_device(), store.n_obs
+    if store.k.get_device() != dev:
+        raise VlaB200Error(ERR_ARG, f"the store is on {store.k.device}, q on {q.device}")
+    n_q, S = q.shape[1], q.shape[2]
+    _need_tensor(q, "q", torch.bfloat16, (B, n_q, S, store.head_dim), dev)
+    if lens is not None:
+        _need_tensor(lens, "lens", torch.int32, (B,), dev)
+    if pad_ranges is not None:
+        _need_tensor(pad_ranges, "pad_ranges", torch.int32, (B, 2), dev)
+    return dev, S, n_q, store.cap if max_len is None else max_len
+
+
+def key_mass(store, layer, q, lse, lens=None, max_len=None, pad_ranges=None, scale=None, decay=1.0, mass=None, out=None):
+    """The attention weight every cached row got from the query tokens, accumulated.
+
+    q: bf16 [n_obs, n_q, S, hd]; lse: f32 [n_obs, n_q, S] (cross_attention's); lens: int32 [n_obs] rows of every observation or None
+    (max_len, by default the store's cap); pad_ranges: int32 [n_obs, 2] hidden rows [lo, hi) or None; mass: f32 [n_obs, n_kv, cap] the
+    weights so far, times decay, or None; out: where the new ones go (mass itself: in place), rows from lens on are left as they were.
+    Returns out (a zeroed new tensor if None)."""
+    import torch
+
+    dev, S, n_q, max_len = _ragged_args(store, q, lens, max_len, pad_ranges)
+    shape = (store.n_obs, store.n_kv, store.cap)
+    _need_tensor(lse, "lse", torch.float32, (store.n_obs, n_q, S), dev)
+    if mass is not None:
+        _need_tensor(mass, "mass", torch.float32, shape, dev)
+    if out is None:
+        out = torch.zeros(shape, dtype=torch.float32, device=q.device)
+    else:
+        _need_tensor(out, "out", torch.float32, shape, dev)
+    _call_on(dev, lib().vlab200_key_mass, "vlab200_key_mass", C.byref(store.c), layer, C.c_void_p(q.data_ptr()), C.c_void_p(lse.data_ptr()),
+             C.c_void_p(mass.data_ptr()) if mass is not None else None, C.c_void_p(out.data_ptr()), S, n_q,
+             C.c_void_p(lens.data_ptr()) if lens is not None else None, max_len,
+             C.c_void_p(pad_ranges.data_ptr()) if pad_ranges is not None else None, C.c_float(0.0 if scale is None else scale),
+             C.c_float(decay))
+    return out
 
 
 class _DenoiseAttnArgs(C.Structure):
