@@ -6,14 +6,18 @@
 // K Q^T puts keys on the lanes of TMEM and query rows on its columns: a thread owns one key and adds up its columns in
 // registers -- nothing is reduced across threads but the two halves of the columns, no atomics, the same bits every time.
 //
-// Work unit = (observation, kv head, 128 keys).  Persistent CTAs walk the units:
-//   loader warp      TMA: the unit's K tile through a ring of KS, its query rows in chunks of at most NQ through a ring of QS
-//   MMA warp         D[128 keys][n rows] = K_tile Q_chunk^T, n = the chunk's rows rounded up to 16 (one token: 16 columns), NB accumulators
+// Work unit = (observation, kv head, 256 keys) for a pair of CTAs (tcgen05 cta_group::2, M = 256): each holds 128 keys and stages half
+// of every chunk of query rows, so that an SM fetches half of what 128 keys of its own would need -- with a CTA per 128 keys the
+// fetching of query rows took 2,000 cycles per 128 of them, twice the exponentials.  Persistent pairs walk the units:
+//   loader warp      TMA: the unit's K tile and its query rows, chunks of at most NQ, through rings whose depths share 192 KB
+//   MMA warp         even CTA: D[256 keys][n rows] = K Q_chunk^T, n = the chunk's rows rounded up to 32 (one token: 32 columns), NB
+//                    accumulators; odd CTA: tells the even one what has landed
 //   8 sum warps      lane quarter = warp & 3, column half = warp >> 2: p = 2^(s c - lse'), two columns per FMA instruction
 //
-// One query token: K streams once, HBM bounds it.  Many: 16 exponentials per clock and SM (heads of 64 and 128) or the product (256).
+// One query token: K streams once, HBM bounds it.  Many: the exponentials (heads of 64 and 128) or the product (256).
 #include <cuda_bf16.h>
 
+#include "f32x2.cuh"
 #include "host_common.h"
 #include "tc5.cuh"
 
@@ -21,13 +25,14 @@ namespace vb {
 
 constexpr int KM_THREADS = 320;  // warps 0-7 sums, 8 loader, 9 MMA
 constexpr int KM_LOADER = 8, KM_MMA = 9;
+constexpr int KM_POLY = 1;  // of every four pairs of columns: powers of two on the FMA pipe instead of the exponential unit
 
 struct KeyMassParams {
     const float *lse;      // [n_obs][n_q][S]: an item's g * S rows in one piece
     const float *mass_in;  // [n_obs][n_kv][cap] or nullptr
     float *mass_out;
     const int32_t *lens, *pad;
-    int R, n_kv, cap, max_len, n_tiles, n_units, n_chunks, page0, box_rows;
+    int R, n_kv, cap, max_len, n_tiles, n_units, n_chunks, page0, box_rows, k_stages, q_stages;
     float scale_log2, decay;
     int *status;
 };
@@ -35,18 +40,17 @@ struct KeyMassParams {
 template <int HD>
 struct KeyMassSmem {
     static constexpr int CB = HD / 64;                // 64-element column blocks
-    static constexpr int NQ = HD == 256 ? 64 : 128;   // query rows per chunk
-    static constexpr int KS = HD == 128 ? 3 : 2, QS = 2;
-    static constexpr int NB = HD == 64 ? 2 : 4;       // accumulators
+    static constexpr int NQ = HD == 256 ? 128 : 256;  // query rows per chunk
+    static constexpr int NB = 512 / NQ;               // accumulators
+    static constexpr int MAX_STAGES = 6;
     static constexpr int K_BYTES = CB * 128 * 128;    // [CB][128 keys][128 B]
-    static constexpr int Q_BYTES = CB * NQ * 128;     // [CB][box_rows][128 B]
-    static constexpr int Q_OFF = KS * K_BYTES, BAR_OFF = Q_OFF + QS * Q_BYTES;
-    static constexpr int LSE_OFF = BAR_OFF + 256;     // float [2][8 warps][NQ / 2]
+    static constexpr int Q_BYTES = CB * (NQ / 2) * 128;  // [CB][box_rows][128 B]: this CTA's half of a chunk
+    static constexpr int RING = 192 * 1024;
+    static constexpr int BAR_OFF = RING;
+    static constexpr int LSE_OFF = BAR_OFF + 512;     // float [2][8 warps][NQ / 2]
     static constexpr int SUM_OFF = LSE_OFF + 2 * 8 * (NQ / 2) * 4;  // float [2][128]
     static constexpr int TOTAL = SUM_OFF + 2 * 128 * 4 + 1024;
-    static constexpr int TMEM_COLS = NB * NQ;
-    static_assert(TMEM_COLS == 256 || TMEM_COLS == 512, "TMEM");
-    static_assert(TOTAL <= 227 * 1024, "shared memory");
+    static_assert(2 * K_BYTES + 2 * Q_BYTES <= RING && TOTAL <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ float km_ex2(float x) {
@@ -55,43 +59,80 @@ __device__ __forceinline__ float km_ex2(float x) {
     return y;
 }
 
+// acc + 2^t for two columns on the FMA pipe: t = i + r with i the nearest whole number (left in the low bits of t + 1.5 2^23 + 127),
+// 2^r a polynomial of degree 5 fitted to [-1/2, 1/2] for the least relative error (1.5e-7 with these float32 coefficients), 2^i the
+// exponent bits.  Below 2^-126 the power is 0, above 2^127 it stops.
+__device__ __forceinline__ F2 km_add_ex2_poly(F2 t, F2 acc) {
+    float t0, t1;
+    f2_get(t, t0, t1);
+    t = f2(fminf(fmaxf(t0, -127.0f), 127.0f), fminf(fmaxf(t1, -127.0f), 127.0f));
+    const F2 whole = f2_add(t, f2(12583039.0f, 12583039.0f));
+    const F2 r = f2_add(t, f2_mul(f2_add(whole, f2(-12583039.0f, -12583039.0f)), f2(-1.0f, -1.0f)));
+    F2 y = f2(0.001327647129073739f, 0.001327647129073739f);
+    y = f2_fma(y, r, f2(0.009675540961325169f, 0.009675540961325169f));
+    y = f2_fma(y, r, f2(0.05550713092088699f, 0.05550713092088699f));
+    y = f2_fma(y, r, f2(0.24022120237350464f, 0.24022120237350464f));
+    y = f2_fma(y, r, f2(0.6931469440460205f, 0.6931469440460205f));
+    y = f2_fma(y, r, f2(1.0000001192092896f, 1.0000001192092896f));
+    float w0, w1;
+    f2_get(whole, w0, w1);
+    return f2_fma(y, f2(__uint_as_float(__float_as_uint(w0) << 23), __uint_as_float(__float_as_uint(w1) << 23)), acc);
+}
+
+// A stage of a ring and the parity its barriers are at.
+struct KmStage {
+    uint32_t i = 0, ph = 0;
+    __device__ __forceinline__ void next(uint32_t n) {
+        if (++i == n) {
+            i = 0;
+            ph ^= 1u;
+        }
+    }
+};
+
 template <int HD>
-__global__ void __launch_bounds__(KM_THREADS, HD == 64 ? 2 : 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KM_THREADS, 1)
 key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const KeyMassParams p) {
     using L = KeyMassSmem<HD>;
     extern __shared__ uint8_t km_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(km_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
-    uint64_t *k_full = bars, *k_free = bars + 3, *q_full = bars + 6, *q_free = bars + 8, *a_full = bars + 10, *a_free = bars + 14;
-    uint64_t *meet = bars + 18;  // [4] the two warps of a lane quarter
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
+    constexpr int MS = L::MAX_STAGES;
+    uint64_t *k_full = bars, *k_free = k_full + MS, *q_full = k_free + MS, *q_free = q_full + MS, *a_full = q_free + MS, *a_free = a_full + 4;
+    uint64_t *meet = a_free + 4;  // [4] the two warps of a lane quarter
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(meet + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
     const WaitCtx wc{abort_flag, p.status};
+    const uint32_t KS = p.k_stages, QS = p.q_stages;
+    const uint32_t both = rank == 0 ? 2u : 1u;  // even CTA: its own TMA and the odd CTA's word
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::KS; ++i) {
-            mbar_init(&k_full[i], 1);
+        for (int i = 0; i < MS; ++i) {
+            mbar_init(&k_full[i], both);
             mbar_init(&k_free[i], 1);
-        }
-        for (int i = 0; i < L::QS; ++i) {
-            mbar_init(&q_full[i], 1);
+            mbar_init(&q_full[i], both);
             mbar_init(&q_free[i], 1);
         }
-        for (int i = 0; i < L::NB; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&a_full[i], 1);
-            mbar_init(&a_free[i], 8);
+            mbar_init(&a_free[i], 16);  // the sum warps of both CTAs (used in the even one)
+            mbar_init(&meet[i], 64);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 64);
         *abort_flag = 0;
         fence_barrier_init();
     }
+    __syncthreads();
+    cluster_sync_all();
     if (warp == KM_MMA) {
-        tmem_alloc(tmem_slot, L::TMEM_COLS);
-        tmem_relinquish();
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     if (threadIdx.x == 0) {
@@ -103,120 +144,169 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 
     // the keys of an observation that are there; the same for every role
     auto len_of = [&](int obs) { return p.lens ? min(max(p.lens[obs], 0), p.max_len) : p.max_len; };
+    auto live_from = [&](int unit) {  // the first of this pair's units from here on that has keys
+        while (unit < p.n_units && unit % p.n_tiles * 256 >= len_of(unit / p.n_tiles / p.n_kv)) unit += ncl;
+        return unit;
+    };
+    auto columns_of = [&](int c) { return (min(p.R - c * L::NQ, L::NQ) + 31) & ~31; };
 
     if (warp == KM_LOADER) {
         if (lane == 0) {
-            uint32_t ku = 0, qu = 0;
+            KmStage k, q;
             bool ok = true;
-            const uint32_t q_tx = (uint32_t)(L::CB * p.box_rows * 128);
-            for (int unit = blockIdx.x; ok && unit < p.n_units; unit += gridDim.x) {
-                const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 128;
-                if (key0 >= len_of(item / p.n_kv)) continue;
-                const int ks = ku % L::KS;
-                ok = mbar_wait(&k_free[ks], (ku / L::KS & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+            const uint32_t q_stage = (uint32_t)(L::CB * p.box_rows * 128);
+            uint8_t *const q_smem = smem + KS * L::K_BYTES;
+            for (int unit = live_from(cid); ok && unit < p.n_units; unit = live_from(unit + ncl)) {
+                const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 256 + (int)rank * 128;
+                ok = mbar_wait(&k_free[k.i], k.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                 if (!ok) break;
-                mbar_expect_tx(&k_full[ks], L::K_BYTES);
+                mbar_expect_tx(&k_full[k.i], L::K_BYTES);
                 for (int cb = 0; cb < L::CB; ++cb)
-                    tma_load_3d(smem + ks * L::K_BYTES + cb * 16384, &k_map, &k_full[ks], cb * 64, key0, p.page0 + item);
-                ++ku;
-                for (int c = 0; c < p.n_chunks; ++c, ++qu) {
-                    const int qs = qu % L::QS;
-                    ok = mbar_wait(&q_free[qs], (qu / L::QS & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                    tma_load_3d(smem + k.i * L::K_BYTES + cb * 16384, &k_map, &k_full[k.i], cb * 64, key0, p.page0 + item);
+                k.next(KS);
+                for (int c = 0; c < p.n_chunks; ++c) {
+                    ok = mbar_wait(&q_free[q.i], q.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                     if (!ok) break;
-                    mbar_expect_tx(&q_full[qs], q_tx);
+                    mbar_expect_tx(&q_full[q.i], q_stage);
+                    const int row = c * L::NQ + (int)rank * (columns_of(c) >> 1);
                     for (int cb = 0; cb < L::CB; ++cb)
-                        tma_load_3d(smem + L::Q_OFF + qs * L::Q_BYTES + cb * p.box_rows * 128, &q_map, &q_full[qs], cb * 64, c * L::NQ, item);
+                        tma_load_3d(q_smem + q.i * q_stage + cb * p.box_rows * 128, &q_map, &q_full[q.i], cb * 64, row, item);
+                    q.next(QS);
                 }
             }
         }
     } else if (warp == KM_MMA) {
-        const uint32_t k_base = smem_u32(smem), q_base = k_base + L::Q_OFF;
-        const uint32_t q_cb = (uint32_t)p.box_rows * 128;
-        uint32_t ku = 0, qu = 0;
+        KmStage k, q, acc;
         bool ok = true;
-        for (int unit = blockIdx.x; ok && unit < p.n_units; unit += gridDim.x) {
-            const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 128;
-            if (key0 >= len_of(item / p.n_kv)) continue;
-            const uint32_t ks = ku % L::KS;
-            ok = warp_wait(&k_full[ks], ku / L::KS & 1u, wc, DEV_TIMEOUT_FULL);
-            if (!ok) break;
-            const uint32_t k_addr = k_base + ks * L::K_BYTES;
-            for (int c = 0; c < p.n_chunks; ++c, ++qu) {
-                const uint32_t qs = qu % L::QS, ab = qu % L::NB;
-                ok = warp_wait(&q_full[qs], qu / L::QS & 1u, wc, DEV_TIMEOUT_FULL);
-                if (ok) ok = warp_wait(&a_free[ab], (qu / L::NB & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+        if (rank == 0) {  // the whole warp walks the units, one elected lane issues
+            const uint32_t k_base = smem_u32(smem), q_base = k_base + KS * L::K_BYTES;
+            const uint32_t q_cb = (uint32_t)p.box_rows * 128, q_stage = L::CB * q_cb;
+            for (int unit = live_from(cid); ok && unit < p.n_units; unit = live_from(unit + ncl)) {
+                ok = warp_wait(&k_full[k.i], k.ph, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
-                tc_fence_after();
-                const int n = (min(p.R - c * L::NQ, L::NQ) + 15) & ~15;
-                const uint32_t idesc = make_idesc(1, 1, 1, 0, 0, 128, n);
-                const uint32_t q_addr = q_base + qs * L::Q_BYTES, d = tmem_base + ab * L::NQ;
-                if (elect_one()) {
+                const uint32_t k_addr = k_base + k.i * L::K_BYTES;
+                for (int c = 0; c < p.n_chunks; ++c) {
+                    ok = warp_wait(&q_full[q.i], q.ph, wc, DEV_TIMEOUT_FULL);
+                    if (ok) ok = warp_wait(&a_free[acc.i], acc.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t idesc = make_idesc(1, 1, 1, 0, 0, 256, columns_of(c));
+                    const uint32_t q_addr = q_base + q.i * q_stage, d = tmem_base + acc.i * L::NQ;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk)
-                        mma_f16(d, smem_desc_sw128(k_addr + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                                smem_desc_sw128(q_addr + (kk >> 2) * q_cb + (kk & 3) * 32, 16, 1024), idesc, kk != 0 ? 1u : 0u);
-                    tc_commit(&a_full[ab]);
-                    tc_commit(&q_free[qs]);
-                    if (c + 1 == p.n_chunks) tc_commit(&k_free[ks]);
+                        for (int kk = 0; kk < HD / 16; ++kk)
+                            mma_f16_pair(d, smem_desc_sw128(k_addr + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
+                                         smem_desc_sw128(q_addr + (kk >> 2) * q_cb + (kk & 3) * 32, 16, 1024), idesc, kk != 0 ? 1u : 0u);
+                        tc_commit_pair(&a_full[acc.i], 3);
+                        tc_commit_pair(&q_free[q.i], 3);
+                        if (c + 1 == p.n_chunks) tc_commit_pair(&k_free[k.i], 3);
+                    }
+                    q.next(QS);
+                    acc.next(L::NB);
+                }
+                k.next(KS);
+            }
+        } else if (lane == 0) {
+            for (int unit = live_from(cid); ok && unit < p.n_units; unit = live_from(unit + ncl)) {
+                ok = mbar_wait(&k_full[k.i], k.ph, wc, DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                mbar_arrive_cluster(&k_full[k.i], 0);
+                k.next(KS);
+                for (int c = 0; c < p.n_chunks; ++c) {
+                    ok = mbar_wait(&q_full[q.i], q.ph, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    mbar_arrive_cluster(&q_full[q.i], 0);
+                    q.next(QS);
                 }
             }
-            ++ku;
         }
     } else {
         const int qtr = warp & 3, half = warp >> 2;
-        constexpr int HALF = L::NQ / 2;  // columns of a chunk that this warp adds up
+        constexpr int HALF = L::NQ / 2, NBLK = HALF / 32;  // columns of a chunk that this warp adds up
         float *lse_s = reinterpret_cast<float *>(smem + L::LSE_OFF) + warp * HALF;
         float *sum_s = reinterpret_cast<float *>(smem + L::SUM_OFF);
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
+        const F2 scale2 = f2(p.scale_log2, p.scale_log2);
+        float lv[NBLK];  // the next chunk's lse, requested while this one is worked on
+        auto fetch_lse = [&](int unit, int c) {
+#pragma unroll
+            for (int i = 0; i < NBLK; ++i) {
+                const int r = c * L::NQ + half * HALF + i * 32 + lane;
+                lv[i] = unit < p.n_units && r < p.R ? p.lse[(long long)(unit / p.n_tiles) * p.R + r] : INFINITY;
+            }
+        };
         uint32_t qu = 0, un = 0;
+        KmStage ab;
         bool ok = true;
-        for (int unit = blockIdx.x; ok && unit < p.n_units; unit += gridDim.x) {
-            const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 128, obs = item / p.n_kv;
-            const int len = len_of(obs);
-            if (key0 >= len) continue;
-            const float *lse = p.lse + (long long)item * p.R;
-            float sum = 0.0f;
+        int unit = live_from(cid);
+        fetch_lse(unit, 0);
+        while (ok && unit < p.n_units) {
+            const int unit_next = live_from(unit + ncl);
+            const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 256 + (int)rank * 128, obs = item / p.n_kv;
+            F2 acc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = f2(0.0f, 0.0f);
             for (int c = 0; c < p.n_chunks; ++c, ++qu) {
-                const uint32_t ab = qu % L::NB;
                 // rows past the last, and rows that saw nothing (-inf), weigh nothing: 2^(s - inf)
                 float *ls = lse_s + (qu & 1u) * (8 * HALF);
 #pragma unroll
-                for (int i = 0; i < HALF / 32; ++i) {
-                    const int r = c * L::NQ + half * HALF + i * 32 + lane;
-                    const float v = r < p.R ? lse[r] : INFINITY;
-                    ls[i * 32 + lane] = v == -INFINITY ? -INFINITY : -1.4426950408889634f * v;
-                }
+                for (int i = 0; i < NBLK; ++i) ls[i * 32 + lane] = lv[i] == -INFINITY ? -INFINITY : -1.4426950408889634f * lv[i];
                 __syncwarp();
-                ok = mbar_wait(&a_full[ab], qu / L::NB & 1u, wc, DEV_TIMEOUT_ACCUM);
+                if (c + 1 < p.n_chunks) fetch_lse(unit, c + 1);
+                else fetch_lse(unit_next, 0);
+                ok = mbar_wait(&a_full[ab.i], ab.ph, wc, DEV_TIMEOUT_ACCUM);
                 if (!ok) break;
                 tc_fence_after();
                 const int n = min(p.R - c * L::NQ - half * HALF, HALF);  // of this warp's columns; may be 0 or less
-                float a0 = 0.0f, a1 = 0.0f;
+                const uint32_t d = tmem_base + lane_sel + ab.i * L::NQ + (uint32_t)(half * HALF);
 #pragma unroll
-                for (int b = 0; b < HALF / 32; ++b) {
-                    if (b * 32 >= n) break;
-                    uint32_t s[32];
-                    tmem_ld32(tmem_base + lane_sel + ab * L::NQ + (uint32_t)(half * HALF + b * 32), s);
+                for (int b0 = 0; b0 < NBLK; b0 += 2) {
+                    uint32_t s[2][32];
+                    if (b0 * 32 < n) tmem_ld32(d + (uint32_t)(b0 * 32), s[0]);
+                    if (b0 * 32 + 32 < n) tmem_ld32(d + (uint32_t)(b0 * 32 + 32), s[1]);
                     tmem_ld_wait();
-                    if (n < b * 32 + 32) {  // columns that no row stands behind hold anything
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = b * 32 + e < n ? s[e] : 0u;
+                    if (b0 + 2 == NBLK) {  // the accumulator is out of TMEM
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (rank == 0) mbar_arrive(&a_free[ab.i]);
+                            else mbar_arrive_cluster(&a_free[ab.i], 0);
+                        }
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 l4 = *reinterpret_cast<const float4 *>(ls + b * 32 + e);
-                        a0 += km_ex2(fmaf(__uint_as_float(s[e]), p.scale_log2, l4.x));
-                        a1 += km_ex2(fmaf(__uint_as_float(s[e + 1]), p.scale_log2, l4.y));
-                        a0 += km_ex2(fmaf(__uint_as_float(s[e + 2]), p.scale_log2, l4.z));
-                        a1 += km_ex2(fmaf(__uint_as_float(s[e + 3]), p.scale_log2, l4.w));
+                    for (int bb = 0; bb < 2; ++bb) {
+                        const int b = b0 + bb;
+                        if (b * 32 >= n) break;
+                        if (n < b * 32 + 32) {  // columns that no row stands behind hold anything
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) s[bb][e] = b * 32 + e < n ? s[bb][e] : 0u;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            const ulonglong2 la = *reinterpret_cast<const ulonglong2 *>(ls + b * 32 + e);
+                            const ulonglong2 lb = *reinterpret_cast<const ulonglong2 *>(ls + b * 32 + e + 4);
+                            const unsigned long long l[4] = {la.x, la.y, lb.x, lb.y};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const F2 t = f2_fma(f2(__uint_as_float(s[bb][e + 2 * i]), __uint_as_float(s[bb][e + 2 * i + 1])), scale2, F2{l[i]});
+                                if (i < KM_POLY) {
+                                    acc[i] = km_add_ex2_poly(t, acc[i]);
+                                } else {
+                                    float t0, t1;
+                                    f2_get(t, t0, t1);
+                                    acc[i] = f2_add(acc[i], f2(km_ex2(t0), km_ex2(t1)));
+                                }
+                            }
+                        }
                     }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&a_free[ab]);
-                sum += a0 + a1;
+                ab.next(L::NB);
             }
             if (!ok) break;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f2_get(acc[i], x[2 * i], x[2 * i + 1]);
+            float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             // the two halves of the columns meet; the slots are used in turn, so one meeting per unit is enough
             float *slot = sum_s + (un & 1u) * 128;
             if (half) slot[qtr * 32 + lane] = sum;
@@ -225,19 +315,21 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             if (!ok) break;
             ++un;
             const int key = key0 + qtr * 32 + lane;
-            if (!half && key < len) {
+            if (!half && key < len_of(obs)) {
                 sum += slot[qtr * 32 + lane];
                 if (p.pad && key >= p.pad[2 * obs] && key < p.pad[2 * obs + 1]) sum = 0.0f;
                 const long long at = (long long)item * p.cap + key;
                 p.mass_out[at] = p.mass_in ? fmaf(p.decay, p.mass_in[at], sum) : sum;
             }
+            unit = unit_next;
         }
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync_all();  // neither CTA may exit while the other can still signal its barriers
     if (warp == KM_MMA) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, L::TMEM_COLS);
+        tmem_dealloc_pair(tmem_base, 512);
     }
 }
 
@@ -245,7 +337,13 @@ template <int HD>
 static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassParams &p, cudaStream_t stream) {
     using L = KeyMassSmem<HD>;
     p.n_chunks = (p.R + L::NQ - 1) / L::NQ;
-    p.box_rows = p.R >= L::NQ ? L::NQ : (p.R + 15) & ~15;
+    p.box_rows = p.R >= L::NQ ? L::NQ / 2 : ((p.R + 31) & ~31) / 2;  // a multiple of 8: whole swizzle groups
+    // A unit that takes its query rows in one chunk streams keys: the ring goes to K.  More chunks: K stays, query rows stream.
+    const int q_stage = L::CB * p.box_rows * 128;
+    p.q_stages = p.n_chunks == 1 ? 2 : (L::RING - 2 * L::K_BYTES) / q_stage;
+    if (p.q_stages > L::MAX_STAGES) p.q_stages = L::MAX_STAGES;
+    p.k_stages = (L::RING - p.q_stages * q_stage) / L::K_BYTES;
+    if (p.k_stages > L::MAX_STAGES) p.k_stages = L::MAX_STAGES;
     CUtensorMap qmap, kmap;
     {
         const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)p.R, (uint64_t)st->n_obs * st->n_kv};
@@ -261,8 +359,8 @@ static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassPar
             return rc;
     }
     if (int rc = ensure_dyn_smem(key_mass_kernel<HD>, L::TOTAL)) return rc;
-    const int slots = (HD == 64 ? 2 : 1) * sm_count();
-    return launch_pdl(key_mass_kernel<HD>, dim3(p.n_units < slots ? p.n_units : slots), dim3(KM_THREADS), L::TOTAL, stream, qmap, kmap, p);
+    const int pairs = sm_count() / 2;
+    return launch_pdl(key_mass_kernel<HD>, dim3(2 * (p.n_units < pairs ? p.n_units : pairs)), dim3(KM_THREADS), L::TOTAL, stream, qmap, kmap, p);
 }
 
 }  // namespace vb
@@ -276,7 +374,7 @@ extern "C" int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, c
     if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(st->k_pages) & 15)) return VLAB200_ERR_ARG;
     const int hd = st->head_dim;
     if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
-    const long long R = (long long)(n_q / st->n_kv) * S, tiles = (max_len + 127LL) / 128, units = (long long)st->n_obs * st->n_kv * tiles;
+    const long long R = (long long)(n_q / st->n_kv) * S, tiles = (max_len + 255LL) / 256, units = (long long)st->n_obs * st->n_kv * tiles;
     if (R > 0x7fffff00LL || units > 0x7fffff00LL || (long long)st->n_layers * st->n_obs * st->n_kv > 0x7fffff00LL) {
         vb::set_last_error("key_mass: more than 2^31 query rows per kv head, pages or key tiles");
         return VLAB200_ERR_UNSUPPORTED;

@@ -14,6 +14,7 @@
 
 #include <cmath>
 
+#include "f32x2.cuh"
 #include "host_common.h"
 #include "tc5.cuh"
 
@@ -34,33 +35,6 @@ struct RopeNormParams {
 };
 
 enum : int { ROPE_PAIRS = 0, ROPE_HALF_LANES = 1, ROPE_HALF_ANY = 2 };
-
-// Two float32 per register pair: one instruction of the FMA pipe serves both.
-struct F2 {
-    unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void f2_get(F2 a, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ uint32_t f2_bf16(F2 a) {
-    float lo, hi;
-    f2_get(a, lo, hi);
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 
 // 8 columns of a lane
 template <bool F32>
