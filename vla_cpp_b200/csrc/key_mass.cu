@@ -19,6 +19,7 @@
 
 #include "f32x2.cuh"
 #include "host_common.h"
+#include "ragged.cuh"
 #include "tc5.cuh"
 
 namespace vb {
@@ -32,7 +33,7 @@ struct KeyMassParams {
     const float *mass_in;  // [n_obs][n_kv][cap] or nullptr
     float *mass_out;
     const int32_t *lens, *pad;
-    int R, n_kv, cap, max_len, n_tiles, n_units, n_chunks, page0, box_rows, k_stages, q_stages;
+    int R, n_obs, n_kv, cap, max_len, n_chunks, page0, box_rows, k_stages, q_stages;
     float scale_log2, decay;
     int *status;
 };
@@ -144,35 +145,35 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 
     // the keys of an observation that are there; the same for every role
     auto len_of = [&](int obs) { return p.lens ? min(max(p.lens[obs], 0), p.max_len) : p.max_len; };
-    auto live_from = [&](int unit) {  // the first of this pair's units from here on that has keys
-        while (unit < p.n_units && unit % p.n_tiles * 256 >= len_of(unit / p.n_tiles / p.n_kv)) unit += ncl;
-        return unit;
-    };
+    RaggedCursor cursor(len_of, p.n_obs, p.n_kv, 256);
+    RaggedUnit unit;
     auto columns_of = [&](int c) { return (min(p.R - c * L::NQ, L::NQ) + 31) & ~31; };
 
     if (warp == KM_LOADER) {
-        if (lane == 0) {
-            KmStage k, q;
-            bool ok = true;
-            const uint32_t q_stage = (uint32_t)(L::CB * p.box_rows * 128);
-            uint8_t *const q_smem = smem + KS * L::K_BYTES;
-            for (int unit = live_from(cid); ok && unit < p.n_units; unit = live_from(unit + ncl)) {
-                const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 256 + (int)rank * 128;
-                ok = mbar_wait(&k_free[k.i], k.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
-                if (!ok) break;
+        KmStage k, q;
+        bool ok = true;
+        const uint32_t q_stage = (uint32_t)(L::CB * p.box_rows * 128);
+        uint8_t *const q_smem = smem + KS * L::K_BYTES;
+        for (int ui = cid; ok && cursor.find(ui, unit); ui += ncl) {
+            const int item = unit.obs * p.n_kv + unit.kvh, key0 = unit.block * 256 + (int)rank * 128;
+            ok = warp_wait(&k_free[k.i], k.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+            if (!ok) break;
+            if (elect_one()) {
                 mbar_expect_tx(&k_full[k.i], L::K_BYTES);
                 for (int cb = 0; cb < L::CB; ++cb)
                     tma_load_3d(smem + k.i * L::K_BYTES + cb * 16384, &k_map, &k_full[k.i], cb * 64, key0, p.page0 + item);
-                k.next(KS);
-                for (int c = 0; c < p.n_chunks; ++c) {
-                    ok = mbar_wait(&q_free[q.i], q.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
-                    if (!ok) break;
+            }
+            k.next(KS);
+            for (int c = 0; c < p.n_chunks; ++c) {
+                ok = warp_wait(&q_free[q.i], q.ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                if (elect_one()) {
                     mbar_expect_tx(&q_full[q.i], q_stage);
                     const int row = c * L::NQ + (int)rank * (columns_of(c) >> 1);
                     for (int cb = 0; cb < L::CB; ++cb)
                         tma_load_3d(q_smem + q.i * q_stage + cb * p.box_rows * 128, &q_map, &q_full[q.i], cb * 64, row, item);
-                    q.next(QS);
                 }
+                q.next(QS);
             }
         }
     } else if (warp == KM_MMA) {
@@ -181,7 +182,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         if (rank == 0) {  // the whole warp walks the units, one elected lane issues
             const uint32_t k_base = smem_u32(smem), q_base = k_base + KS * L::K_BYTES;
             const uint32_t q_cb = (uint32_t)p.box_rows * 128, q_stage = L::CB * q_cb;
-            for (int unit = live_from(cid); ok && unit < p.n_units; unit = live_from(unit + ncl)) {
+            for (int ui = cid; ok && cursor.find(ui, unit); ui += ncl) {
                 ok = warp_wait(&k_full[k.i], k.ph, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
                 const uint32_t k_addr = k_base + k.i * L::K_BYTES;
@@ -206,16 +207,16 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                 }
                 k.next(KS);
             }
-        } else if (lane == 0) {
-            for (int unit = live_from(cid); ok && unit < p.n_units; unit = live_from(unit + ncl)) {
-                ok = mbar_wait(&k_full[k.i], k.ph, wc, DEV_TIMEOUT_FULL);
+        } else {
+            for (int ui = cid; ok && cursor.find(ui, unit); ui += ncl) {
+                ok = warp_wait(&k_full[k.i], k.ph, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
-                mbar_arrive_cluster(&k_full[k.i], 0);
+                if (lane == 0) mbar_arrive_cluster(&k_full[k.i], 0);
                 k.next(KS);
                 for (int c = 0; c < p.n_chunks; ++c) {
-                    ok = mbar_wait(&q_full[q.i], q.ph, wc, DEV_TIMEOUT_FULL);
+                    ok = warp_wait(&q_full[q.i], q.ph, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
-                    mbar_arrive_cluster(&q_full[q.i], 0);
+                    if (lane == 0) mbar_arrive_cluster(&q_full[q.i], 0);
                     q.next(QS);
                 }
             }
@@ -228,21 +229,24 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
         float lv[NBLK];  // the next chunk's lse, requested while this one is worked on
-        auto fetch_lse = [&](int unit, int c) {
+        auto fetch_lse = [&](bool there, const RaggedUnit &u, int c) {
 #pragma unroll
             for (int i = 0; i < NBLK; ++i) {
                 const int r = c * L::NQ + half * HALF + i * 32 + lane;
-                lv[i] = unit < p.n_units && r < p.R ? p.lse[(long long)(unit / p.n_tiles) * p.R + r] : INFINITY;
+                lv[i] = there && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : INFINITY;
             }
         };
         uint32_t qu = 0, un = 0;
         KmStage ab;
         bool ok = true;
-        int unit = live_from(cid);
-        fetch_lse(unit, 0);
-        while (ok && unit < p.n_units) {
-            const int unit_next = live_from(unit + ncl);
-            const int item = unit / p.n_tiles, key0 = unit % p.n_tiles * 256 + (int)rank * 128, obs = item / p.n_kv;
+        int ui = cid;
+        bool there = cursor.find(ui, unit);
+        fetch_lse(there, unit, 0);
+        while (ok && there) {
+            const RaggedUnit now = unit;
+            ui += ncl;
+            there = cursor.find(ui, unit);
+            const int item = now.obs * p.n_kv + now.kvh, key0 = now.block * 256 + (int)rank * 128, obs = now.obs;
             F2 acc[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i] = f2(0.0f, 0.0f);
@@ -252,8 +256,8 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 #pragma unroll
                 for (int i = 0; i < NBLK; ++i) ls[i * 32 + lane] = lv[i] == -INFINITY ? -INFINITY : -1.4426950408889634f * lv[i];
                 __syncwarp();
-                if (c + 1 < p.n_chunks) fetch_lse(unit, c + 1);
-                else fetch_lse(unit_next, 0);
+                if (c + 1 < p.n_chunks) fetch_lse(true, now, c + 1);
+                else fetch_lse(there, unit, 0);
                 ok = mbar_wait(&a_full[ab.i], ab.ph, wc, DEV_TIMEOUT_ACCUM);
                 if (!ok) break;
                 tc_fence_after();
@@ -276,7 +280,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 #pragma unroll
                     for (int bb = 0; bb < 2; ++bb) {
                         const int b = b0 + bb;
-                        if (b * 32 >= n) break;
+                        if (b * 32 >= n) continue;
                         if (n < b * 32 + 32) {  // columns that no row stands behind hold anything
 #pragma unroll
                             for (int e = 0; e < 32; ++e) s[bb][e] = b * 32 + e < n ? s[bb][e] : 0u;
@@ -315,13 +319,12 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             if (!ok) break;
             ++un;
             const int key = key0 + qtr * 32 + lane;
-            if (!half && key < len_of(obs)) {
+            if (!half && key < now.len) {
                 sum += slot[qtr * 32 + lane];
                 if (p.pad && key >= p.pad[2 * obs] && key < p.pad[2 * obs + 1]) sum = 0.0f;
                 const long long at = (long long)item * p.cap + key;
                 p.mass_out[at] = p.mass_in ? fmaf(p.decay, p.mass_in[at], sum) : sum;
             }
-            unit = unit_next;
         }
     }
     tc_fence_before();
@@ -334,7 +337,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 }
 
 template <int HD>
-static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassParams &p, cudaStream_t stream) {
+static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassParams &p, int max_units, cudaStream_t stream) {
     using L = KeyMassSmem<HD>;
     p.n_chunks = (p.R + L::NQ - 1) / L::NQ;
     p.box_rows = p.R >= L::NQ ? L::NQ / 2 : ((p.R + 31) & ~31) / 2;  // a multiple of 8: whole swizzle groups
@@ -360,7 +363,7 @@ static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassPar
     }
     if (int rc = ensure_dyn_smem(key_mass_kernel<HD>, L::TOTAL)) return rc;
     const int pairs = sm_count() / 2;
-    return launch_pdl(key_mass_kernel<HD>, dim3(2 * (p.n_units < pairs ? p.n_units : pairs)), dim3(KM_THREADS), L::TOTAL, stream, qmap, kmap, p);
+    return launch_pdl(key_mass_kernel<HD>, dim3(2 * (max_units < pairs ? max_units : pairs)), dim3(KM_THREADS), L::TOTAL, stream, qmap, kmap, p);
 }
 
 }  // namespace vb
@@ -390,15 +393,14 @@ extern "C" int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, c
     p.n_kv = st->n_kv;
     p.cap = st->cap;
     p.max_len = max_len;
-    p.n_tiles = (int)tiles;
-    p.n_units = (int)units;
+    p.n_obs = st->n_obs;
     p.page0 = layer * st->n_obs * st->n_kv;
     p.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)hd));
     p.decay = decay;
     p.status = vb::device_status_ptr();
     if (!p.status) return vb::cuda_fail(cudaGetLastError(), "device_status_ptr");
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (hd == 64) return vb::launch_key_mass<64>(st, q, p, cs);
-    if (hd == 128) return vb::launch_key_mass<128>(st, q, p, cs);
-    return vb::launch_key_mass<256>(st, q, p, cs);
+    if (hd == 64) return vb::launch_key_mass<64>(st, q, p, (int)units, cs);
+    if (hd == 128) return vb::launch_key_mass<128>(st, q, p, (int)units, cs);
+    return vb::launch_key_mass<256>(st, q, p, (int)units, cs);
 }
