@@ -4,7 +4,7 @@
 //
 // with the log-sum-exp of each query row given, so a row's weights need neither its maximum nor its sum.  The transposed product
 // K Q^T puts keys on the lanes of TMEM and query rows on its columns: a thread owns one key and adds up its columns in
-// registers -- nothing is reduced across threads but the two halves of the columns, no atomics, the same bits every time.
+// registers -- nothing is reduced across threads but the parts of the columns, no atomics, the same bits every time.
 //
 // Work unit = (observation, kv head, 256 keys) for a pair of CTAs (tcgen05 cta_group::2, M = 256): each holds 128 keys and stages half
 // of every chunk of query rows, so that an SM fetches half of what 128 keys of its own would need -- with a CTA per 128 keys the
@@ -12,7 +12,7 @@
 //   loader warp      TMA: the unit's K tile and its query rows, chunks of at most NQ, through rings whose depths share 192 KB
 //   MMA warp         even CTA: D[256 keys][n rows] = K Q_chunk^T, n = the chunk's rows rounded up to 32 (one token: 32 columns), NB
 //                    accumulators; odd CTA: tells the even one what has landed
-//   8 sum warps      lane quarter = warp & 3, column half = warp >> 2: p = 2^(s c - lse'), two columns per FMA instruction
+//   16 sum warps     lane quarter = warp & 3, a quarter of the columns = warp >> 2: p = 2^(s c - lse'), two columns per FMA instruction
 //
 // One query token: K streams once, HBM bounds it.  Many: the exponentials (heads of 64 and 128) or the product (256).
 #include <cuda_bf16.h>
@@ -24,9 +24,8 @@
 
 namespace vb {
 
-constexpr int KM_THREADS = 320;  // warps 0-7 sums, 8 loader, 9 MMA
-constexpr int KM_LOADER = 8, KM_MMA = 9;
-constexpr int KM_POLY = 1;  // of every four pairs of columns: powers of two on the FMA pipe instead of the exponential unit
+constexpr int KM_PARTS = 4;  // sum warps per lane quarter: each takes NQ / KM_PARTS columns of a chunk
+constexpr int KM_SUMS = 4 * KM_PARTS, KM_LOADER = KM_SUMS, KM_MMA = KM_SUMS + 1, KM_THREADS = 32 * (KM_SUMS + 2);
 
 struct KeyMassParams {
     const float *lse;      // [n_obs][n_q][S]: an item's g * S rows in one piece
@@ -48,9 +47,10 @@ struct KeyMassSmem {
     static constexpr int Q_BYTES = CB * (NQ / 2) * 128;  // [CB][box_rows][128 B]: this CTA's half of a chunk
     static constexpr int RING = 192 * 1024;
     static constexpr int BAR_OFF = RING;
-    static constexpr int LSE_OFF = BAR_OFF + 512;     // float [2][8 warps][NQ / 2]
-    static constexpr int SUM_OFF = LSE_OFF + 2 * 8 * (NQ / 2) * 4;  // float [2][128]
-    static constexpr int TOTAL = SUM_OFF + 2 * 128 * 4 + 1024;
+    static constexpr int PART = NQ / KM_PARTS;        // columns of a sum warp
+    static constexpr int LSE_OFF = BAR_OFF + 512;     // float [2][KM_SUMS][PART]
+    static constexpr int SUM_OFF = LSE_OFF + 2 * KM_SUMS * PART * 4;  // float [2][KM_PARTS - 1][128]
+    static constexpr int TOTAL = SUM_OFF + 2 * (KM_PARTS - 1) * 128 * 4 + 1024;
     static_assert(2 * K_BYTES + 2 * Q_BYTES <= RING && TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -58,26 +58,6 @@ __device__ __forceinline__ float km_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-// acc + 2^t for two columns on the FMA pipe: t = i + r with i the nearest whole number (left in the low bits of t + 1.5 2^23 + 127),
-// 2^r a polynomial of degree 5 fitted to [-1/2, 1/2] for the least relative error (1.5e-7 with these float32 coefficients), 2^i the
-// exponent bits.  Below 2^-126 the power is 0, above 2^127 it stops.
-__device__ __forceinline__ F2 km_add_ex2_poly(F2 t, F2 acc) {
-    float t0, t1;
-    f2_get(t, t0, t1);
-    t = f2(fminf(fmaxf(t0, -127.0f), 127.0f), fminf(fmaxf(t1, -127.0f), 127.0f));
-    const F2 whole = f2_add(t, f2(12583039.0f, 12583039.0f));
-    const F2 r = f2_add(t, f2_mul(f2_add(whole, f2(-12583039.0f, -12583039.0f)), f2(-1.0f, -1.0f)));
-    F2 y = f2(0.001327647129073739f, 0.001327647129073739f);
-    y = f2_fma(y, r, f2(0.009675540961325169f, 0.009675540961325169f));
-    y = f2_fma(y, r, f2(0.05550713092088699f, 0.05550713092088699f));
-    y = f2_fma(y, r, f2(0.24022120237350464f, 0.24022120237350464f));
-    y = f2_fma(y, r, f2(0.6931469440460205f, 0.6931469440460205f));
-    y = f2_fma(y, r, f2(1.0000001192092896f, 1.0000001192092896f));
-    float w0, w1;
-    f2_get(whole, w0, w1);
-    return f2_fma(y, f2(__uint_as_float(__float_as_uint(w0) << 23), __uint_as_float(__float_as_uint(w1) << 23)), acc);
 }
 
 // A stage of a ring and the parity its barriers are at.
@@ -100,7 +80,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
     constexpr int MS = L::MAX_STAGES;
     uint64_t *k_full = bars, *k_free = k_full + MS, *q_full = k_free + MS, *q_free = q_full + MS, *a_full = q_free + MS, *a_free = a_full + 4;
-    uint64_t *meet = a_free + 4;  // [4] the two warps of a lane quarter
+    uint64_t *meet = a_free + 4;  // [4] the warps of a lane quarter
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(meet + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -119,8 +99,8 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&a_full[i], 1);
-            mbar_init(&a_free[i], 16);  // the sum warps of both CTAs (used in the even one)
-            mbar_init(&meet[i], 64);
+            mbar_init(&a_free[i], 2 * KM_SUMS);  // the sum warps of both CTAs (used in the even one)
+            mbar_init(&meet[i], 32 * KM_PARTS);
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -222,9 +202,9 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             }
         }
     } else {
-        const int qtr = warp & 3, half = warp >> 2;
-        constexpr int HALF = L::NQ / 2, NBLK = HALF / 32;  // columns of a chunk that this warp adds up
-        float *lse_s = reinterpret_cast<float *>(smem + L::LSE_OFF) + warp * HALF;
+        const int qtr = warp & 3, part = warp >> 2;
+        constexpr int PART = L::PART, NBLK = PART / 32;
+        float *lse_s = reinterpret_cast<float *>(smem + L::LSE_OFF) + warp * PART;
         float *sum_s = reinterpret_cast<float *>(smem + L::SUM_OFF);
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
@@ -232,7 +212,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         auto fetch_lse = [&](bool there, const RaggedUnit &u, int c) {
 #pragma unroll
             for (int i = 0; i < NBLK; ++i) {
-                const int r = c * L::NQ + half * HALF + i * 32 + lane;
+                const int r = c * L::NQ + part * PART + i * 32 + lane;
                 lv[i] = there && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : INFINITY;
             }
         };
@@ -252,7 +232,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             for (int i = 0; i < 4; ++i) acc[i] = f2(0.0f, 0.0f);
             for (int c = 0; c < p.n_chunks; ++c, ++qu) {
                 // rows past the last, and rows that saw nothing (-inf), weigh nothing: 2^(s - inf)
-                float *ls = lse_s + (qu & 1u) * (8 * HALF);
+                float *ls = lse_s + (qu & 1u) * (KM_SUMS * PART);
 #pragma unroll
                 for (int i = 0; i < NBLK; ++i) ls[i * 32 + lane] = lv[i] == -INFINITY ? -INFINITY : -1.4426950408889634f * lv[i];
                 __syncwarp();
@@ -261,15 +241,16 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                 ok = mbar_wait(&a_full[ab.i], ab.ph, wc, DEV_TIMEOUT_ACCUM);
                 if (!ok) break;
                 tc_fence_after();
-                const int n = min(p.R - c * L::NQ - half * HALF, HALF);  // of this warp's columns; may be 0 or less
-                const uint32_t d = tmem_base + lane_sel + ab.i * L::NQ + (uint32_t)(half * HALF);
+                const int n = min(p.R - c * L::NQ - part * PART, PART);  // of this warp's columns; may be 0 or less
+                const uint32_t d = tmem_base + lane_sel + ab.i * L::NQ + (uint32_t)(part * PART);
 #pragma unroll
-                for (int b0 = 0; b0 < NBLK; b0 += 2) {
-                    uint32_t s[2][32];
-                    if (b0 * 32 < n) tmem_ld32(d + (uint32_t)(b0 * 32), s[0]);
-                    if (b0 * 32 + 32 < n) tmem_ld32(d + (uint32_t)(b0 * 32 + 32), s[1]);
-                    tmem_ld_wait();
-                    if (b0 + 2 == NBLK) {  // the accumulator is out of TMEM
+                for (int b = 0; b < NBLK; ++b) {
+                    uint32_t s[32];
+                    if (b * 32 < n) {
+                        tmem_ld32(d + (uint32_t)(b * 32), s);
+                        tmem_ld_wait();
+                    }
+                    if (b + 1 == NBLK) {  // the accumulator is out of TMEM
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -277,30 +258,22 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                             else mbar_arrive_cluster(&a_free[ab.i], 0);
                         }
                     }
+                    if (b * 32 >= n) continue;
+                    if (n < b * 32 + 32) {  // columns that no row stands behind hold anything
 #pragma unroll
-                    for (int bb = 0; bb < 2; ++bb) {
-                        const int b = b0 + bb;
-                        if (b * 32 >= n) continue;
-                        if (n < b * 32 + 32) {  // columns that no row stands behind hold anything
+                        for (int e = 0; e < 32; ++e) s[e] = b * 32 + e < n ? s[e] : 0u;
+                    }
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) s[bb][e] = b * 32 + e < n ? s[bb][e] : 0u;
-                        }
+                    for (int e = 0; e < 32; e += 8) {
+                        const ulonglong2 la = *reinterpret_cast<const ulonglong2 *>(ls + b * 32 + e);
+                        const ulonglong2 lb = *reinterpret_cast<const ulonglong2 *>(ls + b * 32 + e + 4);
+                        const unsigned long long l[4] = {la.x, la.y, lb.x, lb.y};
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            const ulonglong2 la = *reinterpret_cast<const ulonglong2 *>(ls + b * 32 + e);
-                            const ulonglong2 lb = *reinterpret_cast<const ulonglong2 *>(ls + b * 32 + e + 4);
-                            const unsigned long long l[4] = {la.x, la.y, lb.x, lb.y};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const F2 t = f2_fma(f2(__uint_as_float(s[bb][e + 2 * i]), __uint_as_float(s[bb][e + 2 * i + 1])), scale2, F2{l[i]});
-                                if (i < KM_POLY) {
-                                    acc[i] = km_add_ex2_poly(t, acc[i]);
-                                } else {
-                                    float t0, t1;
-                                    f2_get(t, t0, t1);
-                                    acc[i] = f2_add(acc[i], f2(km_ex2(t0), km_ex2(t1)));
-                                }
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            const F2 t = f2_fma(f2(__uint_as_float(s[e + 2 * i]), __uint_as_float(s[e + 2 * i + 1])), scale2, F2{l[i]});
+                            float t0, t1;
+                            f2_get(t, t0, t1);
+                            acc[i] = f2_add(acc[i], f2(km_ex2(t0), km_ex2(t1)));
                         }
                     }
                 }
@@ -311,16 +284,17 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 4; ++i) f2_get(acc[i], x[2 * i], x[2 * i + 1]);
             float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            // the two halves of the columns meet; the slots are used in turn, so one meeting per unit is enough
-            float *slot = sum_s + (un & 1u) * 128;
-            if (half) slot[qtr * 32 + lane] = sum;
+            // the parts of the columns meet; the slots are used in turn, so one meeting per unit is enough
+            float *slot = sum_s + (un & 1u) * ((KM_PARTS - 1) * 128) + qtr * 32 + lane;
+            if (part) slot[(part - 1) * 128] = sum;
             mbar_arrive(&meet[qtr]);
             ok = mbar_wait(&meet[qtr], un & 1u, wc, DEV_TIMEOUT_MISC);
             if (!ok) break;
             ++un;
             const int key = key0 + qtr * 32 + lane;
-            if (!half && key < now.len) {
-                sum += slot[qtr * 32 + lane];
+            if (!part && key < now.len) {
+#pragma unroll
+                for (int i = 0; i < KM_PARTS - 1; ++i) sum += slot[i * 128];
                 if (p.pad && key >= p.pad[2 * obs] && key < p.pad[2 * obs + 1]) sum = 0.0f;
                 const long long at = (long long)item * p.cap + key;
                 p.mass_out[at] = p.mass_in ? fmaf(p.decay, p.mass_in[at], sum) : sum;
