@@ -219,6 +219,20 @@ VLAB200_API int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, 
                                      float *mass_out, int32_t S, int32_t n_q, const int32_t *lens, int32_t max_len,
                                      const int32_t *pad_ranges, float scale, float decay, void *stream);
 
+/* Eviction from a cache by accumulated attention weight: of the first n = lens[b] rows of every page of `src` (layer, observation, kv
+ * head) the min(n, keep) that matter most are copied, in their order, to rows 0 .. of the same page of `dst`: the first `sink` and the last
+ * `recent` rows in any case (sink + recent <= keep), then those of largest weight in mass (float32 [n_layers][n_obs][n_kv][src cap]), ties to
+ * the lower row, weights that are no number last.  Protected rows that overlap (n < sink + recent) count once.
+ * kept: int32 [n_layers][n_obs][n_kv][keep], the rows' indices in src, then -1.  mass_out (optional): float32
+ * [n_layers][n_obs][n_kv][dst cap], their weights, then 0.  lens_out (optional): int32 [n_obs], min(n, keep).  Rows of dst behind
+ * them are left as they were.  lens: int32 [n_obs], taken into [0, max_len], or NULL (max_len); max_len <= src cap, keep <= dst cap.  The
+ * stores differ in nothing but cap and prefix_len, and no buffer that is written may overlap another of the call (VLAB200_ERR_ARG).
+ * A store of keep + suffix rows with prefix_len = keep then serves the calls above as the larger one did, with the suffix at its old
+ * positions.  No counterpart in the reference. */
+VLAB200_API int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_kv_store *dst, const float *mass, const int32_t *lens,
+                                     int32_t max_len, int32_t keep, int32_t sink, int32_t recent, int32_t *kept, float *mass_out,
+                                     int32_t *lens_out, void *stream);
+
 /* ------------------------------------------------------------- whole denoise loop (engine) */
 
 /* Shape of a flow-matching policy's action expert (fields follow vla_config of include/vla.h:59-96

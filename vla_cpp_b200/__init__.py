@@ -26,6 +26,7 @@ from .api import (  # noqa: F401
     device_status,
     fold_norm_weight,
     key_mass,
+    kv_evict,
     lib,
     node_bin,
     node_mul_mat,

@@ -77,7 +77,7 @@ EXPORTS = [
     "vlab200_qkv_rope_append",
     "vlab200_attention", "vlab200_denoise_attn_loop", "vlab200_denoise_attn_loop_host",
     "vlab200_denoise_attn_loop_static",
-    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append", "vlab200_key_mass",
+    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append", "vlab200_key_mass", "vlab200_kv_evict",
     "vlab200_engine_create", "vlab200_engine_free", "vlab200_engine_set_prefix", "vlab200_engine_denoise",
     "vlab200_engine_denoise_host", "vlab200_engine_run_stage", "vlab200_engine_set_prefix_len",
     "vlab200_engine_loop_phases", "vlab200_loop_kernel_phases",
@@ -397,6 +397,42 @@ def key_mass(store, layer, q, lse, lens=None, max_len=None, pad_ranges=None, sca
              C.c_void_p(pad_ranges.data_ptr()) if pad_ranges is not None else None, C.c_float(0.0 if scale is None else scale),
              C.c_float(decay))
     return out
+
+
+def kv_evict(src, dst, mass, keep, lens=None, max_len=None, sink=0, recent=0, mass_out=None, kept=None, lens_out=None):
+    """Copies the `keep` heaviest rows of every page of src, in their order, to the front of dst's pages.
+
+    mass: f32 [n_layers, n_obs, n_kv, src.cap] (key_mass per layer); lens: int32 [n_obs] rows of every observation or None (max_len, by
+    default src.cap); the first `sink` and last `recent` rows stay in any case.  mass_out: f32 [n_layers, n_obs, n_kv, dst.cap], kept: int32
+    [n_layers, n_obs, n_kv, keep] (indices in src, then -1) and lens_out: int32 [n_obs] are allocated where they are None.
+    Returns (lens_out, kept, mass_out)."""
+    import torch
+
+    dev = src.k.get_device()
+    pages = (src.n_layers, src.n_obs, src.n_kv)
+    if dst.k.get_device() != dev:
+        raise VlaB200Error(ERR_ARG, f"the stores are on {src.k.device} and {dst.k.device}")
+    if keep <= 0:
+        raise VlaB200Error(ERR_ARG, f"keep: {keep} rows")
+    _need_tensor(mass, "mass", torch.float32, (*pages, src.cap), dev)
+    if lens is not None:
+        _need_tensor(lens, "lens", torch.int32, (src.n_obs,), dev)
+    if mass_out is None:
+        mass_out = torch.empty((*pages, dst.cap), dtype=torch.float32, device=src.k.device)
+    else:
+        _need_tensor(mass_out, "mass_out", torch.float32, (*pages, dst.cap), dev)
+    if kept is None:
+        kept = torch.empty((*pages, keep), dtype=torch.int32, device=src.k.device)
+    else:
+        _need_tensor(kept, "kept", torch.int32, (*pages, keep), dev)
+    if lens_out is None:
+        lens_out = torch.empty((src.n_obs,), dtype=torch.int32, device=src.k.device)
+    else:
+        _need_tensor(lens_out, "lens_out", torch.int32, (src.n_obs,), dev)
+    _call_on(dev, lib().vlab200_kv_evict, "vlab200_kv_evict", C.byref(src.c), C.byref(dst.c), C.c_void_p(mass.data_ptr()),
+             C.c_void_p(lens.data_ptr()) if lens is not None else None, src.cap if max_len is None else max_len, keep, sink, recent,
+             C.c_void_p(kept.data_ptr()), C.c_void_p(mass_out.data_ptr()), C.c_void_p(lens_out.data_ptr()))
+    return lens_out, kept, mass_out
 
 
 class _DenoiseAttnArgs(C.Structure):
