@@ -208,6 +208,23 @@ typedef struct {
 VLAB200_API int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, const vlab200_qk_norm_rope_args *a,
                                                 void *stream);
 
+/* Attention of a call's query tokens to cached rows whose number differs from observation to observation (an encoder's states, a prefix
+ * after eviction), with the log-sum-exp of every query row:
+ *   out[b][tok][h*hd ..] = softmax(scale q K^T) V,   lse[b][h][tok] = log sum exp(scale q K^T)
+ * over the rows j < lens[b] of `layer` outside [pad_ranges[b][0], pad_ranges[b][1]); query head h reads kv head h / (n_q / n_kv).  A query
+ * row that sees nothing gives 0 and -inf; hidden rows may hold anything, no-numbers too.
+ * q: bf16 [n_obs][n_q][S][hd]; out: bf16 [n_obs][S][n_q*hd]; lse: float32 [n_obs][n_q][S] or NULL.  lens: int32 [n_obs], taken into
+ * [0, max_len], or NULL (max_len for all); 0 <= max_len <= cap bounds the rows that may be read.  scale 0 = 1 / sqrt(hd).
+ * ws: device memory of vlab200_cross_attention_ws_bytes() (32-byte aligned, nothing kept between calls, not shared by calls whose
+ * kernels may overlap) lets the blocks of a call be dealt to the SMs evenly; NULL: whole rows of 256 queries each.  Results are the same from
+ * run to run for the same lengths, and agree to rounding between the two.  The head widths are 64, 128 and 256.
+ * Stands beside vlab200_attention, which has one key range for all observations (src/models/smolvla.cpp:870-881 are the reference's cross
+ * layers). */
+VLAB200_API int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q); /* -1: arguments or no device */
+VLAB200_API int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const void *q, void *out, float *lse, int32_t S,
+                                            int32_t n_q, const int32_t *lens, int32_t max_len, const int32_t *pad_ranges, float scale,
+                                            void *ws, int64_t ws_bytes, void *stream);
+
 /* The attention weight that every cached row of `layer` got from a call's query tokens, accumulated over calls: for rows j < lens[b]
  *   mass_out[b][h][j] = decay * mass_in[b][h][j] + sum over the n_q / n_kv heads of kv head h and the S tokens of exp(scale q . k_j - lse)
  * q: bf16 [n_obs][n_q][S][head_dim] and lse: float32 [n_obs][n_q][S] as vlab200_cross_attention takes and returns them (a query row whose

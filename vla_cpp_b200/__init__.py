@@ -23,6 +23,7 @@ from .api import (  # noqa: F401
     act_quant,
     attention,
     bitvla_norm_quant,
+    cross_attention,
     device_status,
     fold_norm_weight,
     key_mass,

@@ -36,6 +36,7 @@ def lib():
             if name.startswith("vlab200_") and name not in ("vlab200_last_error",):
                 fn.restype = C.c_int32
         L.vlab200_kv_store_bytes.restype = C.c_int64
+        L.vlab200_cross_attention_ws_bytes.restype = C.c_int64
         L.vlab200_engine_create.restype = C.c_void_p
         L.vlab200_engine_free.restype = None
         L.vlab200_prefill_create.restype = C.c_void_p
@@ -77,7 +78,7 @@ EXPORTS = [
     "vlab200_qkv_rope_append",
     "vlab200_attention", "vlab200_denoise_attn_loop", "vlab200_denoise_attn_loop_host",
     "vlab200_denoise_attn_loop_static",
-    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append", "vlab200_key_mass", "vlab200_kv_evict",
+    "vlab200_rope_freqs", "vlab200_qk_norm_rope_append", "vlab200_cross_attention_ws_bytes", "vlab200_cross_attention", "vlab200_key_mass", "vlab200_kv_evict",
     "vlab200_engine_create", "vlab200_engine_free", "vlab200_engine_set_prefix", "vlab200_engine_denoise",
     "vlab200_engine_denoise_host", "vlab200_engine_run_stage", "vlab200_engine_set_prefix_len",
     "vlab200_engine_loop_phases", "vlab200_loop_kernel_phases",
@@ -371,6 +372,40 @@ def _ragged_args(store, q, lens, max_len, pad_ranges):
     if pad_ranges is not None:
         _need_tensor(pad_ranges, "pad_ranges", torch.int32, (B, 2), dev)
     return dev, S, n_q, store.cap if max_len is None else max_len
+
+
+def cross_attention(store, layer, q, lens=None, max_len=None, pad_ranges=None, scale=None, out=None, lse=None, split=True):
+    """Attention of query tokens to each observation's own number of cached rows -> (out, lse).
+
+    q: bf16 [n_obs, n_q, S, hd]; lens: int32 [n_obs] rows of every observation or None (max_len, by default the store's cap);
+    pad_ranges: int32 [n_obs, 2] hidden rows [lo, hi) or None.  out: bf16 [n_obs, S, n_q * hd], lse: f32 [n_obs, n_q, S] (0 and -inf for a
+    row that sees nothing).  split=False takes no workspace: work is cut at whole units only."""
+    import torch
+
+    dev, S, n_q, max_len = _ragged_args(store, q, lens, max_len, pad_ranges)
+    if out is None:
+        out = torch.empty((store.n_obs, S, n_q * store.head_dim), dtype=torch.bfloat16, device=q.device)
+    else:
+        _need_tensor(out, "out", torch.bfloat16, (store.n_obs, S, n_q * store.head_dim), dev)
+    if lse is None:
+        lse = torch.empty((store.n_obs, n_q, S), dtype=torch.float32, device=q.device)
+    else:
+        _need_tensor(lse, "lse", torch.float32, (store.n_obs, n_q, S), dev)
+    ws, n = None, 0
+    if split:
+        if torch.cuda.current_device() == dev:
+            n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q)
+        else:
+            with torch.cuda.device(dev):
+                n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q)
+        if n < 0:
+            raise VlaB200Error(ERR_ARG, f"cross_attention: {n_q} query heads on {store.n_kv} kv heads, {S} tokens")
+        ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
+    _call_on(dev, lib().vlab200_cross_attention, "vlab200_cross_attention", C.byref(store.c), layer, C.c_void_p(q.data_ptr()),
+             C.c_void_p(out.data_ptr()), C.c_void_p(lse.data_ptr()), S, n_q, C.c_void_p(lens.data_ptr()) if lens is not None else None, max_len,
+             C.c_void_p(pad_ranges.data_ptr()) if pad_ranges is not None else None, C.c_float(0.0 if scale is None else scale),
+             C.c_void_p(ws.data_ptr()) if ws is not None else None, C.c_int64(n))
+    return out, lse
 
 
 def key_mass(store, layer, q, lse, lens=None, max_len=None, pad_ranges=None, scale=None, decay=1.0, mass=None, out=None):

@@ -1,0 +1,998 @@
+// Attention of a call's query tokens to cached rows whose number differs from observation to observation:
+//
+//   out = softmax(scale q K^T over the visible rows) V,     lse = log sum exp(scale q K^T)
+//
+// visible: row < len[b], not in the observation's hidden range [lo, hi).  A row that sees nothing gives 0 and -inf, whatever the pages hold.
+//
+// Heads of 64 and 128, a unit = (observation, kv head, 256 of the g S stacked query rows), one CTA:
+//   loader warp       TMA: the two 128-row Q tiles of a unit, K and V in blocks of 128 rows through rings
+//   MMA warp          S_t = Q_t K_j^T, then O_t += P_t V_j with P_t read from TMEM, for the tiles t = 0, 1 in turn, so that the
+//                     tensor pipe works on one tile while the other is in its softmax
+//   2 x 4 warps       one per tile and lane quarter, a row per thread: maximum, 2^(s c - m), row sum, P over S in TMEM
+// TMEM: O_0, O_1 and one S per tile (512 columns at heads of 128).  Both the exponentials (16 per clock and SM) and the products need
+// 1,024 clocks per tile and block at heads of 128; at 64 the exponentials bound it.
+//
+// Work is dealt out in blocks, not units: the units' blocks form one list and every CTA takes an equal piece of it, so neither ragged
+// lengths nor few units leave SMs idle.  A unit cut by a piece's border leaves un-normalised rows with their maximum and sum in the
+// workspace, at most two per CTA, and cross_combine_kernel merges them in order.  Without a workspace borders move to whole units.
+#include <cuda_bf16.h>
+
+#include "f32x2.cuh"
+#include "host_common.h"
+#include "ragged.cuh"
+#include "tc5.cuh"
+
+namespace vb {
+
+constexpr int XA_BKV = 128;      // rows of K / V per block
+constexpr int XA_THREADS = 320;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA
+constexpr int XA_LOADER = 8, XA_MMA = 9;
+constexpr float XA_RAISE = 8.0f; // the running maximum is raised, and O rescaled, only by blocks that exceed it by more than 2^8
+
+struct CrossParams {
+    __nv_bfloat16 *out;  // [n_obs][S][n_q * HD]
+    float *lse;          // [n_obs][n_q][S] or nullptr
+    const int32_t *lens, *pad;
+    int S, n_q, n_kv, g, R, n_obs, max_len, page0;
+    int n_mt, unit_rows; // units per item and their rows
+    int n_work;          // CTAs (CTA pairs) the blocks are dealt to
+    int out_al32;
+    float scale_log2;
+    int *status;
+    float *ws_o;         // [2 n_work][ws_rows][HD], nullptr: whole units
+    float *ws_ml;        // [2 n_work][ws_rows][2]: maximum (log2 units), row sum
+    int ws_rows;
+};
+
+__device__ __forceinline__ int xa_len(const CrossParams &p, int obs) {
+    return p.lens ? min(max(p.lens[obs], 0), p.max_len) : p.max_len;
+}
+__device__ __forceinline__ float xa_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float xa_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// The blocks of all units, and the piece of CTA `c` of `n`.
+__device__ __forceinline__ int xa_total_blocks(const CrossParams &p) {  // whole warp
+    int sum = 0;
+    for (int b = threadIdx.x & 31; b < p.n_obs; b += 32) sum += (xa_len(p, b) + XA_BKV - 1) / XA_BKV;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum * p.n_kv * p.n_mt;
+}
+__device__ __forceinline__ int xa_border(int c, int n, int total) { return (int)((long long)c * total / n); }
+
+struct XaSegment {  // a run of blocks [j0, j1) of one unit
+    int obs, kvh, mt, j0, j1, len, slot;  // slot: of the workspace; -1: the unit is whole
+};
+
+template <typename LenOf>
+struct XaWork {
+    RaggedCursor<LenOf> cur;
+    int w, w1, w0, c, n_mt;
+    bool whole_units;
+    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, int cta) : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV) {
+        const int total = xa_total_blocks(p), n = min(p.n_work, total);
+        c = cta;
+        w = w0 = cta < n ? xa_border(cta, n, total) : total;
+        w1 = cta < n ? xa_border(cta + 1, n, total) : total;
+        n_mt = p.n_mt;
+        whole_units = p.ws_o == nullptr;
+    }
+    __device__ __forceinline__ bool next(XaSegment &s) {  // whole warp
+        RaggedUnit u;
+        while (w < w1 && cur.find(w, u)) {
+            const int nb = (u.len + XA_BKV - 1) / XA_BKV;
+            if (whole_units && u.block > 0) {  // begun by the CTA before, which finishes it
+                w += nb - u.block;
+                continue;
+            }
+            s.obs = u.obs;
+            s.len = u.len;
+            s.kvh = u.kvh / n_mt;
+            s.mt = u.kvh - s.kvh * n_mt;
+            s.j0 = u.block;
+            s.j1 = whole_units ? nb : min(nb, u.block + (w1 - w));
+            s.slot = s.j0 == 0 && s.j1 == nb ? -1 : 2 * c + (s.j0 > 0 ? 0 : 1);
+            w += s.j1 - s.j0;
+            return true;
+        }
+        return false;
+    }
+};
+
+template <int HD>
+struct CrossSmem {
+    static constexpr int CB = HD / 64;                // 64-element column blocks
+    static constexpr int Q_BYTES = CB * 128 * 128;    // a tile: [CB][128 rows][128 B]
+    static constexpr int KV_BYTES = CB * XA_BKV * 128;
+    static constexpr int STAGES = HD == 64 ? 4 : 2;
+    static constexpr int K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES, BAR_OFF = V_OFF + STAGES * KV_BYTES;
+    static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+    static constexpr int S_COL = 2 * HD;  // O_0, O_1, S_0, S_1
+    static_assert(S_COL + 2 * XA_BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
+};
+
+// Zeroes the rows of a V block in shared memory that the mask hides: they meet weights of 0, and 0 times what stands there need not be 0.
+// `tid` of 128 takes row tid; V: [n_cb][128 rows][128 B].
+__device__ __forceinline__ void xa_clean_v(uint8_t *v, int n_cb, int tid, int row, int len, int pad_lo, int pad_hi) {
+    if (row >= len || (row >= pad_lo && row < pad_hi)) {
+        for (int cb = 0; cb < n_cb; ++cb) {
+            uint4 *r = reinterpret_cast<uint4 *>(v + cb * (XA_BKV * 128) + tid * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    fence_proxy_async_smem();
+}
+
+// 32 columns of O of one row, divided and rounded, to 32 bf16 at dst.
+__device__ __forceinline__ void xa_store32(__nv_bfloat16 *dst, const uint32_t (&o)[32], float inv, int al32) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[16 * q + 2 * e]) * inv, __uint_as_float(o[16 * q + 2 * e + 1]) * inv);
+            w[e] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        if (al32) {
+            st_global_v8(dst + 16 * q, w);
+        } else {
+            uint4 *d4 = reinterpret_cast<uint4 *>(dst + 16 * q);
+            d4[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            d4[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(XA_THREADS, 1)
+cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                  const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
+    using L = CrossSmem<HD>;
+    constexpr uint32_t NS = L::STAGES;
+    extern __shared__ uint8_t xa_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xa_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
+    uint64_t *q_full = bars, *q_free = bars + 1, *k_full = bars + 2, *k_free = bars + 6, *v_full = bars + 10, *v_free = bars + 14;
+    uint64_t *s_full = bars + 18, *p_full = bars + 20, *pv_done = bars + 22, *o_free = bars + 24;  // [2 tiles]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 26);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtx wc{abort_flag, p.status};
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_free, 1);
+        for (uint32_t i = 0; i < NS; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_free[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+            mbar_init(&o_free[i], 4);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == XA_MMA) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&q_map);
+        tma_prefetch_desc(&k_map);
+        tma_prefetch_desc(&v_map);
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+
+    auto len_of = [&](int obs) { return xa_len(p, obs); };
+    XaWork work(len_of, p, blockIdx.x);
+    XaSegment s;
+    bool ok = true;
+
+    if (warp == XA_LOADER) {
+        uint32_t si = 0, jb = 0;
+        for (; ok && work.next(s); ++si) {
+            const int item = s.obs * p.n_kv + s.kvh, row0 = s.mt * 256;
+            const int tiles = p.R > row0 + 128 ? 2 : 1;
+            ok = warp_wait(q_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+            if (!ok) break;
+            if (elect_one()) {
+                mbar_expect_tx(q_full, tiles * L::Q_BYTES);
+                for (int t = 0; t < tiles; ++t)
+                    for (int cb = 0; cb < L::CB; ++cb)
+                        tma_load_3d(smem + t * L::Q_BYTES + cb * 16384, &q_map, q_full, cb * 64, row0 + t * 128, item);
+            }
+            for (int j = s.j0; j < s.j1; ++j, ++jb) {
+                const uint32_t st = jb % NS, ph = (jb / NS) & 1u;
+                ok = warp_wait(&k_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                if (elect_one()) {
+                    mbar_expect_tx(&k_full[st], L::KV_BYTES);
+                    for (int cb = 0; cb < L::CB; ++cb)
+                        tma_load_3d(smem + L::K_OFF + st * L::KV_BYTES + cb * 16384, &k_map, &k_full[st], cb * 64, j * XA_BKV, p.page0 + item);
+                }
+                ok = warp_wait(&v_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                if (elect_one()) {
+                    mbar_expect_tx(&v_full[st], L::KV_BYTES);
+                    for (int cb = 0; cb < L::CB; ++cb)
+                        tma_load_3d(smem + L::V_OFF + st * L::KV_BYTES + cb * 16384, &v_map, &v_full[st], cb * 64, j * XA_BKV, p.page0 + item);
+                }
+            }
+        }
+    } else if (warp == XA_MMA) {
+        constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, XA_BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
+        const uint32_t base = smem_u32(smem);
+        auto issue_s = [&](int t, uint32_t st) {
+            const uint32_t q = base + t * L::Q_BYTES, k = base + L::K_OFF + st * L::KV_BYTES, d = tmem_base + L::S_COL + t * XA_BKV;
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    mma_f16(d, smem_desc_sw128(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
+                            smem_desc_sw128(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
+                tc_commit(&s_full[t]);
+            }
+        };
+        auto issue_pv = [&](int t, uint32_t st, bool first) {
+            const uint32_t v = base + L::V_OFF + st * L::KV_BYTES, pt = tmem_base + L::S_COL + t * XA_BKV;
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < XA_BKV / 16; ++kk)
+                    mma_f16_tmem_a(tmem_base + t * HD, pt + (uint32_t)(kk * 8), smem_desc_sw128(v + kk * 2048, 16384, 1024), idesc_o,
+                                   first && kk == 0 ? 0u : 1u);
+                tc_commit(&pv_done[t]);
+            }
+        };
+        uint32_t si = 0, jb = 0;
+        uint32_t blk[2] = {0, 0}, seg[2] = {0, 0};  // blocks and segments of each tile so far
+        for (; ok && work.next(s); ++si) {
+            const int tiles = p.R > s.mt * 256 + 128 ? 2 : 1;
+            ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
+            if (ok) ok = warp_wait(&k_full[jb % NS], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            // a tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order
+            for (int t = 0; t < tiles; ++t) issue_s(t, jb % NS);
+            if (elect_one()) {
+                tc_commit(&k_free[jb % NS]);
+                if (s.j1 - s.j0 == 1) tc_commit(q_free);
+            }
+            for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
+                const uint32_t st = jb % NS, ph = (jb / NS) & 1u, jn = jb + 1, sn = jn % NS;
+                for (int t = 0; t < tiles; ++t) {
+                    ok = warp_wait(&p_full[t], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (ok && t == 0) ok = warp_wait(&v_full[st], ph, wc, DEV_TIMEOUT_FULL);
+                    if (ok && j == s.j0) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                    if (ok && t == 0 && j + 1 < s.j1) ok = warp_wait(&k_full[sn], (jn / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(t, st, j == s.j0);
+                    ++blk[t];
+                    if (j + 1 < s.j1) issue_s(t, sn);
+                }
+                if (!ok) break;
+                if (elect_one()) {
+                    tc_commit(&v_free[st]);
+                    if (j + 1 < s.j1) tc_commit(&k_free[sn]);
+                    if (j + 2 == s.j1) tc_commit(q_free);  // the segment's last S blocks have been issued
+                }
+            }
+            for (int t = 0; t < tiles; ++t) ++seg[t];
+        }
+    } else {
+        const int t = warp >> 2, qtr = warp & 3;
+        const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
+        const uint32_t s_addr = tmem_base + L::S_COL + t * XA_BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
+        const F2 scale2 = f2(p.scale_log2, p.scale_log2);
+        uint32_t blk = 0;  // blocks of this tile so far; tile 0 has every block of the CTA
+        while (ok && work.next(s)) {
+            const int row0 = s.mt * 256 + t * 128;
+            if (t == 1 && row0 >= p.R) continue;
+            const int lr = t * 128 + qtr * 32 + lane, row = s.mt * 256 + lr;  // in the unit, in the item
+            const bool live = row0 + qtr * 32 < p.R;                          // of the warp
+            int pad_lo = 0, pad_hi = 0;
+            if (p.pad) {
+                pad_lo = p.pad[2 * s.obs];
+                pad_hi = p.pad[2 * s.obs + 1];
+            }
+            if (pad_hi <= pad_lo) pad_lo = pad_hi = 0x7fffffff;
+            float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units, row sum
+            for (int j = s.j0; j < s.j1; ++j, ++blk) {
+                ok = warp_wait(&s_full[t], blk & 1u, wc, DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                tc_fence_after();
+                const int c0 = j * XA_BKV;
+                const bool dirty = c0 + XA_BKV > s.len || (c0 < pad_hi && c0 + XA_BKV > pad_lo);
+                if (live) {
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + (uint32_t)(i * 32), x[i]);
+                    tmem_ld_wait();
+                    if (dirty) {
+                        const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const int c = i * 32 + e;
+                                x[i][e] = c < lim && (c < lo || c >= hi) ? x[i][e] : 0xff800000u;
+                            }
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mx[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
+#pragma unroll
+                        for (int e = 2; e < 32; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
+                    }
+                    const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                    float factor = 1.0f;
+                    const bool raise = bm > m_used + XA_RAISE;
+                    if (raise) {
+                        factor = m_used == -INFINITY ? 0.0f : xa_ex2(m_used - bm);
+                        m_used = bm;
+                        l_sum *= factor;
+                    }
+                    if (j > s.j0 && __any_sync(0xffffffffu, raise)) {  // O was summed under the old maximum
+                        ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t ov[16];
+                            tmem_ld16(o_addr + (uint32_t)c, ov);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
+                            tmem_st16(o_addr + (uint32_t)c, ov);
+                        }
+                    }
+                    const float mref = m_used == -INFINITY ? 0.0f : m_used;
+                    const F2 neg = f2(-mref, -mref);
+                    F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int e = 0; e < 64; e += 2) {
+                            const F2 a = f2_fma(f2(__uint_as_float(x[i + (e >> 5)][e & 31]), __uint_as_float(x[i + (e >> 5)][(e & 31) + 1])), scale2, neg);
+                            float a0, a1;
+                            f2_get(a, a0, a1);
+                            const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
+                            sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
+                            pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
+                        }
+                        tmem_st32(s_addr + (uint32_t)(i * 16), pk);
+                    }
+                    float u0, u1, u2, u3;
+                    f2_get(sum[0], u0, u1);
+                    f2_get(sum[1], u2, u3);
+                    l_sum += (u0 + u1) + (u2 + u3);
+                    tmem_st_wait();
+                }
+                if (dirty && t == 0) {  // before either tile's product: the MMA warp takes tile 0 first
+                    const uint32_t st = blk % NS;
+                    ok = warp_wait(&v_full[st], (blk / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    xa_clean_v(smem + L::V_OFF + st * L::KV_BYTES, L::CB, threadIdx.x, c0 + (int)threadIdx.x, s.len, pad_lo, pad_hi);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+            }
+            if (!ok) break;
+            // ---- O / l -> bf16 -> out, or the piece into the workspace ----
+            ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+            if (!ok) break;
+            tc_fence_after();
+            const bool row_ok = row < p.R;
+            const int head = row_ok ? s.kvh * p.g + row / p.S : 0, tok = row_ok ? row % p.S : 0;
+            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
+            __nv_bfloat16 *dst = p.out + (((long long)s.obs * p.S + tok) * p.n_q + head) * HD;
+            float *wo = p.ws_o + ((long long)s.slot * p.ws_rows + lr) * HD;
+            if (live) {
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t ov[32];
+                    tmem_ld32(o_addr + (uint32_t)c, ov);
+                    tmem_ld_wait();
+                    if (!row_ok) continue;
+                    if (s.slot < 0) {
+                        xa_store32(dst + c, ov, inv, p.out_al32);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            const uint32_t w[8] = {ov[e], ov[e + 1], ov[e + 2], ov[e + 3], ov[e + 4], ov[e + 5], ov[e + 6], ov[e + 7]};
+                            st_global_v8(wo + c + e, w);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[t]);
+            if (row_ok) {
+                if (s.slot >= 0)
+                    *reinterpret_cast<float2 *>(p.ws_ml + ((long long)s.slot * p.ws_rows + lr) * 2) = make_float2(m_used, l_sum);
+                else if (p.lse)
+                    p.lse[((long long)s.obs * p.n_q + head) * p.S + tok] = l_sum == 0.0f ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == XA_MMA) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// ------------------------------------------------------------------ heads of 256: CTA pairs --
+// O alone takes 256 columns of TMEM and K, V of 128 rows 64 KB each, so one CTA has room for one tile and no second block.  A pair of CTAs
+// (tcgen05 cta_group::2, M = 256) shares every block: each stages half of K's rows and half of V's columns, and holds one of the
+// unit's two tiles.  Two S buffers lie behind O; two warps of the even CTA issue the products, Q K^T up to a block ahead of P V (the first
+// follows the second by a counter: the pipe keeps their order); the odd CTA tells the even one what has landed.
+//   8 softmax warps   lane quarter = warp & 3, column half = warp >> 2: the two warps of a row exchange maxima and sums through shared memory
+// A unit's O is drained after the next unit's first block, so the pipe does not wait for it.
+constexpr int XP_THREADS = 352, XP_LOADER = 8, XP_S = 9, XP_PV = 10;
+
+struct CrossPairSmem {
+    static constexpr int HD = 256, CB = 4, CBH = 2;  // 64-element column blocks of the head, and of the half of V that a CTA stages
+    static constexpr int STAGES = 2, NS = 2;
+    static constexpr int Q_BYTES = CB * 128 * 128, K_BYTES = CB * 64 * 128, V_BYTES = CBH * 128 * 128;
+    static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + STAGES * K_BYTES, BAR_OFF = V_OFF + STAGES * V_BYTES;
+    static constexpr int XCH_OFF = BAR_OFF + 256;  // float [2][2 halves][128]: block maxima, used in turn; then the row sums
+    static constexpr int TOTAL = XCH_OFF + 3 * 2 * 128 * 4 + 1024;
+    static_assert(TOTAL <= 227 * 1024, "shared memory");
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XP_THREADS, 1)
+cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
+    using L = CrossPairSmem;
+    constexpr int HD = L::HD;
+    constexpr uint32_t ST = L::STAGES, NS = L::NS;
+    extern __shared__ uint8_t xp_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xp_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
+    uint64_t *q_full = bars, *q_free = bars + 1, *o_done = bars + 2, *o_free = bars + 3;
+    uint64_t *k_full = bars + 4, *k_free = bars + 6, *v_full = bars + 8, *v_free = bars + 10;  // [ST]
+    uint64_t *s_full = bars + 12, *p_full = bars + 14, *pv_done = bars + 16;                   // [NS]
+    uint64_t *meet = bars + 18;                                                                // [4] the two warps of a lane quarter
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile uint32_t *pv_issued = reinterpret_cast<volatile uint32_t *>(tmem_slot + 2);  // P V blocks issued so far (even CTA)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const WaitCtx wc{abort_flag, p.status};
+    const uint32_t both = rank == 0 ? 2u : 1u;  // even CTA: its own TMA and the odd CTA's word
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, both);
+        mbar_init(q_free, 1);
+        mbar_init(o_done, 1);
+        mbar_init(o_free, 16);  // the softmax warps of both CTAs (used in the even one)
+        for (uint32_t i = 0; i < ST; ++i) {
+            mbar_init(&k_full[i], both);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_full[i], both);
+            mbar_init(&v_free[i], 1);
+        }
+        for (uint32_t i = 0; i < NS; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 16);
+            mbar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 64);
+        *abort_flag = 0;
+        *pv_issued = 0;
+        fence_barrier_init();
+    }
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == XP_S) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&q_map);
+        tma_prefetch_desc(&k_map);
+        tma_prefetch_desc(&v_map);
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+
+    auto len_of = [&](int obs) { return xa_len(p, obs); };
+    XaWork work(len_of, p, blockIdx.x >> 1);
+    XaSegment s;
+    bool ok = true;
+    uint32_t si = 0, jb = 0;  // segments and blocks so far
+
+    if (warp == XP_LOADER) {
+        for (; ok && work.next(s); ++si) {
+            const int item = s.obs * p.n_kv + s.kvh;
+            ok = warp_wait(q_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+            if (!ok) break;
+            if (elect_one()) {
+                mbar_expect_tx(q_full, L::Q_BYTES);
+                for (int cb = 0; cb < L::CB; ++cb)
+                    tma_load_3d(smem + cb * 16384, &q_map, q_full, cb * 64, s.mt * 256 + (int)rank * 128, item);
+            }
+            for (int j = s.j0; j < s.j1; ++j, ++jb) {
+                const uint32_t st = jb % ST, ph = (jb / ST) & 1u;
+                ok = warp_wait(&k_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                if (elect_one()) {
+                    mbar_expect_tx(&k_full[st], L::K_BYTES);
+                    for (int cb = 0; cb < L::CB; ++cb)
+                        tma_load_3d(smem + L::K_OFF + st * L::K_BYTES + cb * 8192, &k_map, &k_full[st], cb * 64, j * XA_BKV + (int)rank * 64,
+                                    p.page0 + item);
+                }
+                ok = warp_wait(&v_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                if (elect_one()) {
+                    mbar_expect_tx(&v_full[st], L::V_BYTES);
+                    for (int cb = 0; cb < L::CBH; ++cb)
+                        tma_load_3d(smem + L::V_OFF + st * L::V_BYTES + cb * 16384, &v_map, &v_full[st], ((int)rank * L::CBH + cb) * 64,
+                                    j * XA_BKV, p.page0 + item);
+                }
+            }
+        }
+    } else if (warp == XP_S) {
+        if (rank == 0) {
+            constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 256, XA_BKV);
+            const uint64_t q_desc0 = smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc0 = smem_desc_sw128(smem_u32(smem) + L::K_OFF, 16, 1024);
+            for (; ok && work.next(s); ++si) {
+                ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
+                for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
+                    ok = warp_wait(&k_full[jb % ST], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
+                    // the P V of the block that used this S buffer has to be in the pipe
+                    if (ok && jb >= NS && *pv_issued < jb - NS + 1u) {
+                        const long long t0 = clock64();
+                        for (uint32_t it = 1; *pv_issued < jb - NS + 1u; ++it) {
+                            if ((it & 63u) == 0) {
+                                if (*abort_flag) {
+                                    ok = false;
+                                    break;
+                                }
+                                if (clock64() - t0 > wc.budget) {
+                                    *abort_flag = 1;
+                                    atomicCAS(p.status, 0, (int)DEV_TIMEOUT_FULL);
+                                    ok = false;
+                                    break;
+                                }
+                            }
+                        }
+                    }
+                    ok = __all_sync(0xffffffffu, ok) != 0;
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t st = jb % ST, d = tmem_base + HD + (jb % NS) * XA_BKV;
+                    const uint64_t k_desc = k_desc0 + (uint64_t)(st * (L::K_BYTES >> 4));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk)
+                            mma_f16_pair(d, q_desc0 + (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2), k_desc + (uint64_t)((kk >> 2) * 512 + (kk & 3) * 2),
+                                         idesc_s, kk != 0 ? 1u : 0u);
+                        tc_commit_pair(&s_full[jb % NS], 3);
+                        tc_commit_pair(&k_free[st], 3);
+                        if (j + 1 == s.j1) tc_commit_pair(q_free, 3);
+                    }
+                }
+            }
+        } else {
+            for (; ok && work.next(s); ++si) {
+                ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_cluster(q_full, 0);
+                for (int j = s.j0; j < s.j1; ++j, ++jb) {
+                    const uint32_t st = jb % ST, ph = (jb / ST) & 1u;
+                    ok = warp_wait(&k_full[st], ph, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_cluster(&k_full[st], 0);
+                    ok = warp_wait(&v_full[st], ph, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_cluster(&v_full[st], 0);
+                }
+            }
+        }
+    } else if (warp == XP_PV) {
+        if (rank == 0) {
+            constexpr uint32_t idesc_o = make_idesc(1, 1, 1, 0, 1, 256, HD);
+            const uint64_t v_desc0 = smem_desc_sw128(smem_u32(smem) + L::V_OFF, 16384, 1024);
+            for (; ok && work.next(s); ++si) {
+                for (int j = s.j0; j < s.j1; ++j, ++jb) {
+                    const uint32_t sb = jb % NS, st = jb % ST;
+                    ok = warp_wait(&p_full[sb], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (ok) ok = warp_wait(&v_full[st], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (ok && j == s.j0) ok = warp_wait(o_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t v_desc = v_desc0 + (uint64_t)(st * (L::V_BYTES >> 4));
+                    const uint32_t p_tmem = tmem_base + HD + sb * XA_BKV;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < XA_BKV / 16; ++kk)
+                            mma_f16_tmem_a_pair(tmem_base, p_tmem + (uint32_t)(kk * 8), v_desc + (uint64_t)(kk * 128), idesc_o,
+                                                j != s.j0 || kk != 0 ? 1u : 0u);
+                        *pv_issued = jb + 1u;
+                        tc_commit_pair(&pv_done[sb], 3);
+                        tc_commit_pair(&v_free[st], 3);
+                        if (j + 1 == s.j1) tc_commit_pair(o_done, 3);
+                    }
+                }
+            }
+        }
+    } else {
+        const int qtr = warp & 3, half = warp >> 2;
+        const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
+        float *xch = reinterpret_cast<float *>(smem + L::XCH_OFF);
+        const int my_slot = qtr * 32 + lane, lr = (int)rank * 128 + my_slot;  // row of the unit
+        const F2 scale2 = f2(p.scale_log2, p.scale_log2);
+        uint32_t met = 0;
+        auto pair_sync = [&]() -> bool {
+            mbar_arrive(&meet[qtr]);
+            return warp_wait(&meet[qtr], (met++) & 1u, wc, DEV_TIMEOUT_MISC);
+        };
+        auto arrive_even = [&](uint64_t *bar) {  // one arrival per warp on the even CTA's barrier
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) mbar_arrive(bar);
+                else mbar_arrive_cluster(bar, 0);
+            }
+        };
+        // segment `u` is complete: O / l -> bf16 -> out, or the piece into the workspace
+        auto drain = [&](uint32_t u, const XaSegment &sg, float m, float l_mine) -> bool {
+            xch[512 + half * 128 + my_slot] = l_mine;
+            if (!warp_wait(o_done, u & 1u, wc, DEV_TIMEOUT_ACCUM)) return false;
+            tc_fence_after();
+            if (!pair_sync()) return false;
+            const float l = l_mine + xch[512 + (half ^ 1) * 128 + my_slot];
+            const int row = sg.mt * 256 + lr;
+            const bool row_ok = row < p.R;
+            const int head = row_ok ? sg.kvh * p.g + row / p.S : 0, tok = row_ok ? row % p.S : 0;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            __nv_bfloat16 *dst = p.out + (((long long)sg.obs * p.S + tok) * p.n_q + head) * HD;
+            float *wo = p.ws_o + ((long long)sg.slot * p.ws_rows + lr) * HD;
+#pragma unroll 1
+            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                uint32_t ov[32];
+                tmem_ld32(tmem_base + lane_sel + (uint32_t)c, ov);
+                tmem_ld_wait();
+                if (c + 32 == (half + 1) * (HD / 2)) {  // O is out of TMEM
+                    tc_fence_before();
+                    arrive_even(o_free);
+                }
+                if (!row_ok) continue;
+                if (sg.slot < 0) {
+                    xa_store32(dst + c, ov, inv, p.out_al32);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        const uint32_t w[8] = {ov[e], ov[e + 1], ov[e + 2], ov[e + 3], ov[e + 4], ov[e + 5], ov[e + 6], ov[e + 7]};
+                        st_global_v8(wo + c + e, w);
+                    }
+                }
+            }
+            if (row_ok && half == 0) {
+                if (sg.slot >= 0)
+                    *reinterpret_cast<float2 *>(p.ws_ml + ((long long)sg.slot * p.ws_rows + lr) * 2) = make_float2(m, l);
+                else if (p.lse)
+                    p.lse[((long long)sg.obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            }
+            return true;  // (the row-sum slots are next written after at least one more meeting of the pair)
+        };
+        XaSegment prev;
+        float prev_m = 0.0f, prev_l = 0.0f;
+        for (; ok && work.next(s); ++si) {
+            int pad_lo = 0, pad_hi = 0;
+            if (p.pad) {
+                pad_lo = p.pad[2 * s.obs];
+                pad_hi = p.pad[2 * s.obs + 1];
+            }
+            if (pad_hi <= pad_lo) pad_lo = pad_hi = 0x7fffffff;
+            float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units (the same in both halves), this half's part of the row sum
+            for (int j = s.j0; j < s.j1; ++j, ++jb) {
+                const uint32_t sb = jb % NS;
+                const uint32_t s_addr = tmem_base + HD + sb * XA_BKV + lane_sel;
+                ok = warp_wait(&s_full[sb], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t x[2][32];
+                tmem_ld32(s_addr + (uint32_t)(half * 64), x[0]);
+                tmem_ld32(s_addr + (uint32_t)(half * 64 + 32), x[1]);
+                tmem_ld_wait();
+                const int b0 = j * XA_BKV, c0 = b0 + half * 64;
+                const bool dirty = b0 + XA_BKV > s.len || (b0 < pad_hi && b0 + XA_BKV > pad_lo);
+                if (dirty) {
+                    const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int c = i * 32 + e;
+                            x[i][e] = c < lim && (c < lo || c >= hi) ? x[i][e] : 0xff800000u;
+                        }
+                }
+                float mx[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    mx[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
+#pragma unroll
+                    for (int e = 2; e < 32; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
+                }
+                float bm = fmaxf(mx[0], mx[1]);
+                float *xm = xch + (jb & 1u) * 256;  // two sets of slots, used in turn: one meeting per block is enough
+                xm[half * 128 + my_slot] = bm;
+                ok = pair_sync();
+                if (!ok) break;
+                bm = fmaxf(bm, xm[(half ^ 1) * 128 + my_slot]) * p.scale_log2;
+                float factor = 1.0f;
+                const bool raise = bm > m_used + XA_RAISE;
+                if (raise) {
+                    factor = m_used == -INFINITY ? 0.0f : xa_ex2(m_used - bm);
+                    m_used = bm;
+                    l_sum *= factor;
+                }
+                if (j > s.j0 && __any_sync(0xffffffffu, raise)) {  // O was summed under the old maximum
+                    ok = warp_wait(&pv_done[(jb - 1) % NS], ((jb - 1) / NS) & 1u, wc, DEV_TIMEOUT_ACCUM);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                        uint32_t ov[32];
+                        tmem_ld32(tmem_base + lane_sel + (uint32_t)c, ov);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
+                        tmem_st32(tmem_base + lane_sel + (uint32_t)c, ov);
+                    }
+                    tmem_st_wait();
+                }
+                const float mref = m_used == -INFINITY ? 0.0f : m_used;
+                const F2 neg = f2(-mref, -mref);
+                F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+                uint32_t pk[32];
+#pragma unroll
+                for (int e = 0; e < 64; e += 2) {
+                    const F2 a = f2_fma(f2(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])), scale2, neg);
+                    float a0, a1;
+                    f2_get(a, a0, a1);
+                    const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
+                    sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
+                    pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
+                }
+                float u0, u1, u2, u3;
+                f2_get(sum[0], u0, u1);
+                f2_get(sum[1], u2, u3);
+                l_sum += (u0 + u1) + (u2 + u3);
+                // P (128 rows of V, bf16) over the first 64 columns of S; both halves have read theirs: they met
+                tmem_st32(s_addr + (uint32_t)(half * 32), pk);
+                tmem_st_wait();
+                if (dirty && half == 0) {  // this CTA's half of V's columns
+                    const uint32_t st = jb % ST;
+                    ok = warp_wait(&v_full[st], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    xa_clean_v(smem + L::V_OFF + st * L::V_BYTES, L::CBH, threadIdx.x, b0 + (int)threadIdx.x, s.len, pad_lo, pad_hi);
+                }
+                tc_fence_before();
+                arrive_even(&p_full[sb]);
+                if (j == s.j0 && si > 0) {
+                    ok = drain(si - 1, prev, prev_m, prev_l);
+                    if (!ok) break;
+                }
+            }
+            if (!ok) break;
+            prev = s;
+            prev_m = m_used;
+            prev_l = l_sum;
+        }
+        if (ok && si > 0) ok = drain(si - 1, prev, prev_m, prev_l);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // neither CTA may exit while the other can still signal its barriers
+    if (warp == XP_S) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Rows of empty
+// observations: 0 and -inf.  A warp per row; rows of whole units are done.
+template <int HD>
+__global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int item = blockIdx.y + (int)gridDim.y * blockIdx.z;
+    if (item >= p.n_obs * p.n_kv) return;
+    const int obs = item / p.n_kv, kvh = item % p.n_kv, row = blockIdx.x * 8 + warp;
+    const int nb = (xa_len(p, obs) + XA_BKV - 1) / XA_BKV;
+    if (nb > 0 && p.ws_o == nullptr) return;
+    int c0 = 0, c1 = 0;
+    if (nb > 0) {
+        int before = 0;
+        for (int b = lane; b < obs; b += 32) before += (xa_len(p, b) + XA_BKV - 1) / XA_BKV;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+        const int total = xa_total_blocks(p), n = min(p.n_work, total);
+        const int at = (before * p.n_kv + nb * kvh) * p.n_mt + nb * (row / p.unit_rows);
+        c0 = (int)(((long long)(at + 1) * n - 1) / total);  // the CTA that has block w: the last whose piece begins at or before w
+        c1 = (int)(((long long)(at + nb) * n - 1) / total);
+        if (c0 == c1) return;
+    }
+    if (row >= p.R) return;
+    const int head = kvh * p.g + row / p.S, tok = row % p.S;
+    constexpr int NV = HD / 64;  // pairs of columns per lane
+    float2 acc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = make_float2(0.0f, 0.0f);
+    float l = 0.0f, M = -INFINITY;
+    if (nb > 0) {
+        const int lr = row % p.unit_rows;
+        auto slot_of = [&](int c) { return (long long)(2 * c + (c == c0 ? 1 : 0)) * p.ws_rows + lr; };
+        for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, p.ws_ml[slot_of(c) * 2]);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        for (int c = c0; c <= c1; c += 4) {
+            float2 v[4][NV], ml[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const long long at = slot_of(min(c + i, c1));
+                ml[i] = *reinterpret_cast<const float2 *>(p.ws_ml + at * 2);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) v[i][k] = reinterpret_cast<const float2 *>(p.ws_o + at * HD)[k * 32 + lane];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (c + i > c1) break;
+                const float w = ml[i].x == -INFINITY ? 0.0f : xa_ex2(ml[i].x - M);
+                l = fmaf(ml[i].y, w, l);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    acc[k].x = fmaf(v[i][k].x, w, acc[k].x);
+                    acc[k].y = fmaf(v[i][k].y, w, acc[k].y);
+                }
+            }
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    __nv_bfloat162 *dst = reinterpret_cast<__nv_bfloat162 *>(p.out + (((long long)obs * p.S + tok) * p.n_q + head) * HD);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) dst[k * 32 + lane] = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv);
+    if (p.lse && lane == 0) p.lse[((long long)obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+}
+
+// Units, workers and workspace of a call; the same for the size query and the launch.
+struct CrossPlan {
+    int unit_rows, n_mt, n_work, ws_rows;
+    long long ws_bytes;
+};
+static CrossPlan cross_plan(int hd, int R, int n_sm) {
+    CrossPlan c;
+    c.unit_rows = 256;
+    c.n_mt = (R + 255) / 256;
+    c.n_work = hd == 256 ? n_sm / 2 : n_sm;
+    c.ws_rows = R < 256 ? R : 256;
+    c.ws_bytes = 2LL * c.n_work * c.ws_rows * (hd + 2) * 4;
+    return c;
+}
+
+template <int HD>
+static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &p, const CrossPlan &plan, cudaStream_t stream) {
+    const uint64_t pages = (uint64_t)st->n_layers * st->n_obs * st->n_kv;
+    CUtensorMap qmap, kmap, vmap;
+    const uint64_t qdims[3] = {(uint64_t)HD, (uint64_t)p.R, (uint64_t)st->n_obs * st->n_kv}, qstr[2] = {(uint64_t)HD * 2, (uint64_t)p.R * HD * 2};
+    const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)p.max_len, pages}, str[2] = {(uint64_t)HD * 2, (uint64_t)st->cap * HD * 2};
+    const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, HD == 256 ? 64 : 128, 1};
+    int rc = make_tensor_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, qdims, qstr, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_tensor_map(&kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->k_pages, dims, str, kbox, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    if constexpr (HD == 256) {
+        if ((rc = ensure_dyn_smem(cross_attn_pair_kernel, CrossPairSmem::TOTAL))) return rc;
+        rc = launch_pdl(cross_attn_pair_kernel, dim3(2 * (unsigned)plan.n_work), dim3(XP_THREADS), CrossPairSmem::TOTAL, stream, qmap, kmap, vmap, p);
+    } else {
+        if ((rc = ensure_dyn_smem(cross_attn_kernel<HD>, CrossSmem<HD>::TOTAL))) return rc;
+        rc = launch_pdl(cross_attn_kernel<HD>, dim3((unsigned)plan.n_work), dim3(XA_THREADS), CrossSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
+    }
+    if (rc) return rc;
+    const int items = st->n_obs * st->n_kv, gy = items < 32768 ? items : 32768;
+    return launch_pdl(cross_combine_kernel<HD>, dim3((unsigned)((p.R + 7) / 8), (unsigned)gy, (unsigned)((items + gy - 1) / gy)), dim3(256), 0, stream, p);
+}
+
+static bool cross_shape_ok(const vlab200_kv_store *st, int S, int n_q) {
+    return st && st->n_layers > 0 && st->n_obs > 0 && st->n_kv > 0 && st->cap > 0 && S > 0 && n_q > 0 && n_q % st->n_kv == 0;
+}
+
+}  // namespace vb
+
+extern "C" {
+
+int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q) {
+    if (!vb::cross_shape_ok(st, S, n_q) || (long long)(n_q / st->n_kv) * S > 0x7fffff00LL) return -1;
+    const int n_sm = vb::sm_count();
+    return n_sm ? vb::cross_plan(st->head_dim, (n_q / st->n_kv) * S, n_sm).ws_bytes : -1;
+}
+
+int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const void *q, void *out, float *lse, int32_t S, int32_t n_q,
+                                const int32_t *lens, int32_t max_len, const int32_t *pad_ranges, float scale, void *ws,
+                                int64_t ws_bytes, void *stream) {
+    if (!vb::cross_shape_ok(st, S, n_q) || !st->k_pages || !st->v_pages || !q || !out) return VLAB200_ERR_ARG;
+    if (layer < 0 || layer >= st->n_layers || max_len < 0 || max_len > st->cap || !(scale >= 0.0f) || ws_bytes < 0) return VLAB200_ERR_ARG;
+    const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(st->k_pages) |
+                         reinterpret_cast<uintptr_t>(st->v_pages);
+    if ((al & 15) || (reinterpret_cast<uintptr_t>(ws) & 31)) return VLAB200_ERR_ARG;
+    const int hd = st->head_dim;
+    if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
+    const long long R = (long long)(n_q / st->n_kv) * S, items = (long long)st->n_obs * st->n_kv;
+    const long long blocks = items * ((R + 127) / 128) * ((max_len + 127LL) / 128);
+    if (R > 0x7fffff00LL || items * st->n_layers > 0x7fffff00LL || items > 32768LL * 65535 || blocks > 0x7fffff00LL) {
+        vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 128 x 128 scores");
+        return VLAB200_ERR_UNSUPPORTED;
+    }
+    const int n_sm = vb::sm_count();
+    if (!n_sm) return vb::cuda_fail(cudaGetLastError(), "sm_count");
+    const vb::CrossPlan plan = vb::cross_plan(hd, (int)R, n_sm);
+    if (ws && ws_bytes < plan.ws_bytes) return VLAB200_ERR_ARG;
+    vb::CrossParams p;
+    p.out = static_cast<__nv_bfloat16 *>(out);
+    p.lse = lse;
+    p.lens = lens;
+    p.pad = pad_ranges;
+    p.S = S;
+    p.n_q = n_q;
+    p.n_kv = st->n_kv;
+    p.g = n_q / st->n_kv;
+    p.R = (int)R;
+    p.n_obs = st->n_obs;
+    p.max_len = max_len;
+    p.page0 = layer * st->n_obs * st->n_kv;
+    p.n_mt = plan.n_mt;
+    p.unit_rows = plan.unit_rows;
+    p.n_work = plan.n_work;
+    p.out_al32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0 ? 1 : 0;
+    p.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)hd));
+    p.status = vb::device_status_ptr();
+    if (!p.status) return vb::cuda_fail(cudaGetLastError(), "device_status_ptr");
+    p.ws_rows = plan.ws_rows;
+    p.ws_o = static_cast<float *>(ws);
+    p.ws_ml = ws ? p.ws_o + 2LL * plan.n_work * plan.ws_rows * hd : nullptr;
+    cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    if (max_len == 0) {  // nothing to map: every row is that of an empty observation
+        p.lens = nullptr;
+        const int gy = items < 32768 ? (int)items : 32768;
+        const dim3 grid((unsigned)((R + 7) / 8), (unsigned)gy, (unsigned)((items + gy - 1) / gy));
+        auto kernel = hd == 64 ? vb::cross_combine_kernel<64> : hd == 128 ? vb::cross_combine_kernel<128> : vb::cross_combine_kernel<256>;
+        return vb::launch_pdl(kernel, grid, dim3(256), 0, cs, p);
+    }
+    if (hd == 64) return vb::launch_cross<64>(st, q, p, plan, cs);
+    if (hd == 128) return vb::launch_cross<128>(st, q, p, plan, cs);
+    return vb::launch_cross<256>(st, q, p, plan, cs);
+}
+
+}  // extern "C"

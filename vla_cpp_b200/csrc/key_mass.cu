@@ -238,7 +238,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                 __syncwarp();
                 if (c + 1 < p.n_chunks) fetch_lse(true, now, c + 1);
                 else fetch_lse(there, unit, 0);
-                ok = mbar_wait(&a_full[ab.i], ab.ph, wc, DEV_TIMEOUT_ACCUM);
+                ok = warp_wait(&a_full[ab.i], ab.ph, wc, DEV_TIMEOUT_ACCUM);
                 if (!ok) break;
                 tc_fence_after();
                 const int n = min(p.R - c * L::NQ - part * PART, PART);  // of this warp's columns; may be 0 or less
@@ -288,7 +288,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             float *slot = sum_s + (un & 1u) * ((KM_PARTS - 1) * 128) + qtr * 32 + lane;
             if (part) slot[(part - 1) * 128] = sum;
             mbar_arrive(&meet[qtr]);
-            ok = mbar_wait(&meet[qtr], un & 1u, wc, DEV_TIMEOUT_MISC);
+            ok = warp_wait(&meet[qtr], un & 1u, wc, DEV_TIMEOUT_MISC);
             if (!ok) break;
             ++un;
             const int key = key0 + qtr * 32 + lane;
