@@ -6,11 +6,10 @@
 //
 // Heads of 64 and 128, a unit = (observation, kv head, 256 of the g S stacked query rows), one CTA:
 //   loader warp       TMA: the two 128-row Q tiles of a unit, K and V in blocks of 128 rows through rings
-//   MMA warp          S_t = Q_t K_j^T, then O_t += P_t V_j with P_t read from TMEM, for the tiles t = 0, 1 in turn, so that the
-//                     tensor pipe works on one tile while the other is in its softmax
+//   MMA warp          S_t = Q_t K_j^T of both tiles t = 0, 1, then O_t += P_t V_(j-1) with P_t read from TMEM
 //   2 x 4 warps       one per tile and lane quarter, a row per thread: maximum, 2^(s c - m), row sum, P over S in TMEM
-// TMEM: O_0, O_1 and one S per tile (512 columns at heads of 128).  Both the exponentials (16 per clock and SM) and the products need
-// 1,024 clocks per tile and block at heads of 128; at 64 the exponentials bound it.
+// TMEM: O_0, O_1 and two S buffers per tile (512 columns at heads of 128).  Both the exponentials (16 per clock and SM) and the products
+// need 512 clocks per tile and block of 64 at heads of 128; at 64 the exponentials bound it.
 //
 // Work is dealt out in blocks, not units: the units' blocks form one list and every CTA takes an equal piece of it, so neither ragged
 // lengths nor few units leave SMs idle.  A unit cut by a piece's border leaves un-normalised rows with their maximum and sum in the
@@ -24,7 +23,10 @@
 
 namespace vb {
 
-constexpr int XA_BKV = 128;      // rows of K / V per block
+// Rows of K / V per block.  Heads of 64 and 128: 64, so that a tile has two S buffers and its next scores are ready when its softmax
+// is (with one S of 128 a block took 5,000 clocks, softmax and products of a tile in turn, against 2,050 of either).
+template <int HD>
+constexpr int xa_bkv() { return HD == 256 ? 128 : 64; }
 constexpr int XA_THREADS = 320;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA
 constexpr int XA_LOADER = 8, XA_MMA = 9;
 constexpr float XA_RAISE = 8.0f; // the running maximum is raised, and O rescaled, only by blocks that exceed it by more than 2^8
@@ -36,6 +38,7 @@ struct CrossParams {
     int S, n_q, n_kv, g, R, n_obs, max_len, page0;
     int n_mt, unit_rows; // units per item and their rows
     int n_work;          // CTAs (CTA pairs) the blocks are dealt to
+    int bkv;             // rows of a block
     int out_al32;
     float scale_log2;
     int *status;
@@ -61,7 +64,7 @@ __device__ __forceinline__ float xa_max3(float a, float b, float c) {
 // The blocks of all units, and the piece of CTA `c` of `n`.
 __device__ __forceinline__ int xa_total_blocks(const CrossParams &p) {  // whole warp
     int sum = 0;
-    for (int b = threadIdx.x & 31; b < p.n_obs; b += 32) sum += (xa_len(p, b) + XA_BKV - 1) / XA_BKV;
+    for (int b = threadIdx.x & 31; b < p.n_obs; b += 32) sum += (xa_len(p, b) + p.bkv - 1) / p.bkv;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum * p.n_kv * p.n_mt;
@@ -75,20 +78,21 @@ struct XaSegment {  // a run of blocks [j0, j1) of one unit
 template <typename LenOf>
 struct XaWork {
     RaggedCursor<LenOf> cur;
-    int w, w1, w0, c, n_mt;
+    int w, w1, c, n_mt, bkv;
     bool whole_units;
-    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, int cta) : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV) {
+    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, int cta) : cur(f, p.n_obs, p.n_kv * p.n_mt, p.bkv) {
         const int total = xa_total_blocks(p), n = min(p.n_work, total);
         c = cta;
-        w = w0 = cta < n ? xa_border(cta, n, total) : total;
+        w = cta < n ? xa_border(cta, n, total) : total;
         w1 = cta < n ? xa_border(cta + 1, n, total) : total;
         n_mt = p.n_mt;
+        bkv = p.bkv;
         whole_units = p.ws_o == nullptr;
     }
     __device__ __forceinline__ bool next(XaSegment &s) {  // whole warp
         RaggedUnit u;
         while (w < w1 && cur.find(w, u)) {
-            const int nb = (u.len + XA_BKV - 1) / XA_BKV;
+            const int nb = (u.len + bkv - 1) / bkv;
             if (whole_units && u.block > 0) {  // begun by the CTA before, which finishes it
                 w += nb - u.block;
                 continue;
@@ -109,25 +113,23 @@ struct XaWork {
 
 template <int HD>
 struct CrossSmem {
-    static constexpr int CB = HD / 64;                // 64-element column blocks
-    static constexpr int Q_BYTES = CB * 128 * 128;    // a tile: [CB][128 rows][128 B]
-    static constexpr int KV_BYTES = CB * XA_BKV * 128;
-    static constexpr int STAGES = HD == 64 ? 4 : 2;
+    static constexpr int CB = HD / 64, BKV = xa_bkv<HD>();  // 64-element column blocks
+    static constexpr int Q_BYTES = CB * 128 * 128;          // a tile: [CB][128 rows][128 B]
+    static constexpr int KV_BYTES = CB * BKV * 128;
+    static constexpr int STAGES = 4;
     static constexpr int K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES, BAR_OFF = V_OFF + STAGES * KV_BYTES;
-    static constexpr int TOTAL = BAR_OFF + 256 + 1024;
-    static constexpr int S_COL = 2 * HD;  // O_0, O_1, S_0, S_1
-    static_assert(S_COL + 2 * XA_BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
+    static constexpr int TOTAL = BAR_OFF + 512 + 1024;
+    static constexpr int S_COL = 2 * HD;  // O_0, O_1, then two S buffers of each tile
+    static_assert(S_COL + 4 * BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
 };
 
 // Zeroes the rows of a V block in shared memory that the mask hides: they meet weights of 0, and 0 times what stands there need not be 0.
-// `tid` of 128 takes row tid; V: [n_cb][128 rows][128 B].
-__device__ __forceinline__ void xa_clean_v(uint8_t *v, int n_cb, int tid, int row, int len, int pad_lo, int pad_hi) {
-    if (row >= len || (row >= pad_lo && row < pad_hi)) {
-        for (int cb = 0; cb < n_cb; ++cb) {
-            uint4 *r = reinterpret_cast<uint4 *>(v + cb * (XA_BKV * 128) + tid * 128);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = make_uint4(0, 0, 0, 0);
-        }
+// 128 threads; V: [n_cb][ROWS][128 B], the first row being row0 of the page.
+template <int ROWS>
+__device__ __forceinline__ void xa_clean_v(uint8_t *v, int n_cb, int tid, int row0, int len, int pad_lo, int pad_hi) {
+    for (int i = tid; i < n_cb * ROWS * 8; i += 128) {
+        const int row = row0 + ((i >> 3) & (ROWS - 1));
+        if (row >= len || (row >= pad_lo && row < pad_hi)) reinterpret_cast<uint4 *>(v)[i] = make_uint4(0, 0, 0, 0);
     }
     fence_proxy_async_smem();
 }
@@ -157,13 +159,15 @@ __global__ void __launch_bounds__(XA_THREADS, 1)
 cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
     using L = CrossSmem<HD>;
+    constexpr int BKV = L::BKV;
     constexpr uint32_t NS = L::STAGES;
     extern __shared__ uint8_t xa_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xa_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
     uint64_t *q_full = bars, *q_free = bars + 1, *k_full = bars + 2, *k_free = bars + 6, *v_full = bars + 10, *v_free = bars + 14;
-    uint64_t *s_full = bars + 18, *p_full = bars + 20, *pv_done = bars + 22, *o_free = bars + 24;  // [2 tiles]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 26);
+    uint64_t *s_full = bars + 18, *p_full = bars + 22, *pv_done = bars + 26;  // [2 tiles][2 buffers]
+    uint64_t *o_free = bars + 30;                                             // [2 tiles]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 32);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{abort_flag, p.status};
@@ -177,12 +181,12 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             mbar_init(&v_full[i], 1);
             mbar_init(&v_free[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
-            mbar_init(&o_free[i], 4);
         }
+        for (int i = 0; i < 2; ++i) mbar_init(&o_free[i], 4);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -227,38 +231,40 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                 if (elect_one()) {
                     mbar_expect_tx(&k_full[st], L::KV_BYTES);
                     for (int cb = 0; cb < L::CB; ++cb)
-                        tma_load_3d(smem + L::K_OFF + st * L::KV_BYTES + cb * 16384, &k_map, &k_full[st], cb * 64, j * XA_BKV, p.page0 + item);
+                        tma_load_3d(smem + L::K_OFF + st * L::KV_BYTES + cb * (BKV * 128), &k_map, &k_full[st], cb * 64, j * BKV, p.page0 + item);
                 }
                 ok = warp_wait(&v_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                 if (!ok) break;
                 if (elect_one()) {
                     mbar_expect_tx(&v_full[st], L::KV_BYTES);
                     for (int cb = 0; cb < L::CB; ++cb)
-                        tma_load_3d(smem + L::V_OFF + st * L::KV_BYTES + cb * 16384, &v_map, &v_full[st], cb * 64, j * XA_BKV, p.page0 + item);
+                        tma_load_3d(smem + L::V_OFF + st * L::KV_BYTES + cb * (BKV * 128), &v_map, &v_full[st], cb * 64, j * BKV, p.page0 + item);
                 }
             }
         }
     } else if (warp == XA_MMA) {
-        constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, XA_BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
-        const uint32_t base = smem_u32(smem);
-        auto issue_s = [&](int t, uint32_t st) {
-            const uint32_t q = base + t * L::Q_BYTES, k = base + L::K_OFF + st * L::KV_BYTES, d = tmem_base + L::S_COL + t * XA_BKV;
+        constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
+        const uint64_t q_desc0 = smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc0 = smem_desc_sw128(smem_u32(smem) + L::K_OFF, 16, 1024);
+        const uint64_t v_desc0 = smem_desc_sw128(smem_u32(smem) + L::V_OFF, BKV * 128, 1024);
+        auto issue_s = [&](int t, uint32_t buf, uint32_t st) {
+            const uint64_t q = q_desc0 + (uint64_t)(t * (L::Q_BYTES >> 4)), k = k_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
+            const uint32_t d = tmem_base + L::S_COL + (t * 2 + buf) * BKV;
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
-                    mma_f16(d, smem_desc_sw128(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                            smem_desc_sw128(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
-                tc_commit(&s_full[t]);
+                    mma_f16(d, q + (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2), k + (uint64_t)((kk >> 2) * (BKV * 8) + (kk & 3) * 2), idesc_s,
+                            kk != 0 ? 1u : 0u);
+                tc_commit(&s_full[t * 2 + buf]);
             }
         };
-        auto issue_pv = [&](int t, uint32_t st, bool first) {
-            const uint32_t v = base + L::V_OFF + st * L::KV_BYTES, pt = tmem_base + L::S_COL + t * XA_BKV;
+        auto issue_pv = [&](int t, uint32_t buf, uint32_t st, bool first) {
+            const uint64_t v = v_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
+            const uint32_t pt = tmem_base + L::S_COL + (t * 2 + buf) * BKV;
             if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < XA_BKV / 16; ++kk)
-                    mma_f16_tmem_a(tmem_base + t * HD, pt + (uint32_t)(kk * 8), smem_desc_sw128(v + kk * 2048, 16384, 1024), idesc_o,
-                                   first && kk == 0 ? 0u : 1u);
-                tc_commit(&pv_done[t]);
+                for (int kk = 0; kk < BKV / 16; ++kk)
+                    mma_f16_tmem_a(tmem_base + t * HD, pt + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), idesc_o, first && kk == 0 ? 0u : 1u);
+                tc_commit(&pv_done[t * 2 + buf]);
             }
         };
         uint32_t si = 0, jb = 0;
@@ -266,41 +272,41 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         for (; ok && work.next(s); ++si) {
             const int tiles = p.R > s.mt * 256 + 128 ? 2 : 1;
             ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
-            if (ok) ok = warp_wait(&k_full[jb % NS], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-            if (!ok) break;
-            tc_fence_after();
-            // a tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order
-            for (int t = 0; t < tiles; ++t) issue_s(t, jb % NS);
-            if (elect_one()) {
-                tc_commit(&k_free[jb % NS]);
-                if (s.j1 - s.j0 == 1) tc_commit(q_free);
-            }
-            for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
-                const uint32_t st = jb % NS, ph = (jb / NS) & 1u, jn = jb + 1, sn = jn % NS;
-                for (int t = 0; t < tiles; ++t) {
-                    ok = warp_wait(&p_full[t], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
-                    if (ok && t == 0) ok = warp_wait(&v_full[st], ph, wc, DEV_TIMEOUT_FULL);
-                    if (ok && j == s.j0) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
-                    if (ok && t == 0 && j + 1 < s.j1) ok = warp_wait(&k_full[sn], (jn / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+            // an S buffer held the P of the tile's block before last: that P V was issued before, and the pipe keeps the order
+            for (int j = s.j0; ok && j <= s.j1; ++j) {  // S of block j, then P V of block j - 1
+                if (j < s.j1) {
+                    const uint32_t jn = jb + (uint32_t)(j - s.j0), st = jn % NS;
+                    ok = warp_wait(&k_full[st], (jn / NS) & 1u, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(t, st, j == s.j0);
-                    ++blk[t];
-                    if (j + 1 < s.j1) issue_s(t, sn);
+                    for (int t = 0; t < tiles; ++t) issue_s(t, (blk[t] + (j > s.j0 ? 1u : 0u)) & 1u, st);
+                    if (elect_one()) {
+                        tc_commit(&k_free[st]);
+                        if (j + 1 == s.j1) tc_commit(q_free);  // the segment's last S blocks have been issued
+                    }
                 }
-                if (!ok) break;
-                if (elect_one()) {
-                    tc_commit(&v_free[st]);
-                    if (j + 1 < s.j1) tc_commit(&k_free[sn]);
-                    if (j + 2 == s.j1) tc_commit(q_free);  // the segment's last S blocks have been issued
+                if (j > s.j0) {
+                    const uint32_t jp = jb + (uint32_t)(j - 1 - s.j0), st = jp % NS;
+                    for (int t = 0; t < tiles; ++t) {
+                        const uint32_t buf = blk[t] & 1u;
+                        ok = warp_wait(&p_full[t * 2 + buf], (blk[t] >> 1) & 1u, wc, DEV_TIMEOUT_FULL);
+                        if (ok && t == 0) ok = warp_wait(&v_full[st], (jp / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                        if (ok && j == s.j0 + 1) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_pv(t, buf, st, j == s.j0 + 1);
+                        ++blk[t];
+                    }
+                    if (ok && elect_one()) tc_commit(&v_free[st]);
                 }
             }
+            jb += (uint32_t)(s.j1 - s.j0);
             for (int t = 0; t < tiles; ++t) ++seg[t];
         }
     } else {
         const int t = warp >> 2, qtr = warp & 3;
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
-        const uint32_t s_addr = tmem_base + L::S_COL + t * XA_BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
+        const uint32_t s_addr0 = tmem_base + L::S_COL + t * 2 * BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
         uint32_t blk = 0;  // blocks of this tile so far; tile 0 has every block of the CTA
         while (ok && work.next(s)) {
@@ -316,20 +322,21 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             if (pad_hi <= pad_lo) pad_lo = pad_hi = 0x7fffffff;
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units, row sum
             for (int j = s.j0; j < s.j1; ++j, ++blk) {
-                ok = warp_wait(&s_full[t], blk & 1u, wc, DEV_TIMEOUT_FULL);
+                const uint32_t buf = blk & 1u, s_addr = s_addr0 + buf * BKV;
+                ok = warp_wait(&s_full[t * 2 + buf], (blk >> 1) & 1u, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
                 tc_fence_after();
-                const int c0 = j * XA_BKV;
-                const bool dirty = c0 + XA_BKV > s.len || (c0 < pad_hi && c0 + XA_BKV > pad_lo);
+                const int c0 = j * BKV;
+                const bool dirty = c0 + BKV > s.len || (c0 < pad_hi && c0 + BKV > pad_lo);
                 if (live) {
-                    uint32_t x[4][32];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + (uint32_t)(i * 32), x[i]);
+                    uint32_t x[2][32];
+                    tmem_ld32(s_addr, x[0]);
+                    tmem_ld32(s_addr + 32, x[1]);
                     tmem_ld_wait();
                     if (dirty) {
                         const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 const int c = i * 32 + e;
@@ -339,9 +346,10 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     float mx[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        mx[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
+                        const uint32_t *y = &x[i >> 1][(i & 1) * 16];
+                        mx[i] = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 #pragma unroll
-                        for (int e = 2; e < 32; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
+                        for (int e = 2; e < 16; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
                     }
                     const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
                     float factor = 1.0f;
@@ -352,7 +360,8 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                         l_sum *= factor;
                     }
                     if (j > s.j0 && __any_sync(0xffffffffu, raise)) {  // O was summed under the old maximum
-                        ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+                        const uint32_t bp = blk - 1;
+                        ok = warp_wait(&pv_done[t * 2 + (bp & 1u)], (bp >> 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -368,20 +377,17 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     const float mref = m_used == -INFINITY ? 0.0f : m_used;
                     const F2 neg = f2(-mref, -mref);
                     F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+                    uint32_t pk[32];
 #pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        uint32_t pk[32];
-#pragma unroll
-                        for (int e = 0; e < 64; e += 2) {
-                            const F2 a = f2_fma(f2(__uint_as_float(x[i + (e >> 5)][e & 31]), __uint_as_float(x[i + (e >> 5)][(e & 31) + 1])), scale2, neg);
-                            float a0, a1;
-                            f2_get(a, a0, a1);
-                            const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
-                            sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
-                            pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
-                        }
-                        tmem_st32(s_addr + (uint32_t)(i * 16), pk);
+                    for (int e = 0; e < 64; e += 2) {
+                        const F2 a = f2_fma(f2(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])), scale2, neg);
+                        float a0, a1;
+                        f2_get(a, a0, a1);
+                        const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
+                        sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
+                        pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
                     }
+                    tmem_st32(s_addr, pk);
                     float u0, u1, u2, u3;
                     f2_get(sum[0], u0, u1);
                     f2_get(sum[1], u2, u3);
@@ -392,15 +398,15 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     const uint32_t st = blk % NS;
                     ok = warp_wait(&v_full[st], (blk / NS) & 1u, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
-                    xa_clean_v(smem + L::V_OFF + st * L::KV_BYTES, L::CB, threadIdx.x, c0 + (int)threadIdx.x, s.len, pad_lo, pad_hi);
+                    xa_clean_v<BKV>(smem + L::V_OFF + st * L::KV_BYTES, L::CB, threadIdx.x, c0, s.len, pad_lo, pad_hi);
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
+                if (lane == 0) mbar_arrive(&p_full[t * 2 + buf]);
             }
             if (!ok) break;
             // ---- O / l -> bf16 -> out, or the piece into the workspace ----
-            ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+            ok = warp_wait(&pv_done[t * 2 + ((blk - 1) & 1u)], ((blk - 1) >> 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
             if (!ok) break;
             tc_fence_after();
             const bool row_ok = row < p.R;
@@ -468,7 +474,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XP_THREADS, 1)
 cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
     using L = CrossPairSmem;
-    constexpr int HD = L::HD;
+    constexpr int HD = L::HD, BKV = xa_bkv<HD>();
     constexpr uint32_t ST = L::STAGES, NS = L::NS;
     extern __shared__ uint8_t xp_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xp_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -548,7 +554,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 if (elect_one()) {
                     mbar_expect_tx(&k_full[st], L::K_BYTES);
                     for (int cb = 0; cb < L::CB; ++cb)
-                        tma_load_3d(smem + L::K_OFF + st * L::K_BYTES + cb * 8192, &k_map, &k_full[st], cb * 64, j * XA_BKV + (int)rank * 64,
+                        tma_load_3d(smem + L::K_OFF + st * L::K_BYTES + cb * 8192, &k_map, &k_full[st], cb * 64, j * BKV + (int)rank * 64,
                                     p.page0 + item);
                 }
                 ok = warp_wait(&v_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
@@ -557,13 +563,13 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     mbar_expect_tx(&v_full[st], L::V_BYTES);
                     for (int cb = 0; cb < L::CBH; ++cb)
                         tma_load_3d(smem + L::V_OFF + st * L::V_BYTES + cb * 16384, &v_map, &v_full[st], ((int)rank * L::CBH + cb) * 64,
-                                    j * XA_BKV, p.page0 + item);
+                                    j * BKV, p.page0 + item);
                 }
             }
         }
     } else if (warp == XP_S) {
         if (rank == 0) {
-            constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 256, XA_BKV);
+            constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 256, BKV);
             const uint64_t q_desc0 = smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc0 = smem_desc_sw128(smem_u32(smem) + L::K_OFF, 16, 1024);
             for (; ok && work.next(s); ++si) {
                 ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
@@ -590,7 +596,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     ok = __all_sync(0xffffffffu, ok) != 0;
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t st = jb % ST, d = tmem_base + HD + (jb % NS) * XA_BKV;
+                    const uint32_t st = jb % ST, d = tmem_base + HD + (jb % NS) * BKV;
                     const uint64_t k_desc = k_desc0 + (uint64_t)(st * (L::K_BYTES >> 4));
                     if (elect_one()) {
 #pragma unroll
@@ -632,10 +638,10 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t v_desc = v_desc0 + (uint64_t)(st * (L::V_BYTES >> 4));
-                    const uint32_t p_tmem = tmem_base + HD + sb * XA_BKV;
+                    const uint32_t p_tmem = tmem_base + HD + sb * BKV;
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < XA_BKV / 16; ++kk)
+                        for (int kk = 0; kk < BKV / 16; ++kk)
                             mma_f16_tmem_a_pair(tmem_base, p_tmem + (uint32_t)(kk * 8), v_desc + (uint64_t)(kk * 128), idesc_o,
                                                 j != s.j0 || kk != 0 ? 1u : 0u);
                         *pv_issued = jb + 1u;
@@ -717,7 +723,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units (the same in both halves), this half's part of the row sum
             for (int j = s.j0; j < s.j1; ++j, ++jb) {
                 const uint32_t sb = jb % NS;
-                const uint32_t s_addr = tmem_base + HD + sb * XA_BKV + lane_sel;
+                const uint32_t s_addr = tmem_base + HD + sb * BKV + lane_sel;
                 ok = warp_wait(&s_full[sb], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
                 tc_fence_after();
@@ -725,8 +731,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 tmem_ld32(s_addr + (uint32_t)(half * 64), x[0]);
                 tmem_ld32(s_addr + (uint32_t)(half * 64 + 32), x[1]);
                 tmem_ld_wait();
-                const int b0 = j * XA_BKV, c0 = b0 + half * 64;
-                const bool dirty = b0 + XA_BKV > s.len || (b0 < pad_hi && b0 + XA_BKV > pad_lo);
+                const int b0 = j * BKV, c0 = b0 + half * 64;
+                const bool dirty = b0 + BKV > s.len || (b0 < pad_hi && b0 + BKV > pad_lo);
                 if (dirty) {
                     const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
 #pragma unroll
@@ -796,7 +802,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     const uint32_t st = jb % ST;
                     ok = warp_wait(&v_full[st], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
-                    xa_clean_v(smem + L::V_OFF + st * L::V_BYTES, L::CBH, threadIdx.x, b0 + (int)threadIdx.x, s.len, pad_lo, pad_hi);
+                    xa_clean_v<128>(smem + L::V_OFF + st * L::V_BYTES, L::CBH, threadIdx.x, b0, s.len, pad_lo, pad_hi);
                 }
                 tc_fence_before();
                 arrive_even(&p_full[sb]);
@@ -822,54 +828,61 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
 }
 
 // Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Rows of empty
-// observations: 0 and -inf.  A warp per row; rows of whole units are done.
-template <int HD>
+// observations: 0 and -inf.  Block x < n_work looks after the unit that CTA x began and did not finish, the others after one observation
+// each, if it is empty.  TEAM warps share a row: 1 where a unit's rows are many (two pieces or three of each), 8 where they are few and the
+// pieces as many as there are CTAs (one token over 16,001 rows, a warp per row: 40 us).
+template <int HD, int TEAM>
 __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p) {
+    __shared__ __align__(8) float s_o[8][TEAM > 1 ? HD : 1], s_l[8];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int item = blockIdx.y + (int)gridDim.y * blockIdx.z;
-    if (item >= p.n_obs * p.n_kv) return;
-    const int obs = item / p.n_kv, kvh = item % p.n_kv, row = blockIdx.x * 8 + warp;
-    const int nb = (xa_len(p, obs) + XA_BKV - 1) / XA_BKV;
-    if (nb > 0 && p.ws_o == nullptr) return;
-    int c0 = 0, c1 = 0;
-    if (nb > 0) {
-        int before = 0;
-        for (int b = lane; b < obs; b += 32) before += (xa_len(p, b) + XA_BKV - 1) / XA_BKV;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
-        const int total = xa_total_blocks(p), n = min(p.n_work, total);
-        const int at = (before * p.n_kv + nb * kvh) * p.n_mt + nb * (row / p.unit_rows);
-        c0 = (int)(((long long)(at + 1) * n - 1) / total);  // the CTA that has block w: the last whose piece begins at or before w
-        c1 = (int)(((long long)(at + nb) * n - 1) / total);
-        if (c0 == c1) return;
+    if ((int)blockIdx.x >= p.n_work) {
+        const int obs = blockIdx.x - p.n_work;
+        if (xa_len(p, obs) > 0) return;
+        const long long n = (long long)p.n_q * p.S;  // rows of the observation
+        uint4 *out = reinterpret_cast<uint4 *>(p.out + obs * n * HD);
+        for (long long i = (long long)blockIdx.y * 256 + threadIdx.x; i < n * (HD / 8); i += 256LL * gridDim.y) out[i] = make_uint4(0, 0, 0, 0);
+        if (p.lse)
+            for (long long i = (long long)blockIdx.y * 256 + threadIdx.x; i < n; i += 256LL * gridDim.y) p.lse[obs * n + i] = -INFINITY;
+        return;
     }
-    if (row >= p.R) return;
-    const int head = kvh * p.g + row / p.S, tok = row % p.S;
+    if (p.ws_o == nullptr) return;
+    const int c0 = blockIdx.x, total = xa_total_blocks(p), n = min(p.n_work, total);
+    if (c0 >= n) return;
+    const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
+    auto len_of = [&](int obs) { return xa_len(p, obs); };
+    RaggedCursor cur(len_of, p.n_obs, p.n_kv * p.n_mt, p.bkv);
+    RaggedUnit u;
+    if (!cur.find(end - 1, u)) return;
+    const int nb = (u.len + p.bkv - 1) / p.bkv, first = end - 1 - u.block;  // of the unit of the CTA's last block
+    if (first < begin || first + nb <= end) return;                         // begun before this CTA, or whole
+    const int c1 = (int)(((long long)(first + nb) * n - 1) / total);        // the CTA that has the unit's last block
+    const int kvh = u.kvh / p.n_mt, row0 = (u.kvh - kvh * p.n_mt) * p.unit_rows, rows = min(p.R - row0, p.unit_rows);
     constexpr int NV = HD / 64;  // pairs of columns per lane
-    float2 acc[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = make_float2(0.0f, 0.0f);
-    float l = 0.0f, M = -INFINITY;
-    if (nb > 0) {
-        const int lr = row % p.unit_rows;
+    for (int r0 = blockIdx.y * (8 / TEAM); r0 < rows; r0 += gridDim.y * (8 / TEAM)) {
+        const int lr = r0 + warp / TEAM, member = warp % TEAM;
+        if (TEAM == 1 && lr >= rows) return;
         auto slot_of = [&](int c) { return (long long)(2 * c + (c == c0 ? 1 : 0)) * p.ws_rows + lr; };
+        float2 acc[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] = make_float2(0.0f, 0.0f);
+        float l = 0.0f, M = -INFINITY;
         for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, p.ws_ml[slot_of(c) * 2]);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        for (int c = c0; c <= c1; c += 4) {
+        for (int c = c0 + member; c <= c1; c += 4 * TEAM) {
             float2 v[4][NV], ml[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const long long at = slot_of(min(c + i, c1));
+                const long long at = slot_of(min(c + i * TEAM, c1));
                 ml[i] = *reinterpret_cast<const float2 *>(p.ws_ml + at * 2);
 #pragma unroll
                 for (int k = 0; k < NV; ++k) v[i][k] = reinterpret_cast<const float2 *>(p.ws_o + at * HD)[k * 32 + lane];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (c + i > c1) break;
+                if (c + i * TEAM > c1) break;
                 const float w = ml[i].x == -INFINITY ? 0.0f : xa_ex2(ml[i].x - M);
                 l = fmaf(ml[i].y, w, l);
 #pragma unroll
@@ -879,12 +892,41 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
                 }
             }
         }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    __nv_bfloat162 *dst = reinterpret_cast<__nv_bfloat162 *>(p.out + (((long long)obs * p.S + tok) * p.n_q + head) * HD);
+        const int row = row0 + lr, head = kvh * p.g + row / p.S, tok = row % p.S;
+        __nv_bfloat16 *dst = p.out + (((long long)u.obs * p.S + tok) * p.n_q + head) * HD;
+        if (TEAM > 1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) dst[k * 32 + lane] = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv);
-    if (p.lse && lane == 0) p.lse[((long long)obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+            for (int k = 0; k < NV; ++k) reinterpret_cast<float2 *>(s_o[warp])[k * 32 + lane] = acc[k];
+            if (lane == 0) s_l[warp] = l;
+            __syncthreads();
+            l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < TEAM; ++w) l += s_l[w];
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            for (int i = threadIdx.x; i < HD; i += 256) {
+                float o = 0.0f;
+#pragma unroll
+                for (int w = 0; w < TEAM; ++w) o += s_o[w][i];
+                dst[i] = __float2bfloat16_rn(o * inv);
+            }
+            __syncthreads();
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                reinterpret_cast<__nv_bfloat162 *>(dst)[k * 32 + lane] = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv);
+        }
+        if (p.lse && lane == 0 && member == 0)
+            p.lse[((long long)u.obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+    }
+}
+
+template <int HD>
+static int launch_combine(const CrossParams &p, cudaStream_t stream) {
+    const unsigned gx = (unsigned)(p.n_work + p.n_obs);
+    if (p.ws_rows <= 64)  // a row per block
+        return launch_pdl(cross_combine_kernel<HD, 8>, dim3(gx, (unsigned)p.ws_rows), dim3(256), 0, stream, p);
+    return launch_pdl(cross_combine_kernel<HD, 1>, dim3(gx, 8), dim3(256), 0, stream, p);  // 32 rows per block
 }
 
 // Units, workers and workspace of a call; the same for the size query and the launch.
@@ -908,10 +950,10 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
     CUtensorMap qmap, kmap, vmap;
     const uint64_t qdims[3] = {(uint64_t)HD, (uint64_t)p.R, (uint64_t)st->n_obs * st->n_kv}, qstr[2] = {(uint64_t)HD * 2, (uint64_t)p.R * HD * 2};
     const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)p.max_len, pages}, str[2] = {(uint64_t)HD * 2, (uint64_t)st->cap * HD * 2};
-    const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, HD == 256 ? 64 : 128, 1};
+    const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, 64, 1};  // pairs stage half of a block's K rows, and all of its V rows
     int rc = make_tensor_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, qdims, qstr, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = make_tensor_map(&kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->k_pages, dims, str, kbox, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, HD == 256 ? box : kbox, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     if constexpr (HD == 256) {
         if ((rc = ensure_dyn_smem(cross_attn_pair_kernel, CrossPairSmem::TOTAL))) return rc;
@@ -921,8 +963,7 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
         rc = launch_pdl(cross_attn_kernel<HD>, dim3((unsigned)plan.n_work), dim3(XA_THREADS), CrossSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
     }
     if (rc) return rc;
-    const int items = st->n_obs * st->n_kv, gy = items < 32768 ? items : 32768;
-    return launch_pdl(cross_combine_kernel<HD>, dim3((unsigned)((p.R + 7) / 8), (unsigned)gy, (unsigned)((items + gy - 1) / gy)), dim3(256), 0, stream, p);
+    return launch_combine<HD>(p, stream);
 }
 
 static bool cross_shape_ok(const vlab200_kv_store *st, int S, int n_q) {
@@ -950,9 +991,9 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     const int hd = st->head_dim;
     if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
     const long long R = (long long)(n_q / st->n_kv) * S, items = (long long)st->n_obs * st->n_kv;
-    const long long blocks = items * ((R + 127) / 128) * ((max_len + 127LL) / 128);
-    if (R > 0x7fffff00LL || items * st->n_layers > 0x7fffff00LL || items > 32768LL * 65535 || blocks > 0x7fffff00LL) {
-        vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 128 x 128 scores");
+    const long long blocks = items * ((R + 255) / 256) * ((max_len + 63LL) / 64);
+    if (R > 0x7fffff00LL || items * st->n_layers > 0x7fffff00LL || blocks > 0x7fffff00LL) {
+        vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 256 x 64 scores");
         return VLAB200_ERR_UNSUPPORTED;
     }
     const int n_sm = vb::sm_count();
@@ -975,6 +1016,7 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     p.n_mt = plan.n_mt;
     p.unit_rows = plan.unit_rows;
     p.n_work = plan.n_work;
+    p.bkv = hd == 256 ? vb::xa_bkv<256>() : vb::xa_bkv<64>();
     p.out_al32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0 ? 1 : 0;
     p.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)hd));
     p.status = vb::device_status_ptr();
@@ -985,10 +1027,8 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     if (max_len == 0) {  // nothing to map: every row is that of an empty observation
         p.lens = nullptr;
-        const int gy = items < 32768 ? (int)items : 32768;
-        const dim3 grid((unsigned)((R + 7) / 8), (unsigned)gy, (unsigned)((items + gy - 1) / gy));
-        auto kernel = hd == 64 ? vb::cross_combine_kernel<64> : hd == 128 ? vb::cross_combine_kernel<128> : vb::cross_combine_kernel<256>;
-        return vb::launch_pdl(kernel, grid, dim3(256), 0, cs, p);
+        p.n_work = 0;
+        return hd == 64 ? vb::launch_combine<64>(p, cs) : hd == 128 ? vb::launch_combine<128>(p, cs) : vb::launch_combine<256>(p, cs);
     }
     if (hd == 64) return vb::launch_cross<64>(st, q, p, plan, cs);
     if (hd == 128) return vb::launch_cross<128>(st, q, p, plan, cs);
