@@ -6,10 +6,12 @@
 //
 // Heads of 64 and 128, a unit = (observation, kv head, 256 of the g S stacked query rows), one CTA:
 //   loader warp       TMA: the two 128-row Q tiles of a unit, K and V in blocks of 128 rows through rings
-//   MMA warp          S_t = Q_t K_j^T of both tiles t = 0, 1, then O_t += P_t V_(j-1) with P_t read from TMEM
+//   MMA warp          O_t += P_t V_j with P_t read from TMEM, in two halves of the block's rows, then S_t = Q_t K_(j+1)^T, for the tiles
+//                     t = 0, 1 in turn, so that the tensor pipe works on one tile while the other is in its softmax
 //   2 x 4 warps       one per tile and lane quarter, a row per thread: maximum, 2^(s c - m), row sum, P over S in TMEM
-// TMEM: O_0, O_1 and two S buffers per tile (512 columns at heads of 128).  Both the exponentials (16 per clock and SM) and the products
-// need 512 clocks per tile and block of 64 at heads of 128; at 64 the exponentials bound it.
+// TMEM: O_0, O_1 and one S per tile (512 columns at heads of 128).  Both the exponentials (16 per clock and SM) and the products need
+// 1,024 clocks per tile and block at heads of 128; at 64 the exponentials bound it.  Blocks of 64 rows with two S buffers per tile were
+// slower: a product whose A comes from shared memory takes 64 clocks a step of 16 whether N is 64 or 128.
 //
 // Work is dealt out in blocks, not units: the units' blocks form one list and every CTA takes an equal piece of it, so neither ragged
 // lengths nor few units leave SMs idle.  A unit cut by a piece's border leaves un-normalised rows with their maximum and sum in the
@@ -23,12 +25,11 @@
 
 namespace vb {
 
-// Rows of K / V per block.  Heads of 64 and 128: 64, so that a tile has two S buffers and its next scores are ready when its softmax
-// is (with one S of 128 a block took 5,000 clocks, softmax and products of a tile in turn, against 2,050 of either).
-template <int HD>
-constexpr int xa_bkv() { return HD == 256 ? 128 : 64; }
-constexpr int XA_THREADS = 320;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA
+constexpr int XA_BKV = 128;      // rows of K / V per block
+constexpr int XA_THREADS = 384;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA, 10 and 11 fill the warpgroup that gives up registers
 constexpr int XA_LOADER = 8, XA_MMA = 9;
+// Registers of a thread: 384 x 168 at launch = 64,512; 2 x 128 x 208 + 128 x 88 = 64,512 after the split.
+constexpr int XA_REGS_SOFTMAX = 208, XA_REGS_REST = 88;
 constexpr float XA_RAISE = 8.0f; // the running maximum is raised, and O rescaled, only by blocks that exceed it by more than 2^8
 
 struct CrossParams {
@@ -38,7 +39,6 @@ struct CrossParams {
     int S, n_q, n_kv, g, R, n_obs, max_len, page0;
     int n_mt, unit_rows; // units per item and their rows
     int n_work;          // CTAs (CTA pairs) the blocks are dealt to
-    int bkv;             // rows of a block
     int out_al32;
     float scale_log2;
     int *status;
@@ -64,7 +64,7 @@ __device__ __forceinline__ float xa_max3(float a, float b, float c) {
 // The blocks of all units, and the piece of CTA `c` of `n`.
 __device__ __forceinline__ int xa_total_blocks(const CrossParams &p) {  // whole warp
     int sum = 0;
-    for (int b = threadIdx.x & 31; b < p.n_obs; b += 32) sum += (xa_len(p, b) + p.bkv - 1) / p.bkv;
+    for (int b = threadIdx.x & 31; b < p.n_obs; b += 32) sum += (xa_len(p, b) + XA_BKV - 1) / XA_BKV;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum * p.n_kv * p.n_mt;
@@ -78,21 +78,20 @@ struct XaSegment {  // a run of blocks [j0, j1) of one unit
 template <typename LenOf>
 struct XaWork {
     RaggedCursor<LenOf> cur;
-    int w, w1, c, n_mt, bkv;
+    int w, w1, c, n_mt;
     bool whole_units;
-    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, int cta) : cur(f, p.n_obs, p.n_kv * p.n_mt, p.bkv) {
+    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, int cta) : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV) {
         const int total = xa_total_blocks(p), n = min(p.n_work, total);
         c = cta;
         w = cta < n ? xa_border(cta, n, total) : total;
         w1 = cta < n ? xa_border(cta + 1, n, total) : total;
         n_mt = p.n_mt;
-        bkv = p.bkv;
         whole_units = p.ws_o == nullptr;
     }
     __device__ __forceinline__ bool next(XaSegment &s) {  // whole warp
         RaggedUnit u;
         while (w < w1 && cur.find(w, u)) {
-            const int nb = (u.len + bkv - 1) / bkv;
+            const int nb = (u.len + XA_BKV - 1) / XA_BKV;
             if (whole_units && u.block > 0) {  // begun by the CTA before, which finishes it
                 w += nb - u.block;
                 continue;
@@ -113,14 +112,14 @@ struct XaWork {
 
 template <int HD>
 struct CrossSmem {
-    static constexpr int CB = HD / 64, BKV = xa_bkv<HD>();  // 64-element column blocks
+    static constexpr int CB = HD / 64, BKV = XA_BKV;  // 64-element column blocks
     static constexpr int Q_BYTES = CB * 128 * 128;          // a tile: [CB][128 rows][128 B]
     static constexpr int KV_BYTES = CB * BKV * 128;
-    static constexpr int STAGES = 4;
+    static constexpr int STAGES = HD == 64 ? 4 : 2;
     static constexpr int K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES, BAR_OFF = V_OFF + STAGES * KV_BYTES;
     static constexpr int TOTAL = BAR_OFF + 512 + 1024;
-    static constexpr int S_COL = 2 * HD;  // O_0, O_1, then two S buffers of each tile
-    static_assert(S_COL + 4 * BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
+    static constexpr int S_COL = 2 * HD;  // O_0, O_1, S_0, S_1
+    static_assert(S_COL + 2 * BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
 };
 
 // Zeroes the rows of a V block in shared memory that the mask hides: they meet weights of 0, and 0 times what stands there need not be 0.
@@ -165,9 +164,9 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xa_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
     uint64_t *q_full = bars, *q_free = bars + 1, *k_full = bars + 2, *k_free = bars + 6, *v_full = bars + 10, *v_free = bars + 14;
-    uint64_t *s_full = bars + 18, *p_full = bars + 22, *pv_done = bars + 26;  // [2 tiles][2 buffers]
-    uint64_t *o_free = bars + 30;                                             // [2 tiles]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 32);
+    uint64_t *s_full = bars + 18, *pv_done = bars + 20, *o_free = bars + 22;  // [2 tiles]
+    uint64_t *p_full = bars + 24;                                             // [2 tiles][2 halves of a block's rows]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 28);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{abort_flag, p.status};
@@ -181,12 +180,12 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             mbar_init(&v_full[i], 1);
             mbar_init(&v_free[i], 1);
         }
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
+            mbar_init(&o_free[i], 4);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(&o_free[i], 4);
+        for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -212,6 +211,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     bool ok = true;
 
     if (warp == XA_LOADER) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
         uint32_t si = 0, jb = 0;
         for (; ok && work.next(s); ++si) {
             const int item = s.obs * p.n_kv + s.kvh, row0 = s.mt * 256;
@@ -243,28 +243,30 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             }
         }
     } else if (warp == XA_MMA) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
         constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
         const uint64_t q_desc0 = smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc0 = smem_desc_sw128(smem_u32(smem) + L::K_OFF, 16, 1024);
         const uint64_t v_desc0 = smem_desc_sw128(smem_u32(smem) + L::V_OFF, BKV * 128, 1024);
-        auto issue_s = [&](int t, uint32_t buf, uint32_t st) {
+        auto issue_s = [&](int t, uint32_t st) {
             const uint64_t q = q_desc0 + (uint64_t)(t * (L::Q_BYTES >> 4)), k = k_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
-            const uint32_t d = tmem_base + L::S_COL + (t * 2 + buf) * BKV;
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
-                    mma_f16(d, q + (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2), k + (uint64_t)((kk >> 2) * (BKV * 8) + (kk & 3) * 2), idesc_s,
-                            kk != 0 ? 1u : 0u);
-                tc_commit(&s_full[t * 2 + buf]);
+                    mma_f16(tmem_base + L::S_COL + t * BKV, q + (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2),
+                            k + (uint64_t)((kk >> 2) * (BKV * 8) + (kk & 3) * 2), idesc_s, kk != 0 ? 1u : 0u);
+                tc_commit(&s_full[t]);
             }
         };
-        auto issue_pv = [&](int t, uint32_t buf, uint32_t st, bool first) {
+        auto issue_pv = [&](int t, uint32_t st, int h, bool first) {  // half h of the block's rows
             const uint64_t v = v_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
-            const uint32_t pt = tmem_base + L::S_COL + (t * 2 + buf) * BKV;
+            const uint32_t pt = tmem_base + L::S_COL + t * BKV;
             if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < BKV / 16; ++kk)
+                for (int k = 0; k < BKV / 32; ++k) {
+                    const int kk = h * (BKV / 32) + k;
                     mma_f16_tmem_a(tmem_base + t * HD, pt + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), idesc_o, first && kk == 0 ? 0u : 1u);
-                tc_commit(&pv_done[t * 2 + buf]);
+                }
+                if (h) tc_commit(&pv_done[t]);
             }
         };
         uint32_t si = 0, jb = 0;
@@ -272,41 +274,48 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         for (; ok && work.next(s); ++si) {
             const int tiles = p.R > s.mt * 256 + 128 ? 2 : 1;
             ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
-            // an S buffer held the P of the tile's block before last: that P V was issued before, and the pipe keeps the order
-            for (int j = s.j0; ok && j <= s.j1; ++j) {  // S of block j, then P V of block j - 1
-                if (j < s.j1) {
-                    const uint32_t jn = jb + (uint32_t)(j - s.j0), st = jn % NS;
-                    ok = warp_wait(&k_full[st], (jn / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+            if (ok) ok = warp_wait(&k_full[jb % NS], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            // a tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order
+            for (int t = 0; t < tiles; ++t) issue_s(t, jb % NS);
+            if (elect_one()) {
+                tc_commit(&k_free[jb % NS]);
+                if (s.j1 - s.j0 == 1) tc_commit(q_free);
+            }
+            for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
+                const uint32_t st = jb % NS, sn = (jb + 1) % NS;
+                const bool more = j + 1 < s.j1;
+                for (int t = 0; ok && t < tiles; ++t) {
+                    ok = warp_wait(&p_full[2 * t], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (ok && t == 0) ok = warp_wait(&v_full[st], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (ok && j == s.j0) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int t = 0; t < tiles; ++t) issue_s(t, (blk[t] + (j > s.j0 ? 1u : 0u)) & 1u, st);
-                    if (elect_one()) {
-                        tc_commit(&k_free[st]);
-                        if (j + 1 == s.j1) tc_commit(q_free);  // the segment's last S blocks have been issued
-                    }
+                    issue_pv(t, st, 0, j == s.j0);
+                    if (t == 0 && more) ok = warp_wait(&k_full[sn], ((jb + 1) / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (ok) ok = warp_wait(&p_full[2 * t + 1], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(t, st, 1, false);
+                    if (more) issue_s(t, sn);
+                    ++blk[t];
                 }
-                if (j > s.j0) {
-                    const uint32_t jp = jb + (uint32_t)(j - 1 - s.j0), st = jp % NS;
-                    for (int t = 0; t < tiles; ++t) {
-                        const uint32_t buf = blk[t] & 1u;
-                        ok = warp_wait(&p_full[t * 2 + buf], (blk[t] >> 1) & 1u, wc, DEV_TIMEOUT_FULL);
-                        if (ok && t == 0) ok = warp_wait(&v_full[st], (jp / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-                        if (ok && j == s.j0 + 1) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_pv(t, buf, st, j == s.j0 + 1);
-                        ++blk[t];
-                    }
-                    if (ok && elect_one()) tc_commit(&v_free[st]);
+                if (ok && elect_one()) {
+                    tc_commit(&v_free[st]);
+                    if (more) tc_commit(&k_free[sn]);
+                    if (j + 2 == s.j1) tc_commit(q_free);  // the segment's last S blocks have been issued
                 }
             }
-            jb += (uint32_t)(s.j1 - s.j0);
             for (int t = 0; t < tiles; ++t) ++seg[t];
         }
+    } else if (warp > XA_MMA) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));  // fills the warpgroup
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XA_REGS_SOFTMAX));
         const int t = warp >> 2, qtr = warp & 3;
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
-        const uint32_t s_addr0 = tmem_base + L::S_COL + t * 2 * BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
+        const uint32_t s_addr = tmem_base + L::S_COL + t * BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
         uint32_t blk = 0;  // blocks of this tile so far; tile 0 has every block of the CTA
         while (ok && work.next(s)) {
@@ -322,21 +331,21 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             if (pad_hi <= pad_lo) pad_lo = pad_hi = 0x7fffffff;
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units, row sum
             for (int j = s.j0; j < s.j1; ++j, ++blk) {
-                const uint32_t buf = blk & 1u, s_addr = s_addr0 + buf * BKV;
-                ok = warp_wait(&s_full[t * 2 + buf], (blk >> 1) & 1u, wc, DEV_TIMEOUT_FULL);
+                ok = warp_wait(&s_full[t], blk & 1u, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
                 tc_fence_after();
                 const int c0 = j * BKV;
                 const bool dirty = c0 + BKV > s.len || (c0 < pad_hi && c0 + BKV > pad_lo);
+                uint32_t x[4][32];
+                float mref = 0.0f;
                 if (live) {
-                    uint32_t x[2][32];
-                    tmem_ld32(s_addr, x[0]);
-                    tmem_ld32(s_addr + 32, x[1]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + (uint32_t)(i * 32), x[i]);
                     tmem_ld_wait();
                     if (dirty) {
                         const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 const int c = i * 32 + e;
@@ -346,10 +355,9 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     float mx[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t *y = &x[i >> 1][(i & 1) * 16];
-                        mx[i] = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+                        mx[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
 #pragma unroll
-                        for (int e = 2; e < 16; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+                        for (int e = 2; e < 32; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
                     }
                     const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
                     float factor = 1.0f;
@@ -360,8 +368,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                         l_sum *= factor;
                     }
                     if (j > s.j0 && __any_sync(0xffffffffu, raise)) {  // O was summed under the old maximum
-                        const uint32_t bp = blk - 1;
-                        ok = warp_wait(&pv_done[t * 2 + (bp & 1u)], (bp >> 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+                        ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -374,25 +381,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                             tmem_st16(o_addr + (uint32_t)c, ov);
                         }
                     }
-                    const float mref = m_used == -INFINITY ? 0.0f : m_used;
-                    const F2 neg = f2(-mref, -mref);
-                    F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int e = 0; e < 64; e += 2) {
-                        const F2 a = f2_fma(f2(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])), scale2, neg);
-                        float a0, a1;
-                        f2_get(a, a0, a1);
-                        const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
-                        sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
-                        pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
-                    }
-                    tmem_st32(s_addr, pk);
-                    float u0, u1, u2, u3;
-                    f2_get(sum[0], u0, u1);
-                    f2_get(sum[1], u2, u3);
-                    l_sum += (u0 + u1) + (u2 + u3);
-                    tmem_st_wait();
+                    mref = m_used == -INFINITY ? 0.0f : m_used;
                 }
                 if (dirty && t == 0) {  // before either tile's product: the MMA warp takes tile 0 first
                     const uint32_t st = blk % NS;
@@ -400,13 +389,37 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     if (!ok) break;
                     xa_clean_v<BKV>(smem + L::V_OFF + st * L::KV_BYTES, L::CB, threadIdx.x, c0, s.len, pad_lo, pad_hi);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t * 2 + buf]);
+                // P V of the block's first 64 rows starts while the weights of the others are formed
+                const F2 neg = f2(-mref, -mref);
+                F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (live) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int e = 0; e < 64; e += 2) {
+                            const F2 a = f2_fma(f2(__uint_as_float(x[2 * h + (e >> 5)][e & 31]), __uint_as_float(x[2 * h + (e >> 5)][(e & 31) + 1])), scale2, neg);
+                            float a0, a1;
+                            f2_get(a, a0, a1);
+                            const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
+                            sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
+                            pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
+                        }
+                        tmem_st32(s_addr + (uint32_t)(h * 32), pk);
+                        tmem_st_wait();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
+                }
+                float u0, u1, u2, u3;
+                f2_get(sum[0], u0, u1);
+                f2_get(sum[1], u2, u3);
+                l_sum += (u0 + u1) + (u2 + u3);
             }
             if (!ok) break;
             // ---- O / l -> bf16 -> out, or the piece into the workspace ----
-            ok = warp_wait(&pv_done[t * 2 + ((blk - 1) & 1u)], ((blk - 1) >> 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+            ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
             if (!ok) break;
             tc_fence_after();
             const bool row_ok = row < p.R;
@@ -474,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XP_THREADS, 1)
 cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
     using L = CrossPairSmem;
-    constexpr int HD = L::HD, BKV = xa_bkv<HD>();
+    constexpr int HD = L::HD, BKV = XA_BKV;
     constexpr uint32_t ST = L::STAGES, NS = L::NS;
     extern __shared__ uint8_t xp_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xp_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -852,10 +865,10 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
     if (c0 >= n) return;
     const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
     auto len_of = [&](int obs) { return xa_len(p, obs); };
-    RaggedCursor cur(len_of, p.n_obs, p.n_kv * p.n_mt, p.bkv);
+    RaggedCursor cur(len_of, p.n_obs, p.n_kv * p.n_mt, XA_BKV);
     RaggedUnit u;
     if (!cur.find(end - 1, u)) return;
-    const int nb = (u.len + p.bkv - 1) / p.bkv, first = end - 1 - u.block;  // of the unit of the CTA's last block
+    const int nb = (u.len + XA_BKV - 1) / XA_BKV, first = end - 1 - u.block;  // of the unit of the CTA's last block
     if (first < begin || first + nb <= end) return;                         // begun before this CTA, or whole
     const int c1 = (int)(((long long)(first + nb) * n - 1) / total);        // the CTA that has the unit's last block
     const int kvh = u.kvh / p.n_mt, row0 = (u.kvh - kvh * p.n_mt) * p.unit_rows, rows = min(p.R - row0, p.unit_rows);
@@ -950,10 +963,10 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
     CUtensorMap qmap, kmap, vmap;
     const uint64_t qdims[3] = {(uint64_t)HD, (uint64_t)p.R, (uint64_t)st->n_obs * st->n_kv}, qstr[2] = {(uint64_t)HD * 2, (uint64_t)p.R * HD * 2};
     const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)p.max_len, pages}, str[2] = {(uint64_t)HD * 2, (uint64_t)st->cap * HD * 2};
-    const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, 64, 1};  // pairs stage half of a block's K rows, and all of its V rows
+    const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, HD == 256 ? 64 : 128, 1};  // a CTA of a pair stages half of a block's K rows
     int rc = make_tensor_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, qdims, qstr, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = make_tensor_map(&kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->k_pages, dims, str, kbox, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, HD == 256 ? box : kbox, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     if constexpr (HD == 256) {
         if ((rc = ensure_dyn_smem(cross_attn_pair_kernel, CrossPairSmem::TOTAL))) return rc;
@@ -991,9 +1004,9 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     const int hd = st->head_dim;
     if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
     const long long R = (long long)(n_q / st->n_kv) * S, items = (long long)st->n_obs * st->n_kv;
-    const long long blocks = items * ((R + 255) / 256) * ((max_len + 63LL) / 64);
+    const long long blocks = items * ((R + 255) / 256) * ((max_len + 127LL) / 128);
     if (R > 0x7fffff00LL || items * st->n_layers > 0x7fffff00LL || blocks > 0x7fffff00LL) {
-        vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 256 x 64 scores");
+        vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 256 x 128 scores");
         return VLAB200_ERR_UNSUPPORTED;
     }
     const int n_sm = vb::sm_count();
@@ -1016,7 +1029,6 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     p.n_mt = plan.n_mt;
     p.unit_rows = plan.unit_rows;
     p.n_work = plan.n_work;
-    p.bkv = hd == 256 ? vb::xa_bkv<256>() : vb::xa_bkv<64>();
     p.out_al32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0 ? 1 : 0;
     p.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)hd));
     p.status = vb::device_status_ptr();
