@@ -6,8 +6,10 @@
 //
 // Heads of 64 and 128, a unit = (observation, kv head, 256 of the g S stacked query rows), one CTA:
 //   loader warp       TMA: the two 128-row Q tiles of a unit, K and V in blocks of 128 rows through rings
-//   MMA warp          O_t += P_t V_j with P_t read from TMEM, in two halves of the block's rows, then S_t = Q_t K_(j+1)^T, for the tiles
-//                     t = 0, 1 in turn, so that the tensor pipe works on one tile while the other is in its softmax
+//   MMA warp          O_t += P_t V_j with P_t read from TMEM, XA_EARLY of the block's rows while the softmax is at the others, then
+//                     S_t = Q_t K_(j+1)^T, for the tiles t = 0, 1 in turn: the tensor pipe works on one tile while the other is in its
+//                     softmax.  (A warp per tile: the tiles fell into step, both at the exponentials and then both at the pipe.)
+//   V cleaner         zeroes hidden rows
 //   2 x 4 warps       one per tile and lane quarter, a row per thread: maximum, 2^(s c - m), row sum, P over S in TMEM
 // TMEM: O_0, O_1 and one S per tile (512 columns at heads of 128).  Both the exponentials (16 per clock and SM) and the products need
 // 1,024 clocks per tile and block at heads of 128; at 64 the exponentials bound it.  Blocks of 64 rows with two S buffers per tile were
@@ -26,8 +28,9 @@
 namespace vb {
 
 constexpr int XA_BKV = 128;      // rows of K / V per block
-constexpr int XA_THREADS = 384;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA, 10 and 11 fill the warpgroup that gives up registers
-constexpr int XA_LOADER = 8, XA_MMA = 9;
+constexpr int XA_THREADS = 384;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA, 10 V cleaner, 11 fills the warpgroup that gives up registers
+constexpr int XA_LOADER = 8, XA_MMA = 9, XA_CLEANER = 10;
+constexpr int XA_EARLY = 96;     // of a block's rows: their P V runs beside the softmax of the others
 // Registers of a thread: 384 x 168 at launch = 64,512; 2 x 128 x 208 + 128 x 88 = 64,512 after the split.
 constexpr int XA_REGS_SOFTMAX = 208, XA_REGS_REST = 88;
 constexpr float XA_RAISE = 8.0f; // the running maximum is raised, and O rescaled, only by blocks that exceed it by more than 2^8
@@ -122,15 +125,44 @@ struct CrossSmem {
     static_assert(S_COL + 2 * BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
 };
 
-// Zeroes the rows of a V block in shared memory that the mask hides: they meet weights of 0, and 0 times what stands there need not be 0.
-// 128 threads; V: [n_cb][ROWS][128 B], the first row being row0 of the page.
-template <int ROWS>
-__device__ __forceinline__ void xa_clean_v(uint8_t *v, int n_cb, int tid, int row0, int len, int pad_lo, int pad_hi) {
-    for (int i = tid; i < n_cb * ROWS * 8; i += 128) {
-        const int row = row0 + ((i >> 3) & (ROWS - 1));
-        if (row >= len || (row >= pad_lo && row < pad_hi)) reinterpret_cast<uint4 *>(v)[i] = make_uint4(0, 0, 0, 0);
+// The hidden range of an observation; (none, none) if it has none.
+__device__ __forceinline__ void xa_pad(const CrossParams &p, int obs, int &lo, int &hi) {
+    lo = p.pad ? p.pad[2 * obs] : 0;
+    hi = p.pad ? p.pad[2 * obs + 1] : 0;
+    if (hi <= lo) lo = hi = 0x7fffffff;
+}
+// Does the mask hide rows of the block that begins at row c0?
+__device__ __forceinline__ bool xa_dirty(int c0, int len, int pad_lo, int pad_hi) {
+    return c0 + XA_BKV > len || (c0 < pad_hi && c0 + XA_BKV > pad_lo);
+}
+
+// Hidden rows of a V block meet weights of 0, and 0 times what stands there need not be 0.  So a dirty block's TMA completes on v_raw, and
+// this warp zeroes those rows in shared memory and then says v_full in its place.
+template <int CB>
+__device__ __forceinline__ void xa_clean_blocks(const CrossParams &p, XaSegment &s, bool &ok, uint32_t &jb, uint8_t *v_smem, int stages, int stage_bytes,
+                                                uint64_t *v_raw, uint64_t *v_full, uint32_t &raw_phase, const WaitCtx &wc) {
+    const int lane = threadIdx.x & 31;
+    int pad_lo, pad_hi;
+    xa_pad(p, s.obs, pad_lo, pad_hi);
+    for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
+        const int c0 = j * XA_BKV;
+        if (!xa_dirty(c0, s.len, pad_lo, pad_hi)) continue;
+        const uint32_t st = jb % (uint32_t)stages;
+        ok = warp_wait(&v_raw[st], raw_phase >> st & 1u, wc, DEV_TIMEOUT_FULL);
+        if (!ok) break;
+        raw_phase ^= 1u << st;  // a stage's raw barrier turns with its dirty blocks only
+        uint4 *v = reinterpret_cast<uint4 *>(v_smem + st * (uint32_t)stage_bytes);
+        for (int r = lane >> 3; r < XA_BKV; r += 4) {  // [CB][XA_BKV rows][128 B]
+            const int row = c0 + r;
+            if (row >= s.len || (row >= pad_lo && row < pad_hi)) {
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) v[(cb * XA_BKV + r) * 8 + (lane & 7)] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
     }
-    fence_proxy_async_smem();
 }
 
 // 32 columns of O of one row, divided and rounded, to 32 bf16 at dst.
@@ -165,8 +197,9 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
     uint64_t *q_full = bars, *q_free = bars + 1, *k_full = bars + 2, *k_free = bars + 6, *v_full = bars + 10, *v_free = bars + 14;
     uint64_t *s_full = bars + 18, *pv_done = bars + 20, *o_free = bars + 22;  // [2 tiles]
-    uint64_t *p_full = bars + 24;                                             // [2 tiles][2 halves of a block's rows]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 28);
+    uint64_t *p_full = bars + 24;                                             // [2 tiles][early rows of a block, the others]
+    uint64_t *v_raw = bars + 28;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 32);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{abort_flag, p.status};
@@ -178,6 +211,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             mbar_init(&k_full[i], 1);
             mbar_init(&k_free[i], 1);
             mbar_init(&v_full[i], 1);
+            mbar_init(&v_raw[i], 1);
             mbar_init(&v_free[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -216,6 +250,8 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         for (; ok && work.next(s); ++si) {
             const int item = s.obs * p.n_kv + s.kvh, row0 = s.mt * 256;
             const int tiles = p.R > row0 + 128 ? 2 : 1;
+            int pad_lo, pad_hi;
+            xa_pad(p, s.obs, pad_lo, pad_hi);
             ok = warp_wait(q_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
             if (!ok) break;
             if (elect_one()) {
@@ -236,12 +272,17 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                 ok = warp_wait(&v_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                 if (!ok) break;
                 if (elect_one()) {
-                    mbar_expect_tx(&v_full[st], L::KV_BYTES);
+                    uint64_t *landed = xa_dirty(j * BKV, s.len, pad_lo, pad_hi) ? &v_raw[st] : &v_full[st];
+                    mbar_expect_tx(landed, L::KV_BYTES);
                     for (int cb = 0; cb < L::CB; ++cb)
-                        tma_load_3d(smem + L::V_OFF + st * L::KV_BYTES + cb * (BKV * 128), &v_map, &v_full[st], cb * 64, j * BKV, p.page0 + item);
+                        tma_load_3d(smem + L::V_OFF + st * L::KV_BYTES + cb * (BKV * 128), &v_map, landed, cb * 64, j * BKV, p.page0 + item);
                 }
             }
         }
+    } else if (warp == XA_CLEANER) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
+        uint32_t jb = 0, raw_phase = 0;
+        while (ok && work.next(s)) xa_clean_blocks<L::CB>(p, s, ok, jb, smem + L::V_OFF, NS, L::KV_BYTES, v_raw, v_full, raw_phase, wc);
     } else if (warp == XA_MMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
         constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
@@ -255,18 +296,6 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     mma_f16(tmem_base + L::S_COL + t * BKV, q + (uint64_t)((kk >> 2) * 1024 + (kk & 3) * 2),
                             k + (uint64_t)((kk >> 2) * (BKV * 8) + (kk & 3) * 2), idesc_s, kk != 0 ? 1u : 0u);
                 tc_commit(&s_full[t]);
-            }
-        };
-        auto issue_pv = [&](int t, uint32_t st, int h, bool first) {  // half h of the block's rows
-            const uint64_t v = v_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
-            const uint32_t pt = tmem_base + L::S_COL + t * BKV;
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < BKV / 32; ++k) {
-                    const int kk = h * (BKV / 32) + k;
-                    mma_f16_tmem_a(tmem_base + t * HD, pt + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), idesc_o, first && kk == 0 ? 0u : 1u);
-                }
-                if (h) tc_commit(&pv_done[t]);
             }
         };
         uint32_t si = 0, jb = 0;
@@ -285,19 +314,31 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             }
             for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
                 const uint32_t st = jb % NS, sn = (jb + 1) % NS;
+                const uint64_t v = v_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
                 const bool more = j + 1 < s.j1;
+                // what comes early is waited for before the softmax is
+                ok = warp_wait(&v_full[st], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                if (ok && more) ok = warp_wait(&k_full[sn], ((jb + 1) / NS) & 1u, wc, DEV_TIMEOUT_FULL);
                 for (int t = 0; ok && t < tiles; ++t) {
-                    ok = warp_wait(&p_full[2 * t], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
-                    if (ok && t == 0) ok = warp_wait(&v_full[st], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-                    if (ok && j == s.j0) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                    if (j == s.j0) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                    if (ok) ok = warp_wait(&p_full[2 * t], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(t, st, 0, j == s.j0);
-                    if (t == 0 && more) ok = warp_wait(&k_full[sn], ((jb + 1) / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-                    if (ok) ok = warp_wait(&p_full[2 * t + 1], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
+                    const uint32_t pt = tmem_base + L::S_COL + t * BKV, o = tmem_base + t * HD;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < XA_EARLY / 16; ++kk)
+                            mma_f16_tmem_a(o, pt + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), idesc_o, j == s.j0 && kk == 0 ? 0u : 1u);
+                    }
+                    ok = warp_wait(&p_full[2 * t + 1], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(t, st, 1, false);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = XA_EARLY / 16; kk < BKV / 16; ++kk)
+                            mma_f16_tmem_a(o, pt + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), idesc_o, 1u);
+                        tc_commit(&pv_done[t]);
+                    }
                     if (more) issue_s(t, sn);
                     ++blk[t];
                 }
@@ -309,33 +350,29 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             }
             for (int t = 0; t < tiles; ++t) ++seg[t];
         }
-    } else if (warp > XA_MMA) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));  // fills the warpgroup
+    } else if (warp > XA_CLEANER) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XA_REGS_SOFTMAX));
         const int t = warp >> 2, qtr = warp & 3;
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
         const uint32_t s_addr = tmem_base + L::S_COL + t * BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
-        uint32_t blk = 0;  // blocks of this tile so far; tile 0 has every block of the CTA
+        uint32_t blk = 0;  // blocks of this tile so far
         while (ok && work.next(s)) {
             const int row0 = s.mt * 256 + t * 128;
             if (t == 1 && row0 >= p.R) continue;
             const int lr = t * 128 + qtr * 32 + lane, row = s.mt * 256 + lr;  // in the unit, in the item
             const bool live = row0 + qtr * 32 < p.R;                          // of the warp
-            int pad_lo = 0, pad_hi = 0;
-            if (p.pad) {
-                pad_lo = p.pad[2 * s.obs];
-                pad_hi = p.pad[2 * s.obs + 1];
-            }
-            if (pad_hi <= pad_lo) pad_lo = pad_hi = 0x7fffffff;
+            int pad_lo, pad_hi;
+            xa_pad(p, s.obs, pad_lo, pad_hi);
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units, row sum
             for (int j = s.j0; j < s.j1; ++j, ++blk) {
                 ok = warp_wait(&s_full[t], blk & 1u, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
                 tc_fence_after();
                 const int c0 = j * BKV;
-                const bool dirty = c0 + BKV > s.len || (c0 < pad_hi && c0 + BKV > pad_lo);
+                const bool dirty = xa_dirty(c0, s.len, pad_lo, pad_hi);
                 uint32_t x[4][32];
                 float mref = 0.0f;
                 if (live) {
@@ -360,14 +397,15 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                         for (int e = 2; e < 32; e += 2) mx[i] = xa_max3(mx[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
                     }
                     const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                    float factor = 1.0f;
                     const bool raise = bm > m_used + XA_RAISE;
-                    if (raise) {
-                        factor = m_used == -INFINITY ? 0.0f : xa_ex2(m_used - bm);
-                        m_used = bm;
-                        l_sum *= factor;
-                    }
-                    if (j > s.j0 && __any_sync(0xffffffffu, raise)) {  // O was summed under the old maximum
+                    if (__any_sync(0xffffffffu, raise)) {
+                        float factor = 1.0f;
+                        if (raise) {
+                            factor = m_used == -INFINITY ? 0.0f : xa_ex2(m_used - bm);
+                            m_used = bm;
+                            l_sum *= factor;
+                        }
+                        if (j > s.j0) {  // O was summed under the old maximum
                         ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
                         if (!ok) break;
                         tc_fence_after();
@@ -380,37 +418,42 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                             for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
                             tmem_st16(o_addr + (uint32_t)c, ov);
                         }
+                        }
                     }
                     mref = m_used == -INFINITY ? 0.0f : m_used;
                 }
-                if (dirty && t == 0) {  // before either tile's product: the MMA warp takes tile 0 first
-                    const uint32_t st = blk % NS;
-                    ok = warp_wait(&v_full[st], (blk / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-                    if (!ok) break;
-                    xa_clean_v<BKV>(smem + L::V_OFF + st * L::KV_BYTES, L::CB, threadIdx.x, c0, s.len, pad_lo, pad_hi);
-                }
-                // P V of the block's first 64 rows starts while the weights of the others are formed
                 const F2 neg = f2(-mref, -mref);
                 F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+                // quarter q's exponentials are asked for before quarter q - 1's are summed and packed
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (live) {
-                        uint32_t pk[32];
+                for (int q = 0; q <= BKV / 32; ++q) {
+                    if (live && q < BKV / 32) {
 #pragma unroll
-                        for (int e = 0; e < 64; e += 2) {
-                            const F2 a = f2_fma(f2(__uint_as_float(x[2 * h + (e >> 5)][e & 31]), __uint_as_float(x[2 * h + (e >> 5)][(e & 31) + 1])), scale2, neg);
+                        for (int e = 0; e < 32; e += 2) {
+                            const F2 a = f2_fma(f2(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), scale2, neg);
                             float a0, a1;
                             f2_get(a, a0, a1);
-                            const F2 pr = f2(xa_ex2(a0), xa_ex2(a1));
+                            x[q][e] = __float_as_uint(xa_ex2(a0));
+                            x[q][e + 1] = __float_as_uint(xa_ex2(a1));
+                        }
+                    }
+                    if (q == 0) continue;
+                    if (live) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const F2 pr = f2(__uint_as_float(x[q - 1][e]), __uint_as_float(x[q - 1][e + 1]));
                             sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], pr);
                             pk[e >> 1] = f2_bf16(pr);  // weights are rounded to 8 bits for the product, their sum is not
                         }
-                        tmem_st32(s_addr + (uint32_t)(h * 32), pk);
-                        tmem_st_wait();
+                        tmem_st16(s_addr + (uint32_t)((q - 1) * 16), pk);
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
+                    if (q == XA_EARLY / 32 || q == BKV / 32) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[2 * t + (q == BKV / 32 ? 1 : 0)]);
+                    }
                 }
                 float u0, u1, u2, u3;
                 f2_get(sum[0], u0, u1);
@@ -471,7 +514,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
 // follows the second by a counter: the pipe keeps their order); the odd CTA tells the even one what has landed.
 //   8 softmax warps   lane quarter = warp & 3, column half = warp >> 2: the two warps of a row exchange maxima and sums through shared memory
 // A unit's O is drained after the next unit's first block, so the pipe does not wait for it.
-constexpr int XP_THREADS = 352, XP_LOADER = 8, XP_S = 9, XP_PV = 10;
+constexpr int XP_THREADS = 384, XP_LOADER = 8, XP_S = 9, XP_PV = 10, XP_CLEANER = 11;
 
 struct CrossPairSmem {
     static constexpr int HD = 256, CB = 4, CBH = 2;  // 64-element column blocks of the head, and of the half of V that a CTA stages
@@ -496,7 +539,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     uint64_t *k_full = bars + 4, *k_free = bars + 6, *v_full = bars + 8, *v_free = bars + 10;  // [ST]
     uint64_t *s_full = bars + 12, *p_full = bars + 14, *pv_done = bars + 16;                   // [NS]
     uint64_t *meet = bars + 18;                                                                // [4] the two warps of a lane quarter
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
+    uint64_t *v_raw = bars + 22;                                                               // [ST]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile uint32_t *pv_issued = reinterpret_cast<volatile uint32_t *>(tmem_slot + 2);  // P V blocks issued so far (even CTA)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -514,6 +558,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             mbar_init(&k_free[i], 1);
             mbar_init(&v_full[i], both);
             mbar_init(&v_free[i], 1);
+            mbar_init(&v_raw[i], 1);
         }
         for (uint32_t i = 0; i < NS; ++i) {
             mbar_init(&s_full[i], 1);
@@ -553,6 +598,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     if (warp == XP_LOADER) {
         for (; ok && work.next(s); ++si) {
             const int item = s.obs * p.n_kv + s.kvh;
+            int pad_lo, pad_hi;
+            xa_pad(p, s.obs, pad_lo, pad_hi);
             ok = warp_wait(q_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
             if (!ok) break;
             if (elect_one()) {
@@ -573,13 +620,17 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 ok = warp_wait(&v_free[st], ph ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                 if (!ok) break;
                 if (elect_one()) {
-                    mbar_expect_tx(&v_full[st], L::V_BYTES);
+                    uint64_t *landed = xa_dirty(j * BKV, s.len, pad_lo, pad_hi) ? &v_raw[st] : &v_full[st];
+                    mbar_expect_tx(landed, L::V_BYTES);
                     for (int cb = 0; cb < L::CBH; ++cb)
-                        tma_load_3d(smem + L::V_OFF + st * L::V_BYTES + cb * 16384, &v_map, &v_full[st], ((int)rank * L::CBH + cb) * 64,
+                        tma_load_3d(smem + L::V_OFF + st * L::V_BYTES + cb * 16384, &v_map, landed, ((int)rank * L::CBH + cb) * 64,
                                     j * BKV, p.page0 + item);
                 }
             }
         }
+    } else if (warp == XP_CLEANER) {  // of this CTA's half of V's columns
+        uint32_t raw_phase = 0;
+        while (ok && work.next(s)) xa_clean_blocks<L::CBH>(p, s, ok, jb, smem + L::V_OFF, ST, L::V_BYTES, v_raw, v_full, raw_phase, wc);
     } else if (warp == XP_S) {
         if (rank == 0) {
             constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 256, BKV);
@@ -727,12 +778,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         XaSegment prev;
         float prev_m = 0.0f, prev_l = 0.0f;
         for (; ok && work.next(s); ++si) {
-            int pad_lo = 0, pad_hi = 0;
-            if (p.pad) {
-                pad_lo = p.pad[2 * s.obs];
-                pad_hi = p.pad[2 * s.obs + 1];
-            }
-            if (pad_hi <= pad_lo) pad_lo = pad_hi = 0x7fffffff;
+            int pad_lo, pad_hi;
+            xa_pad(p, s.obs, pad_lo, pad_hi);
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units (the same in both halves), this half's part of the row sum
             for (int j = s.j0; j < s.j1; ++j, ++jb) {
                 const uint32_t sb = jb % NS;
@@ -745,7 +792,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 tmem_ld32(s_addr + (uint32_t)(half * 64 + 32), x[1]);
                 tmem_ld_wait();
                 const int b0 = j * BKV, c0 = b0 + half * 64;
-                const bool dirty = b0 + BKV > s.len || (b0 < pad_hi && b0 + BKV > pad_lo);
+                const bool dirty = xa_dirty(b0, s.len, pad_lo, pad_hi);
                 if (dirty) {
                     const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
 #pragma unroll
@@ -811,12 +858,6 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 // P (128 rows of V, bf16) over the first 64 columns of S; both halves have read theirs: they met
                 tmem_st32(s_addr + (uint32_t)(half * 32), pk);
                 tmem_st_wait();
-                if (dirty && half == 0) {  // this CTA's half of V's columns
-                    const uint32_t st = jb % ST;
-                    ok = warp_wait(&v_full[st], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
-                    if (!ok) break;
-                    xa_clean_v<128>(smem + L::V_OFF + st * L::V_BYTES, L::CBH, threadIdx.x, b0, s.len, pad_lo, pad_hi);
-                }
                 tc_fence_before();
                 arrive_even(&p_full[sb]);
                 if (j == s.j0 && si > 0) {
