@@ -31,8 +31,9 @@ def test_argument_checks_need_no_gpu():
         assert call(**bad) == -1, bad
     assert call(hd=80) == -4
     st = api._KvStoreC(16, 16, 1, 2, 2, 64, 8, 0)
-    assert api.lib().vlab200_cross_attention_ws_bytes(C.byref(st), 1, 3) == -1
-    assert api.lib().vlab200_cross_attention_ws_bytes(C.byref(st), 0, 2) == -1
+    assert api.lib().vlab200_cross_attention_ws_bytes(C.byref(st), 1, 3, 8) == -1
+    assert api.lib().vlab200_cross_attention_ws_bytes(C.byref(st), 0, 2, 8) == -1
+    assert api.lib().vlab200_cross_attention_ws_bytes(C.byref(st), 1, 2, 9) == -1
 
 
 CASES = [

@@ -281,11 +281,13 @@ def _call_on(dev, fn, what, *args):
     """fn(*args, stream) with cuda device `dev` (an index) current, on its current stream."""
     import torch
 
+    # the raw handle: making a Stream object of it took 3 us of a call's 16
+    stream = C.c_void_p(torch._C._cuda_getCurrentRawStream(dev))
     if torch.cuda.current_device() == dev:
-        rc = fn(*args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            rc = fn(*args, stream)
     if rc != OK:
         raise VlaB200Error(rc, what)
 
@@ -394,13 +396,14 @@ def cross_attention(store, layer, q, lens=None, max_len=None, pad_ranges=None, s
     ws, n = None, 0
     if split:
         if torch.cuda.current_device() == dev:
-            n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q)
+            n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q, max_len)
         else:
             with torch.cuda.device(dev):
-                n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q)
+                n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q, max_len)
         if n < 0:
-            raise VlaB200Error(ERR_ARG, f"cross_attention: {n_q} query heads on {store.n_kv} kv heads, {S} tokens")
-        ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
+            raise VlaB200Error(ERR_ARG, f"cross_attention: {n_q} query heads on {store.n_kv} kv heads, {S} tokens, {max_len} rows")
+        if n > 0:
+            ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
     _call_on(dev, lib().vlab200_cross_attention, "vlab200_cross_attention", C.byref(store.c), layer, C.c_void_p(q.data_ptr()),
              C.c_void_p(out.data_ptr()), C.c_void_p(lse.data_ptr()), S, n_q, C.c_void_p(lens.data_ptr()) if lens is not None else None, max_len,
              C.c_void_p(pad_ranges.data_ptr()) if pad_ranges is not None else None, C.c_float(0.0 if scale is None else scale),

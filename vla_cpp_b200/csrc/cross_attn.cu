@@ -118,12 +118,25 @@ struct CrossSmem {
     static constexpr int CB = HD / 64, BKV = XA_BKV;  // 64-element column blocks
     static constexpr int Q_BYTES = CB * 128 * 128;          // a tile: [CB][128 rows][128 B]
     static constexpr int KV_BYTES = CB * BKV * 128;
-    static constexpr int STAGES = HD == 64 ? 4 : 2;
-    static constexpr int K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES, BAR_OFF = V_OFF + STAGES * KV_BYTES;
+    static constexpr int STAGES = HD == 64 ? 4 : 2, QS = HD == 64 ? 2 : 1;  // K and V blocks; units' Q tiles
+    static constexpr int K_OFF = QS * 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES, BAR_OFF = V_OFF + STAGES * KV_BYTES;
     static constexpr int TOTAL = BAR_OFF + 512 + 1024;
     static constexpr int S_COL = 2 * HD;  // O_0, O_1, S_0, S_1
     static_assert(S_COL + 2 * BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
 };
+
+// Rows of empty observations: 0 and -inf.  CTA (pair) c looks after every n_work-th observation.
+template <int HD>
+__device__ __forceinline__ void xa_fill_empty(const CrossParams &p, int c, int tid, int n_threads) {
+    for (int obs = c; obs < p.n_obs; obs += p.n_work) {
+        if (xa_len(p, obs) > 0) continue;
+        const long long n = (long long)p.n_q * p.S;
+        uint4 *out = reinterpret_cast<uint4 *>(p.out + obs * n * HD);
+        for (long long i = tid; i < n * (HD / 8); i += n_threads) out[i] = make_uint4(0, 0, 0, 0);
+        if (p.lse)
+            for (long long i = tid; i < n; i += n_threads) p.lse[obs * n + i] = -INFINITY;
+    }
+}
 
 // The hidden range of an observation; (none, none) if it has none.
 __device__ __forceinline__ void xa_pad(const CrossParams &p, int obs, int &lo, int &hi) {
@@ -191,22 +204,24 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                   const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
     using L = CrossSmem<HD>;
     constexpr int BKV = L::BKV;
-    constexpr uint32_t NS = L::STAGES;
+    constexpr uint32_t NS = L::STAGES, QS = L::QS;
     extern __shared__ uint8_t xa_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xa_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
-    uint64_t *q_full = bars, *q_free = bars + 1, *k_full = bars + 2, *k_free = bars + 6, *v_full = bars + 10, *v_free = bars + 14;
+    uint64_t *k_full = bars + 2, *k_free = bars + 6, *v_full = bars + 10, *v_free = bars + 14;
     uint64_t *s_full = bars + 18, *pv_done = bars + 20, *o_free = bars + 22;  // [2 tiles]
     uint64_t *p_full = bars + 24;                                             // [2 tiles][early rows of a block, the others]
-    uint64_t *v_raw = bars + 28;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 32);
+    uint64_t *v_raw = bars + 28, *q_full = bars + 32, *q_free = bars + 34;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 36);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{abort_flag, p.status};
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
-        mbar_init(q_free, 1);
+        for (uint32_t i = 0; i < QS; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_free[i], 1);
+        }
         for (uint32_t i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_free[i], 1);
@@ -240,6 +255,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     pdl_wait();
 
     auto len_of = [&](int obs) { return xa_len(p, obs); };
+    if (warp < XA_LOADER) xa_fill_empty<HD>(p, blockIdx.x, threadIdx.x, 32 * XA_LOADER);
     XaWork work(len_of, p, blockIdx.x);
     XaSegment s;
     bool ok = true;
@@ -252,13 +268,14 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             const int tiles = p.R > row0 + 128 ? 2 : 1;
             int pad_lo, pad_hi;
             xa_pad(p, s.obs, pad_lo, pad_hi);
-            ok = warp_wait(q_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+            const uint32_t qs = si % QS;
+            ok = warp_wait(&q_free[qs], (si / QS & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
             if (!ok) break;
             if (elect_one()) {
-                mbar_expect_tx(q_full, tiles * L::Q_BYTES);
+                mbar_expect_tx(&q_full[qs], tiles * L::Q_BYTES);
                 for (int t = 0; t < tiles; ++t)
                     for (int cb = 0; cb < L::CB; ++cb)
-                        tma_load_3d(smem + t * L::Q_BYTES + cb * 16384, &q_map, q_full, cb * 64, row0 + t * 128, item);
+                        tma_load_3d(smem + (qs * 2 + t) * L::Q_BYTES + cb * 16384, &q_map, &q_full[qs], cb * 64, row0 + t * 128, item);
             }
             for (int j = s.j0; j < s.j1; ++j, ++jb) {
                 const uint32_t st = jb % NS, ph = (jb / NS) & 1u;
@@ -288,8 +305,8 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
         const uint64_t q_desc0 = smem_desc_sw128(smem_u32(smem), 16, 1024), k_desc0 = smem_desc_sw128(smem_u32(smem) + L::K_OFF, 16, 1024);
         const uint64_t v_desc0 = smem_desc_sw128(smem_u32(smem) + L::V_OFF, BKV * 128, 1024);
-        auto issue_s = [&](int t, uint32_t st) {
-            const uint64_t q = q_desc0 + (uint64_t)(t * (L::Q_BYTES >> 4)), k = k_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
+        auto issue_s = [&](uint32_t qs, int t, uint32_t st) {
+            const uint64_t q = q_desc0 + (uint64_t)((qs * 2 + t) * (L::Q_BYTES >> 4)), k = k_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
             if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
@@ -302,15 +319,16 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         uint32_t blk[2] = {0, 0}, seg[2] = {0, 0};  // blocks and segments of each tile so far
         for (; ok && work.next(s); ++si) {
             const int tiles = p.R > s.mt * 256 + 128 ? 2 : 1;
-            ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
+            const uint32_t qs = si % QS;
+            ok = warp_wait(&q_full[qs], si / QS & 1u, wc, DEV_TIMEOUT_FULL);
             if (ok) ok = warp_wait(&k_full[jb % NS], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
             // a tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order
-            for (int t = 0; t < tiles; ++t) issue_s(t, jb % NS);
+            for (int t = 0; t < tiles; ++t) issue_s(qs, t, jb % NS);
             if (elect_one()) {
                 tc_commit(&k_free[jb % NS]);
-                if (s.j1 - s.j0 == 1) tc_commit(q_free);
+                if (s.j1 - s.j0 == 1) tc_commit(&q_free[qs]);
             }
             for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
                 const uint32_t st = jb % NS, sn = (jb + 1) % NS;
@@ -339,13 +357,13 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                             mma_f16_tmem_a(o, pt + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), idesc_o, 1u);
                         tc_commit(&pv_done[t]);
                     }
-                    if (more) issue_s(t, sn);
+                    if (more) issue_s(qs, t, sn);
                     ++blk[t];
                 }
                 if (ok && elect_one()) {
                     tc_commit(&v_free[st]);
                     if (more) tc_commit(&k_free[sn]);
-                    if (j + 2 == s.j1) tc_commit(q_free);  // the segment's last S blocks have been issued
+                    if (j + 2 == s.j1) tc_commit(&q_free[qs]);  // the segment's last S blocks have been issued
                 }
             }
             for (int t = 0; t < tiles; ++t) ++seg[t];
@@ -590,6 +608,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     pdl_wait();
 
     auto len_of = [&](int obs) { return xa_len(p, obs); };
+    if (warp < XP_LOADER) xa_fill_empty<HD>(p, blockIdx.x >> 1, rank * 32 * XP_LOADER + threadIdx.x, 64 * XP_LOADER);
     XaWork work(len_of, p, blockIdx.x >> 1);
     XaSegment s;
     bool ok = true;
@@ -881,9 +900,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     }
 }
 
-// Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Rows of empty
-// observations: 0 and -inf.  Block x < n_work looks after the unit that CTA x began and did not finish, the others after one observation
-// each, if it is empty.  TEAM warps share a row: 1 where a unit's rows are many (two pieces or three of each), 8 where they are few and the
+// Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Block x
+// looks after the unit that CTA x began and did not finish.  TEAM warps share a row: 1 where a unit's rows are many (two pieces or three of each), 8 where they are few and the
 // pieces as many as there are CTAs (one token over 16,001 rows, a warp per row: 40 us).
 template <int HD, int TEAM>
 __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p) {
@@ -891,17 +909,6 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if ((int)blockIdx.x >= p.n_work) {
-        const int obs = blockIdx.x - p.n_work;
-        if (xa_len(p, obs) > 0) return;
-        const long long n = (long long)p.n_q * p.S;  // rows of the observation
-        uint4 *out = reinterpret_cast<uint4 *>(p.out + obs * n * HD);
-        for (long long i = (long long)blockIdx.y * 256 + threadIdx.x; i < n * (HD / 8); i += 256LL * gridDim.y) out[i] = make_uint4(0, 0, 0, 0);
-        if (p.lse)
-            for (long long i = (long long)blockIdx.y * 256 + threadIdx.x; i < n; i += 256LL * gridDim.y) p.lse[obs * n + i] = -INFINITY;
-        return;
-    }
-    if (p.ws_o == nullptr) return;
     const int c0 = blockIdx.x, total = xa_total_blocks(p), n = min(p.n_work, total);
     if (c0 >= n) return;
     const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
@@ -977,7 +984,7 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
 
 template <int HD>
 static int launch_combine(const CrossParams &p, cudaStream_t stream) {
-    const unsigned gx = (unsigned)(p.n_work + p.n_obs);
+    const unsigned gx = (unsigned)p.n_work;
     if (p.ws_rows <= 64)  // a row per block
         return launch_pdl(cross_combine_kernel<HD, 8>, dim3(gx, (unsigned)p.ws_rows), dim3(256), 0, stream, p);
     return launch_pdl(cross_combine_kernel<HD, 1>, dim3(gx, 8), dim3(256), 0, stream, p);  // 32 rows per block
@@ -986,15 +993,20 @@ static int launch_combine(const CrossParams &p, cudaStream_t stream) {
 // Units, workers and workspace of a call; the same for the size query and the launch.
 struct CrossPlan {
     int unit_rows, n_mt, n_work, ws_rows;
-    long long ws_bytes;
+    long long ws_bytes;  // 0: no unit is cut
 };
-static CrossPlan cross_plan(int hd, int R, int n_sm) {
+static CrossPlan cross_plan(int hd, long long items, int R, int max_len, int n_sm) {
     CrossPlan c;
     c.unit_rows = 256;
     c.n_mt = (R + 255) / 256;
     c.n_work = hd == 256 ? n_sm / 2 : n_sm;
     c.ws_rows = R < 256 ? R : 256;
-    c.ws_bytes = 2LL * c.n_work * c.ws_rows * (hd + 2) * 4;
+    // Whole units take rounds of n_work; cut ones fill the last round, for the pieces' way through the workspace and a second kernel:
+    // some 10 us, six blocks.  (64 observations, heads of 64, 1 or 2 blocks: 34 us whole, 45 cut; heads of 256, up to 7 blocks: 47 and
+    // 55; 4 observations of 64 blocks: 272 and 233; 1 of 126 blocks: 176 and 27.)
+    const long long units = items * c.n_mt, nb = (max_len + XA_BKV - 1) / XA_BKV, rounds = (units + c.n_work - 1) / c.n_work;
+    const bool cut = (rounds * c.n_work - units) * nb > 6LL * c.n_work;
+    c.ws_bytes = cut ? 2LL * c.n_work * c.ws_rows * (hd + 2) * 4 : 0;
     return c;
 }
 
@@ -1003,7 +1015,7 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
     const uint64_t pages = (uint64_t)st->n_layers * st->n_obs * st->n_kv;
     CUtensorMap qmap, kmap, vmap;
     const uint64_t qdims[3] = {(uint64_t)HD, (uint64_t)p.R, (uint64_t)st->n_obs * st->n_kv}, qstr[2] = {(uint64_t)HD * 2, (uint64_t)p.R * HD * 2};
-    const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)p.max_len, pages}, str[2] = {(uint64_t)HD * 2, (uint64_t)st->cap * HD * 2};
+    const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)(p.max_len > 0 ? p.max_len : 1), pages}, str[2] = {(uint64_t)HD * 2, (uint64_t)st->cap * HD * 2};
     const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, HD == 256 ? 64 : 128, 1};  // a CTA of a pair stages half of a block's K rows
     int rc = make_tensor_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, qdims, qstr, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = make_tensor_map(&kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->k_pages, dims, str, kbox, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -1016,7 +1028,7 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
         if ((rc = ensure_dyn_smem(cross_attn_kernel<HD>, CrossSmem<HD>::TOTAL))) return rc;
         rc = launch_pdl(cross_attn_kernel<HD>, dim3((unsigned)plan.n_work), dim3(XA_THREADS), CrossSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
     }
-    if (rc) return rc;
+    if (rc || !p.ws_o) return rc;
     return launch_combine<HD>(p, stream);
 }
 
@@ -1028,10 +1040,10 @@ static bool cross_shape_ok(const vlab200_kv_store *st, int S, int n_q) {
 
 extern "C" {
 
-int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q) {
-    if (!vb::cross_shape_ok(st, S, n_q) || (long long)(n_q / st->n_kv) * S > 0x7fffff00LL) return -1;
+int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q, int32_t max_len) {
+    if (!vb::cross_shape_ok(st, S, n_q) || max_len < 0 || max_len > st->cap || (long long)(n_q / st->n_kv) * S > 0x7fffff00LL) return -1;
     const int n_sm = vb::sm_count();
-    return n_sm ? vb::cross_plan(st->head_dim, (n_q / st->n_kv) * S, n_sm).ws_bytes : -1;
+    return n_sm ? vb::cross_plan(st->head_dim, (long long)st->n_obs * st->n_kv, (n_q / st->n_kv) * S, max_len, n_sm).ws_bytes : -1;
 }
 
 int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const void *q, void *out, float *lse, int32_t S, int32_t n_q,
@@ -1052,7 +1064,7 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     }
     const int n_sm = vb::sm_count();
     if (!n_sm) return vb::cuda_fail(cudaGetLastError(), "sm_count");
-    const vb::CrossPlan plan = vb::cross_plan(hd, (int)R, n_sm);
+    const vb::CrossPlan plan = vb::cross_plan(hd, items, (int)R, max_len, n_sm);
     if (ws && ws_bytes < plan.ws_bytes) return VLAB200_ERR_ARG;
     vb::CrossParams p;
     p.out = static_cast<__nv_bfloat16 *>(out);
@@ -1075,14 +1087,9 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     p.status = vb::device_status_ptr();
     if (!p.status) return vb::cuda_fail(cudaGetLastError(), "device_status_ptr");
     p.ws_rows = plan.ws_rows;
-    p.ws_o = static_cast<float *>(ws);
-    p.ws_ml = ws ? p.ws_o + 2LL * plan.n_work * plan.ws_rows * hd : nullptr;
+    p.ws_o = plan.ws_bytes ? static_cast<float *>(ws) : nullptr;
+    p.ws_ml = p.ws_o ? p.ws_o + 2LL * plan.n_work * plan.ws_rows * hd : nullptr;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (max_len == 0) {  // nothing to map: every row is that of an empty observation
-        p.lens = nullptr;
-        p.n_work = 0;
-        return hd == 64 ? vb::launch_combine<64>(p, cs) : hd == 128 ? vb::launch_combine<128>(p, cs) : vb::launch_combine<256>(p, cs);
-    }
     if (hd == 64) return vb::launch_cross<64>(st, q, p, plan, cs);
     if (hd == 128) return vb::launch_cross<128>(st, q, p, plan, cs);
     return vb::launch_cross<256>(st, q, p, plan, cs);
