@@ -30,7 +30,7 @@ struct RopeNormParams {
     const int32_t *pos, *row0, *n_tok;
     __nv_bfloat16 *q_out, *k, *v;  // k, v: pages of the layer
     unsigned M;                    // n_obs * S rows
-    int S, n_q, n_kv, n_heads, cap, prefix_len, rot, parts;  // n_heads: heads of a row; parts: warps that share a token
+    int S, n_q, n_kv, n_heads, nsq, nsk, cap, prefix_len, rot, parts;  // n_heads: heads of a row; parts: warps that share a token
     float eps, mscale;
 };
 
@@ -42,8 +42,7 @@ struct RnChunk;
 template <>
 struct RnChunk<false> {
     uint4 r;
-    __device__ __forceinline__ void load(const void *x, long long i) { r = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(x) + i); }
-    __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const uint8_t *s) { r = *reinterpret_cast<const uint4 *>(s); }
     __device__ __forceinline__ void get(F2 (&f)[4]) {
         f[0] = f2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u));
         f[1] = f2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u));
@@ -55,12 +54,10 @@ struct RnChunk<false> {
 template <>
 struct RnChunk<true> {
     float4 a, b;
-    __device__ __forceinline__ void load(const void *x, long long i) {
-        const float4 *s = reinterpret_cast<const float4 *>(static_cast<const float *>(x) + i);
-        a = s[0];
-        b = s[1];
+    __device__ __forceinline__ void load(const uint8_t *s) {
+        a = reinterpret_cast<const float4 *>(s)[0];
+        b = reinterpret_cast<const float4 *>(s)[1];
     }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
     __device__ __forceinline__ void get(F2 (&f)[4]) {
         f[0] = f2(a.x, a.y);
         f[1] = f2(a.z, a.w);
@@ -74,18 +71,15 @@ struct RnChunk<true> {
     }
 };
 
-// What a warp needs to know of a token before it works on it; fetched while it works on the one before.
+// A token of a warp, and what the warp has to know of it before it works on it (fetched while it works on the one before).
 struct RnToken {
     long long row, pos;
     unsigned m;
     int obs, t;
     bool exists, live;
 };
-__device__ __forceinline__ void rn_fetch_token(RnToken &k, const RopeNormParams &p) {
-    k.exists = k.m < p.M;
-    k.live = k.exists && (p.n_tok == nullptr || k.t < p.n_tok[k.obs]);
-    k.row = (k.live && p.row0 ? (long long)p.row0[k.obs] : (long long)p.prefix_len) + k.t;
-    k.pos = k.live && p.pos ? (long long)p.pos[k.m] : k.row;
+__device__ __forceinline__ bool rn_live(const RnToken &k, const RopeNormParams &p) {
+    return k.exists && (p.n_tok == nullptr || k.t < p.n_tok[k.obs]);
 }
 __device__ __forceinline__ void lds_f2x4(F2 (&f)[4], const float *s) {  // 8 floats, 16-byte aligned
     const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(s), b = *reinterpret_cast<const ulonglong2 *>(s + 4);
@@ -94,18 +88,39 @@ __device__ __forceinline__ void lds_f2x4(F2 (&f)[4], const float *s) {  // 8 flo
     f[2].v = b.x;
     f[3].v = b.y;
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <int HD, bool F32>
+struct RnSmem {
+    static constexpr int STAGE = 512 * (F32 ? 4 : 2);  // a step: 512 columns of 32 / (HD / 16) heads
+    static constexpr int DEPTH = 4;                    // steps in flight per warp
+    static constexpr int TRIG = RN_WARPS * DEPTH * STAGE, WEIGHT = TRIG + RN_WARPS * HD * 4, TURN = WEIGHT + 2 * HD * 4;
+    static constexpr int STEPS = TURN + HD / 2 * 8;    // RnStep [steps of a token][heads of a step]
+};
+// Where the columns of a head come from and go to, but for the token: the same for all tokens, worked out once per block.
+struct __align__(16) RnStep {
+    __nv_bfloat16 *dst;  // of the q rows or the page at token / row 0 of observation 0
+    int src;             // byte offset in a row of x; negative: no such head
+    int pad;
+};
 
 template <int HD, int MODE, bool F32>
 __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const RopeNormParams p) {
-    constexpr int LH = HD / 16;        // lanes per head: two chunks of 8 columns each
-    constexpr int HPW = 32 / LH;       // heads per warp and step
-    constexpr int DEPTH = F32 ? 1 : 2; // steps whose loads are in flight beside the one being worked on
-    __shared__ __align__(16) float s_cos[RN_WARPS][HD / 2], s_sin[RN_WARPS][HD / 2], s_w[2][HD];
-    __shared__ long long s_turn[HD / 2];  // turns per position in units of 2^-64
-    __shared__ float s_y[MODE == ROPE_HALF_ANY ? RN_WARPS : 1][MODE == ROPE_HALF_ANY ? 512 : 1];
+    using L = RnSmem<HD, F32>;
+    constexpr int LH = HD / 16;   // lanes per head: two chunks of 8 columns each
+    constexpr int HPW = 32 / LH;  // heads per warp and step
+    constexpr int ES = F32 ? 4 : 2;
+    constexpr unsigned DEPTH = L::DEPTH;
+    extern __shared__ __align__(16) uint8_t rn_smem[];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    uint8_t *const ring = rn_smem + warp * (int)DEPTH * L::STAGE;
+    float *const s_cos = reinterpret_cast<float *>(rn_smem + L::TRIG) + warp * HD, *const s_sin = s_cos + HD / 2;
+    float *const s_w = reinterpret_cast<float *>(rn_smem + L::WEIGHT);                  // [2][HD]
+    long long *const s_turn = reinterpret_cast<long long *>(rn_smem + L::TURN);         // turns per position in units of 2^-64
     const int half = p.rot >> 1;
     // This lane's two chunks start at columns cu and cv.  Half layout with rot % 16 == 0: the two columns of every pair are in one lane
     // (columns from rot on: two chunks side by side); otherwise 16 columns side by side.
@@ -114,67 +129,115 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
     const int cu = across ? jl * 8 : jl * 16, cv = across ? half + jl * 8 : jl * 16 + 8;
     const bool turned = MODE == ROPE_HALF_LANES ? across : cu < p.rot;
     // a token's steps: those of its q heads, then of its k heads, then of its v heads, HPW heads each; this warp takes every parts-th
-    const int nsq = (p.n_q + HPW - 1) / HPW, nsk = p.n_heads > p.n_q ? (p.n_kv + HPW - 1) / HPW : 0, n_steps = nsq + 2 * nsk;
-    const unsigned n_warps = gridDim.x * RN_WARPS, task = blockIdx.x * RN_WARPS + warp;
-    const int part = (int)(task % (unsigned)p.parts);
-    const int my_steps = (n_steps - part + p.parts - 1) / p.parts;
-    const int my_slots = (my_steps + DEPTH - 1) / DEPTH * DEPTH;  // a token starts at slot 0 of the ring
-    RnToken tok, nxt;
-    tok.m = task / (unsigned)p.parts;
-    tok.obs = (int)(tok.m / (unsigned)p.S);
-    tok.t = (int)(tok.m - (unsigned)tok.obs * (unsigned)p.S);
-    rn_fetch_token(tok, p);
-    // a warp has more than one token only where parts == 1
-    const int d_obs = (int)(n_warps / (unsigned)p.S), d_t = (int)(n_warps - (unsigned)d_obs * (unsigned)p.S);
-    RnChunk<F32> ru[DEPTH], rv[DEPTH];
-    auto fetch = [&](int d, const RnToken &k, int i) {  // this lane's columns in the warp's i-th step of a token
-        const int s = part + i * p.parts;
-        const int h = (s < nsq ? s : s < nsq + nsk ? s - nsq : s - nsq - nsk) * HPW + lh;  // among its kind
-        if (k.live && s < n_steps && h < (s < nsq ? p.n_q : p.n_kv)) {
-            const long long at = (long long)k.m * p.x_stride + (h + (s < nsq ? 0 : s < nsq + nsk ? p.n_q : p.n_q + p.n_kv)) * HD;
-            ru[d].load(p.x, at + cu);
-            rv[d].load(p.x, at + cv);
-        }
-    };
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-        ru[d].zero();
-        rv[d].zero();
-        fetch(d, tok, d);
+    const int nsq = p.nsq, nsqk = p.nsq + p.nsk, n_steps = p.nsq + 2 * p.nsk;
+    const int q_head = p.S * HD, kv_head = p.cap * HD;
+    RnStep *const steps = reinterpret_cast<RnStep *>(rn_smem + L::STEPS);
+    for (int i = threadIdx.x; i < n_steps * HPW; i += RN_WARPS * 32) {
+        const int s = i / HPW, kind = s < nsq ? 0 : s < nsqk ? 1 : 2;
+        const int h = (s - (kind == 0 ? 0 : kind == 1 ? nsq : nsqk)) * HPW + i % HPW;  // among its kind
+        RnStep e;
+        e.src = h < (kind == 0 ? p.n_q : p.n_kv) ? (h + (kind == 0 ? 0 : kind == 1 ? p.n_q : p.n_q + p.n_kv)) * HD * ES : -1;
+        e.dst = (kind == 0 ? p.q_out : kind == 1 ? p.k : p.v) + (long long)h * (kind == 0 ? q_head : kv_head);
+        e.pad = 0;
+        steps[i] = e;
     }
     for (int i = threadIdx.x; i < 2 * HD; i += RN_WARPS * 32) {
         const float *w = i < HD ? p.q_norm : p.k_norm;
-        s_w[0][i] = w ? w[i < HD ? i : i - HD] : 1.0f;
+        s_w[i] = w ? w[i < HD ? i : i - HD] : 1.0f;
     }
     if (threadIdx.x < half) {
         const double turns = p.freqs[threadIdx.x] * 0.15915494309189533577;
         s_turn[threadIdx.x] = __double2ll_rn((turns - rint(turns)) * 18446744073709551616.0);
     }
-    __syncthreads();
-    const int q_head = p.S * HD, kv_head = p.cap * HD;
-    for (; tok.exists; tok = nxt) {
-        nxt.m = tok.m + n_warps;
-        nxt.obs = tok.obs + d_obs;
-        nxt.t = tok.t + d_t;
-        if (nxt.t >= p.S) {
-            nxt.t -= p.S;
-            ++nxt.obs;
+    // warps are dealt to (token, part): a warp keeps its part from token to token, n_warps is a multiple of parts wherever it has several
+    const unsigned n_tok_warps = gridDim.x * RN_WARPS / (unsigned)p.parts, task = blockIdx.x * RN_WARPS + warp;
+    const int part = (int)(task % (unsigned)p.parts);
+    const int d_obs = (int)(n_tok_warps / (unsigned)p.S), d_t = (int)(n_tok_warps - (unsigned)d_obs * (unsigned)p.S);
+    auto step_on = [&](RnToken &k) {  // to the warp's next token
+        k.m += n_tok_warps;
+        k.obs += d_obs;
+        k.t += d_t;
+        if (k.t >= p.S) {
+            k.t -= p.S;
+            ++k.obs;
         }
-        rn_fetch_token(nxt, p);
-        __nv_bfloat16 *const q_dst = p.q_out + ((long long)tok.obs * p.n_q * p.S + tok.t) * HD;
+        k.exists = k.m < p.M;
+    };
+    auto fetch = [&](RnToken &k) {
+        k.live = rn_live(k, p);
+        k.row = (k.live && p.row0 ? (long long)p.row0[k.obs] : (long long)p.prefix_len) + k.t;
+        k.pos = k.live && p.pos ? (long long)p.pos[k.m] : k.row;
+    };
+    RnToken tok;
+    tok.m = task / (unsigned)p.parts;
+    tok.obs = (int)(tok.m / (unsigned)p.S);
+    tok.t = (int)(tok.m - (unsigned)tok.obs * (unsigned)p.S);
+    tok.exists = tok.m < p.M;
+    fetch(tok);
+    // The loads run DEPTH steps ahead through all of the warp's live tokens, each lane's own 2 x 8 columns straight to shared memory:
+    // in registers they left room for two steps (32 KB per SM in flight, a copy alone 47 us for 224 MB).
+    RnToken ld = tok;
+    const int my_steps = (n_steps - part + p.parts - 1) / p.parts;
+    const RnStep *const my_step0 = steps + part * HPW + lh;
+    const int step_stride = p.parts * HPW;
+    const long long row_bytes = p.x_stride * ES, row_jump = row_bytes * n_tok_warps;
+    const uint8_t *ld_row = static_cast<const uint8_t *>(p.x) + (long long)tok.m * row_bytes + cu * ES;
+    const RnStep *ld_step = my_step0;
+    int ld_left = my_steps;
+    const int v_off = (cv - cu) * ES;
+    const uint32_t my_ring = smem_u32(ring) + (uint32_t)((lh * HD + cu) * ES);
+    uint32_t issue_at = 0, use_at = 0;  // byte offsets of stages in the ring
+    static_assert(((DEPTH * L::STAGE) & (DEPTH * L::STAGE - 1)) == 0, "a ring's size is a power of two");
+    auto next_live = [&]() {
+        do {
+            step_on(ld);
+            ld_row += row_jump;
+            ld.live = rn_live(ld, p);
+        } while (ld.exists && !ld.live);
+    };
+    if (ld.exists && !ld.live) next_live();
+    __syncthreads();
+    auto issue = [&]() {
+        if (ld.exists) {
+            const int src_off = ld_step->src;
+            if (src_off >= 0) {
+                const uint8_t *src = ld_row + src_off;
+                const uint32_t dst = my_ring + issue_at;
+#pragma unroll
+                for (int i = 0; i < ES / 2; ++i) {
+                    cp_async16(dst + 16 * i, src + 16 * i);
+                    cp_async16(dst + (uint32_t)v_off + 16 * i, src + v_off + 16 * i);
+                }
+            }
+            ld_step += step_stride;
+            if (--ld_left == 0) {
+                ld_left = my_steps;
+                ld_step = my_step0;
+                next_live();
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        issue_at = (issue_at + L::STAGE) & (DEPTH * L::STAGE - 1);
+    };
+#pragma unroll
+    for (unsigned d = 0; d < DEPTH; ++d) issue();
+    RnToken nxt;
+    for (; tok.exists; tok = nxt) {
+        nxt = tok;
+        step_on(nxt);
+        fetch(nxt);
+        const long long q_at = ((long long)tok.obs * p.n_q * p.S + tok.t) * HD;
         if (!tok.live) {  // a padding token: q is zero, its row of the pages stays as it is
             for (int s = part; s < nsq; s += p.parts) {
-                const int h = s * HPW + lh;
-                if (h >= p.n_q) break;
-                *reinterpret_cast<uint4 *>(q_dst + (long long)h * q_head + cu) = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4 *>(q_dst + (long long)h * q_head + cv) = make_uint4(0, 0, 0, 0);
+                const RnStep e = steps[s * HPW + lh];
+                if (e.src < 0) break;
+                *reinterpret_cast<uint4 *>(e.dst + q_at + cu) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(e.dst + q_at + cv) = make_uint4(0, 0, 0, 0);
             }
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) fetch(d, nxt, d);
             continue;
         }
         const bool row_ok = tok.row >= 0 && tok.row < p.cap;
-        const long long kv0 = (long long)tok.obs * p.n_kv * kv_head + tok.row * HD;
+        const long long kv_at = (long long)tok.obs * p.n_kv * kv_head + tok.row * HD;
         __syncwarp();
         for (int i = lane; i < half; i += 32) {
             // The angle in units of 2^-64 turns: whole turns drop out of the product, which would otherwise cost a float32 angle 0.06 of
@@ -182,24 +245,42 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
             // most: 2^-13 of the rounding to bf16 that follows.
             const unsigned long long a = (unsigned long long)tok.pos * (unsigned long long)s_turn[i];
             const float rad = (float)(int)(a >> 32) * 1.4629180792671596e-9f;  // 2 pi 2^-32
-            s_cos[warp][i] = __cosf(rad) * p.mscale;
-            s_sin[warp][i] = __sinf(rad) * p.mscale;
+            s_cos[i] = __cosf(rad) * p.mscale;
+            s_sin[i] = __sinf(rad) * p.mscale;
         }
         __syncwarp();
         // half layout:  out_u = scale (y_u au - y_v bv),  out_v = scale (y_v av + y_u bu): norm weights times cosine (a) and sine (b)
         // interleaved:  the same within a chunk, with the pair's two products side by side
         F2 au[4], av[4], bu[4], bv[4];
         int kind = -1;  // whose norm weights they hold: 0 q, 1 k
-        for (int i0 = 0; i0 < my_slots; i0 += DEPTH) {
+        const RnStep *at_step = my_step0;
+        for (int s = part; s < n_steps; s += p.parts, at_step += step_stride) {
+            {
+                const RnStep to = *at_step;
+                const uint8_t *const stage = ring + use_at + lh * HD * ES;
+                use_at = (use_at + L::STAGE) & (DEPTH * L::STAGE - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"((int)DEPTH - 1) : "memory");
+                if (MODE == ROPE_HALF_ANY) __syncwarp();
+                RnChunk<F32> xu, xv;
+                xu.load(stage + cu * ES);
+                xv.load(stage + cv * ES);
+                F2 zu[4], zv[4];  // ROPE_HALF_ANY: partners in the middle of other lanes' chunks
+                if (MODE == ROPE_HALF_ANY) {
+                    auto z_of = [&](int c) {
+                        if (c >= p.rot) return 0.0f;
+                        const int at = c < half ? c + half : c - half;
+                        return F32 ? reinterpret_cast<const float *>(stage)[at]
+                                   : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(stage)[at]);
+                    };
 #pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                RnChunk<F32> xu = ru[d], xv = rv[d];
-                const bool more = i0 + DEPTH < my_slots;
-                fetch(d, more ? tok : nxt, more ? i0 + d + DEPTH : d);
-                const int s = part + (i0 + d) * p.parts;
-                if (s >= n_steps) continue;
-                const int now = s < nsq ? 0 : s < nsq + nsk ? 1 : 2;
-                const int h = (now == 0 ? s : now == 1 ? s - nsq : s - nsq - nsk) * HPW + lh;
+                    for (int e = 0; e < 4; ++e) {
+                        zu[e] = f2(z_of(cu + 2 * e), z_of(cu + 2 * e + 1));
+                        zv[e] = f2(z_of(cv + 2 * e), z_of(cv + 2 * e + 1));
+                    }
+                    __syncwarp();
+                }
+                issue();
+                const int now = s < nsq ? 0 : s < nsqk ? 1 : 2;
                 uint4 du, dv;
                 if (now == 2) {
                     du = xu.as_bf16();
@@ -207,7 +288,7 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
                 } else {
                     if (kind != now) {
                         kind = now;
-                        const float *w = s_w[kind], *ct = s_cos[warp], *st = s_sin[warp];
+                        const float *w = s_w + kind * HD, *ct = s_cos, *st = s_sin;
                         if (MODE == ROPE_HALF_LANES) {
                             lds_f2x4(au, w + cu);
                             lds_f2x4(av, w + cv);
@@ -291,21 +372,12 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
                                 if (cv + 2 * e < p.rot) ov[e] = f2_fma(f2(hi, lo), bv[e], ov[e]);
                             }
                         }
-                    } else {  // partners in the middle of other lanes' chunks: through shared memory
-                        float *sy = s_y[warp] + lh * HD;
+                    } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            f2_get(yu[e], sy[cu + 2 * e], sy[cu + 2 * e + 1]);
-                            f2_get(yv[e], sy[cv + 2 * e], sy[cv + 2 * e + 1]);
+                            ou[e] = f2_fma(zu[e], bu[e], ou[e]);
+                            ov[e] = f2_fma(zv[e], bv[e], ov[e]);
                         }
-                        __syncwarp();
-                        auto z_of = [&](int x) { return x >= p.rot ? 0.0f : sy[x < half ? x + half : x - half]; };
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            ou[e] = f2_fma(f2(z_of(cu + 2 * e), z_of(cu + 2 * e + 1)), bu[e], ou[e]);
-                            ov[e] = f2_fma(f2(z_of(cv + 2 * e), z_of(cv + 2 * e + 1)), bv[e], ov[e]);
-                        }
-                        __syncwarp();
                     }
                     const bool normed = (now == 0 ? p.q_norm : p.k_norm) != nullptr;
                     const float inv = normed ? rsqrtf(ss * (1.0f / HD) + p.eps) : 1.0f;
@@ -318,8 +390,8 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
                     du = make_uint4(f2_bf16(ou[0]), f2_bf16(ou[1]), f2_bf16(ou[2]), f2_bf16(ou[3]));
                     dv = make_uint4(f2_bf16(ov[0]), f2_bf16(ov[1]), f2_bf16(ov[2]), f2_bf16(ov[3]));
                 }
-                if (now == 0 ? h < p.n_q : h < p.n_kv && row_ok) {
-                    __nv_bfloat16 *dst = now == 0 ? q_dst + (long long)h * q_head : (now == 1 ? p.k : p.v) + kv0 + (long long)h * kv_head;
+                if (to.src >= 0 && (now == 0 || row_ok)) {
+                    __nv_bfloat16 *dst = to.dst + (now == 0 ? q_at : kv_at);
                     *reinterpret_cast<uint4 *>(dst + cu) = du;
                     *reinterpret_cast<uint4 *>(dst + cv) = dv;
                 }
@@ -331,15 +403,19 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
 template <int HD, int MODE, bool F32>
 static int launch_rope_norm(RopeNormParams &p, cudaStream_t stream) {
     constexpr int HPW = 32 / (HD / 16);
-    const int n_steps = (p.n_q + HPW - 1) / HPW + (p.n_heads > p.n_q ? 2 * ((p.n_kv + HPW - 1) / HPW) : 0);
-    // a warp per token once the tokens alone fill the machine (16 warps on every SM); fewer tokens: their heads over as many warps
-    const unsigned fill = 16u * (unsigned)sm_count();
-    const unsigned parts = p.M >= fill ? 1 : (fill + p.M - 1) / p.M;
-    p.parts = (int)parts < n_steps ? (int)parts : n_steps;
-    // persistent: two blocks on every SM.  One part: any number of blocks is a multiple of it; more: a token's warps are all there is.
-    unsigned blocks = (p.M * (unsigned)p.parts + RN_WARPS - 1) / RN_WARPS;  // M < 2^12, or parts == 1
-    if (p.parts == 1 && blocks > 2u * (unsigned)sm_count()) blocks = 2u * (unsigned)sm_count();
-    return launch_pdl(qk_norm_rope_kernel<HD, MODE, F32>, dim3((unsigned)blocks), dim3(RN_WARPS * 32), 0, stream, p);
+    p.nsq = (p.n_q + HPW - 1) / HPW;
+    p.nsk = p.n_heads > p.n_q ? (p.n_kv + HPW - 1) / HPW : 0;
+    const int n_steps = p.nsq + 2 * p.nsk, smem = RnSmem<HD, F32>::STEPS + n_steps * HPW * (int)sizeof(RnStep);
+    if (int rc = ensure_dyn_smem(qk_norm_rope_kernel<HD, MODE, F32>, smem)) return rc;
+    // Persistent: two blocks on every SM.  A warp takes whole tokens once every warp has four of them; fewer tokens: their heads over
+    // 2, 4 or 8 warps (a power of two divides the number of warps), and over as many as there are steps where one round does it.
+    const unsigned max_blocks = 2u * (unsigned)sm_count(), n_warps = max_blocks * RN_WARPS;
+    unsigned parts = 1;
+    while (parts < 8 && (long long)parts * p.M < 4LL * n_warps && (int)parts * 2 <= n_steps) parts *= 2;
+    if ((long long)p.M * n_steps <= (long long)n_warps) parts = (unsigned)n_steps;
+    p.parts = (int)parts;
+    unsigned blocks = (unsigned)(((long long)p.M * parts + RN_WARPS - 1) / RN_WARPS < max_blocks ? ((long long)p.M * parts + RN_WARPS - 1) / RN_WARPS : max_blocks);
+    return launch_pdl(qk_norm_rope_kernel<HD, MODE, F32>, dim3(blocks), dim3(RN_WARPS * 32), smem, stream, p);
 }
 
 template <int HD, bool F32>
@@ -397,9 +473,9 @@ int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, c
     vb::RopeNormParams p;
     const long long rows = (long long)st->n_obs * a->S;
     if (rows == 0) return VLAB200_OK;
-    if (rows > 0x7fffffffLL || (long long)a->S * hd > 0x7fffffffLL || (long long)n_heads * hd > 0x7fffffffLL ||
+    if (rows > 0x7fffffffLL || (long long)a->S * hd > 0x7fffffffLL || n_heads > 2048 ||
         (long long)st->cap * hd > 0x7fffffffLL) {
-        vb::set_last_error("qk_norm_rope_append: more than 2^31 - 1 rows, columns of a row or elements of a page");
+        vb::set_last_error("qk_norm_rope_append: more than 2^31 - 1 rows or elements of a page, or 2,048 heads of a row");
         return VLAB200_ERR_UNSUPPORTED;
     }
     p.M = (unsigned)rows;
