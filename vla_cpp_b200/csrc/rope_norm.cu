@@ -123,10 +123,11 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
     long long *const s_turn = reinterpret_cast<long long *>(rn_smem + L::TURN);         // turns per position in units of 2^-64
     const int half = p.rot >> 1;
     // This lane's two chunks start at columns cu and cv.  Half layout with rot % 16 == 0: the two columns of every pair are in one lane
-    // (columns from rot on: two chunks side by side); otherwise 16 columns side by side.
+    // (columns from rot on: two chunks side by side); otherwise half a head apart, so that neighbouring lanes read neighbouring chunks.
     const int jl = lane % LH, lh = lane / LH;
     const bool across = MODE == ROPE_HALF_LANES && jl < (p.rot >> 4);
-    const int cu = across ? jl * 8 : jl * 16, cv = across ? half + jl * 8 : jl * 16 + 8;
+    const int cu = MODE != ROPE_HALF_LANES || across ? jl * 8 : jl * 16;
+    const int cv = MODE != ROPE_HALF_LANES ? HD / 2 + jl * 8 : across ? half + jl * 8 : jl * 16 + 8;
     const bool turned = MODE == ROPE_HALF_LANES ? across : cu < p.rot;
     // a token's steps: those of its q heads, then of its k heads, then of its v heads, HPW heads each; this warp takes every parts-th
     const int nsq = p.nsq, nsqk = p.nsq + p.nsk, n_steps = p.nsq + 2 * p.nsk;
