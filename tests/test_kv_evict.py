@@ -49,6 +49,10 @@ CASES = [
     (1, 3, 2, 128, 40, [40, 3, 9], 8, 8, 4, 4, "zero"),             # and overlap in the short ones
     (3, 2, 1, 256, 900, [900, 899], 450, 500, 4, 48, "any"),        # infinities, no-numbers, negative and denormal weights
     (1, 4, 3, 64, 513, [512, 513, 511, 1], 257, 300, 0, 1, "exponents"),
+    (2, 2, 1, 64, 1024, [1024, 993], 992, 1000, 2, 31, "few values"),
+    (1, 3, 2, 64, 1025, [1025, 1024, 0], 1024, 1024, 0, 0, "any"),   # a block per page from here on
+    (1, 2, 1, 128, 5000, [5000, 1300], 1299, 1300, 10, 200, "few values"),
+    (1, 2, 2, 64, 3000, [3000, 2999], 100, 100, 0, 0, "any"),
 ]
 
 
