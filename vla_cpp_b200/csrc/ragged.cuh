@@ -20,9 +20,10 @@ struct RaggedCursor {
     int len, cnt, incl;  // of this lane's observation: rows, units, units up to and with it
     int total;           // units of the loaded 32
 
-    __device__ __forceinline__ RaggedCursor(LenOf f, int n_obs_, int n_kv_, int per_block_) : len_of(f), n_obs(n_obs_), n_kv(n_kv_), per_block(per_block_) {
-        obs0 = base = 0;
-        load();
+    __device__ __forceinline__ RaggedCursor(LenOf f, int n_obs_, int n_kv_, int per_block_, bool used = true)
+        : len_of(f), n_obs(n_obs_), n_kv(n_kv_), per_block(per_block_) {
+        obs0 = base = len = cnt = incl = total = 0;
+        if (used) load();
     }
     __device__ __forceinline__ void load() {
         const int lane = threadIdx.x & 31;
