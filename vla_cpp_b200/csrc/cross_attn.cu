@@ -64,6 +64,12 @@ __device__ __forceinline__ float xa_max3(float a, float b, float c) {
     return d;
 }
 
+// The hidden range of an observation; (none, none) if it has none.
+__device__ __forceinline__ void xa_pad(const CrossParams &p, int obs, int &lo, int &hi) {
+    lo = p.pad ? p.pad[2 * obs] : 0;
+    hi = p.pad ? p.pad[2 * obs + 1] : 0;
+    if (hi <= lo) lo = hi = 0x7fffffff;
+}
 // The blocks of all units, and the piece of CTA `c` of `n`.
 __device__ __forceinline__ int xa_total_blocks(const CrossParams &p) {  // whole warp
     int sum = 0;
@@ -76,6 +82,7 @@ __device__ __forceinline__ int xa_border(int c, int n, int total) { return (int)
 
 struct XaSegment {  // a run of blocks [j0, j1) of one unit
     int obs, kvh, mt, j0, j1, len, slot;  // slot: of the workspace; -1: the unit is whole
+    int pad_lo, pad_hi;                   // hidden rows
 };
 
 // Whole units of up to XA_SORT observations: longest observations first, dealt to the CTAs there and back, so that who has a long one first
@@ -83,13 +90,16 @@ struct XaSegment {  // a run of blocks [j0, j1) of one unit
 // observations, 9 so; 8.5 on average).
 constexpr int XA_SORT = 256;
 struct XaOrder {
-    int len[XA_SORT];  // by observation
-    int obs[XA_SORT];  // by rank
+    int len[XA_SORT], pad_lo[XA_SORT], pad_hi[XA_SORT];  // by observation
+    int obs[XA_SORT];                                    // by rank
     int n_live;        // observations that have rows
 };
 __device__ __forceinline__ void xa_sort(const CrossParams &p, XaOrder &o, int n_threads) {  // the whole block
     if (p.ws_o != nullptr || p.n_obs > XA_SORT) return;
-    for (int i = threadIdx.x; i < p.n_obs; i += n_threads) o.len[i] = xa_len(p, i);
+    for (int i = threadIdx.x; i < p.n_obs; i += n_threads) {
+        o.len[i] = xa_len(p, i);
+        xa_pad(p, i, o.pad_lo[i], o.pad_hi[i]);
+    }
     if (threadIdx.x == 0) o.n_live = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < p.n_obs; i += n_threads) {
@@ -109,10 +119,11 @@ template <typename LenOf>
 struct XaWork {
     RaggedCursor<LenOf> cur;
     const XaOrder &order;
+    const CrossParams &p;
     int w, w1, c, n_mt, n_kv, n_work;  // sorted: w is the round, w1 the number of units
     bool whole_units, sorted;
     __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, const XaOrder &o, int cta)
-        : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV, p.ws_o != nullptr || p.n_obs > XA_SORT), order(o) {
+        : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV, p.ws_o != nullptr || p.n_obs > XA_SORT), order(o), p(p) {
         c = cta;
         n_mt = p.n_mt;
         n_kv = p.n_kv;
@@ -136,6 +147,8 @@ struct XaWork {
             const int upo = n_kv * n_mt, r = k / upo, u = k - r * upo;
             s.obs = order.obs[r];
             s.len = order.len[s.obs];
+            s.pad_lo = order.pad_lo[s.obs];
+            s.pad_hi = order.pad_hi[s.obs];
             s.kvh = u / n_mt;
             s.mt = u - s.kvh * n_mt;
             s.j0 = 0;
@@ -152,6 +165,7 @@ struct XaWork {
             }
             s.obs = u.obs;
             s.len = u.len;
+            xa_pad(p, s.obs, s.pad_lo, s.pad_hi);
             s.kvh = u.kvh / n_mt;
             s.mt = u.kvh - s.kvh * n_mt;
             s.j0 = u.block;
@@ -189,12 +203,6 @@ __device__ __forceinline__ void xa_fill_empty(const CrossParams &p, int c, int t
     }
 }
 
-// The hidden range of an observation; (none, none) if it has none.
-__device__ __forceinline__ void xa_pad(const CrossParams &p, int obs, int &lo, int &hi) {
-    lo = p.pad ? p.pad[2 * obs] : 0;
-    hi = p.pad ? p.pad[2 * obs + 1] : 0;
-    if (hi <= lo) lo = hi = 0x7fffffff;
-}
 // Does the mask hide rows of the block that begins at row c0?
 __device__ __forceinline__ bool xa_dirty(int c0, int len, int pad_lo, int pad_hi) {
     return c0 + XA_BKV > len || (c0 < pad_hi && c0 + XA_BKV > pad_lo);
@@ -203,11 +211,10 @@ __device__ __forceinline__ bool xa_dirty(int c0, int len, int pad_lo, int pad_hi
 // Hidden rows of a V block meet weights of 0, and 0 times what stands there need not be 0.  So a dirty block's TMA completes on v_raw, and
 // this warp zeroes those rows in shared memory and then says v_full in its place.
 template <int CB>
-__device__ __forceinline__ void xa_clean_blocks(const CrossParams &p, XaSegment &s, bool &ok, uint32_t &jb, uint8_t *v_smem, int stages, int stage_bytes,
+__device__ __forceinline__ void xa_clean_blocks(XaSegment &s, bool &ok, uint32_t &jb, uint8_t *v_smem, int stages, int stage_bytes,
                                                 uint64_t *v_raw, uint64_t *v_full, uint32_t &raw_phase, const WaitCtx &wc) {
     const int lane = threadIdx.x & 31;
-    int pad_lo, pad_hi;
-    xa_pad(p, s.obs, pad_lo, pad_hi);
+    const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
     for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
         const int c0 = j * XA_BKV;
         if (!xa_dirty(c0, s.len, pad_lo, pad_hi)) continue;
@@ -226,6 +233,20 @@ __device__ __forceinline__ void xa_clean_blocks(const CrossParams &p, XaSegment 
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[st]);
+    }
+}
+
+// -inf over the hidden ones of 32 columns that begin at row c0; groups that hide nothing cost nothing (all 128 columns of a block tested for
+// length and range took 2,000 clocks).
+__device__ __forceinline__ void xa_mask32(uint32_t (&x)[32], int c0, int len, int pad_lo, int pad_hi) {
+    const int lim = len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
+    if (lim < 32) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = e < lim ? x[e] : 0xff800000u;
+    }
+    if (lo < 32 && hi > 0) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = e < lo || e >= hi ? x[e] : 0xff800000u;
     }
 }
 
@@ -319,8 +340,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         for (; ok && work.next(s); ++si) {
             const int item = s.obs * p.n_kv + s.kvh, row0 = s.mt * 256;
             const int tiles = p.R > row0 + 128 ? 2 : 1;
-            int pad_lo, pad_hi;
-            xa_pad(p, s.obs, pad_lo, pad_hi);
+            const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
             const uint32_t qs = si % QS;
             ok = warp_wait(&q_free[qs], (si / QS & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
             if (!ok) break;
@@ -352,7 +372,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     } else if (warp == XA_CLEANER) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
         uint32_t jb = 0, raw_phase = 0;
-        while (ok && work.next(s)) xa_clean_blocks<L::CB>(p, s, ok, jb, smem + L::V_OFF, NS, L::KV_BYTES, v_raw, v_full, raw_phase, wc);
+        while (ok && work.next(s)) xa_clean_blocks<L::CB>(s, ok, jb, smem + L::V_OFF, NS, L::KV_BYTES, v_raw, v_full, raw_phase, wc);
     } else if (warp == XA_MMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
         constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 128, BKV), idesc_o = make_idesc(1, 1, 1, 0, 1, 128, HD);
@@ -435,8 +455,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             if (t == 1 && row0 >= p.R) continue;
             const int lr = t * 128 + qtr * 32 + lane, row = s.mt * 256 + lr;  // in the unit, in the item
             const bool live = row0 + qtr * 32 < p.R;                          // of the warp
-            int pad_lo, pad_hi;
-            xa_pad(p, s.obs, pad_lo, pad_hi);
+            const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units, row sum
             for (int j = s.j0; j < s.j1; ++j, ++blk) {
                 ok = warp_wait(&s_full[t], blk & 1u, wc, DEV_TIMEOUT_FULL);
@@ -451,14 +470,8 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + (uint32_t)(i * 32), x[i]);
                     tmem_ld_wait();
                     if (dirty) {
-                        const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const int c = i * 32 + e;
-                                x[i][e] = c < lim && (c < lo || c >= hi) ? x[i][e] : 0xff800000u;
-                            }
+                        for (int i = 0; i < 4; ++i) xa_mask32(x[i], c0 + i * 32, s.len, pad_lo, pad_hi);
                     }
                     float mx[4];
 #pragma unroll
@@ -672,8 +685,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     if (warp == XP_LOADER) {
         for (; ok && work.next(s); ++si) {
             const int item = s.obs * p.n_kv + s.kvh;
-            int pad_lo, pad_hi;
-            xa_pad(p, s.obs, pad_lo, pad_hi);
+            const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
             ok = warp_wait(q_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
             if (!ok) break;
             if (elect_one()) {
@@ -704,7 +716,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         }
     } else if (warp == XP_CLEANER) {  // of this CTA's half of V's columns
         uint32_t raw_phase = 0;
-        while (ok && work.next(s)) xa_clean_blocks<L::CBH>(p, s, ok, jb, smem + L::V_OFF, ST, L::V_BYTES, v_raw, v_full, raw_phase, wc);
+        while (ok && work.next(s)) xa_clean_blocks<L::CBH>(s, ok, jb, smem + L::V_OFF, ST, L::V_BYTES, v_raw, v_full, raw_phase, wc);
     } else if (warp == XP_S) {
         if (rank == 0) {
             constexpr uint32_t idesc_s = make_idesc(1, 1, 1, 0, 0, 256, BKV);
@@ -852,8 +864,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         XaSegment prev;
         float prev_m = 0.0f, prev_l = 0.0f;
         for (; ok && work.next(s); ++si) {
-            int pad_lo, pad_hi;
-            xa_pad(p, s.obs, pad_lo, pad_hi);
+            const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units (the same in both halves), this half's part of the row sum
             for (int j = s.j0; j < s.j1; ++j, ++jb) {
                 const uint32_t sb = jb % NS;
@@ -868,14 +879,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 const int b0 = j * BKV, c0 = b0 + half * 64;
                 const bool dirty = xa_dirty(b0, s.len, pad_lo, pad_hi);
                 if (dirty) {
-                    const int lim = s.len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int c = i * 32 + e;
-                            x[i][e] = c < lim && (c < lo || c >= hi) ? x[i][e] : 0xff800000u;
-                        }
+                    for (int i = 0; i < 2; ++i) xa_mask32(x[i], c0 + i * 32, s.len, pad_lo, pad_hi);
                 }
                 float mx[2];
 #pragma unroll
