@@ -965,7 +965,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
 // pieces as many as there are CTAs (one token over 16,001 rows, a warp per row: 40 us).
 template <int HD, int TEAM>
 __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p) {
-    __shared__ __align__(8) float s_o[8][TEAM > 1 ? HD : 1], s_l[8];
+    __shared__ __align__(8) float s_o[8][TEAM > 1 ? HD : 1], s_l[8], s_m[8];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -989,10 +989,7 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
 #pragma unroll
         for (int i = 0; i < NV; ++i) acc[i] = make_float2(0.0f, 0.0f);
         float l = 0.0f, M = -INFINITY;
-        for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, p.ws_ml[slot_of(c) * 2]);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        for (int c = c0 + member; c <= c1; c += 4 * TEAM) {
+        for (int c = c0 + member; c <= c1; c += 4 * TEAM) {  // four pieces asked for at once, under the maximum so far
             float2 v[4][NV], ml[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -1001,10 +998,16 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
 #pragma unroll
                 for (int k = 0; k < NV; ++k) v[i][k] = reinterpret_cast<const float2 *>(p.ws_o + at * HD)[k * 32 + lane];
             }
+            // (a piece that was asked for twice has its weight once)
+            const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M);
+            const float old = M == -INFINITY ? 0.0f : xa_ex2(M - top);
+            M = top;
+            l *= old;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) acc[k] = make_float2(acc[k].x * old, acc[k].y * old);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (c + i * TEAM > c1) break;
-                const float w = ml[i].x == -INFINITY ? 0.0f : xa_ex2(ml[i].x - M);
+                const float w = c + i * TEAM > c1 || ml[i].x == -INFINITY ? 0.0f : xa_ex2(ml[i].x - M);
                 l = fmaf(ml[i].y, w, l);
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
@@ -1018,16 +1021,25 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
         if (TEAM > 1) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) reinterpret_cast<float2 *>(s_o[warp])[k * 32 + lane] = acc[k];
-            if (lane == 0) s_l[warp] = l;
+            if (lane == 0) {
+                s_l[warp] = l;
+                s_m[warp] = M;
+            }
             __syncthreads();
             l = 0.0f;
 #pragma unroll
-            for (int w = 0; w < TEAM; ++w) l += s_l[w];
+            for (int w = 0; w < TEAM; ++w) M = fmaxf(M, s_m[w]);
+            float scale[TEAM];
+#pragma unroll
+            for (int w = 0; w < TEAM; ++w) {
+                scale[w] = s_m[w] == -INFINITY ? 0.0f : xa_ex2(s_m[w] - M);
+                l = fmaf(s_l[w], scale[w], l);
+            }
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             for (int i = threadIdx.x; i < HD; i += 256) {
                 float o = 0.0f;
 #pragma unroll
-                for (int w = 0; w < TEAM; ++w) o += s_o[w][i];
+                for (int w = 0; w < TEAM; ++w) o = fmaf(s_o[w][i], scale[w], o);
                 dst[i] = __float2bfloat16_rn(o * inv);
             }
             __syncthreads();
@@ -1061,11 +1073,10 @@ static CrossPlan cross_plan(int hd, long long items, int R, int max_len, int n_s
     c.n_mt = (R + 255) / 256;
     c.n_work = hd == 256 ? n_sm / 2 : n_sm;
     c.ws_rows = R < 256 ? R : 256;
-    // Whole units take rounds of n_work; cut ones fill the last round, for the pieces' way through the workspace and a second kernel:
-    // some 10 us, six blocks.  (64 observations, heads of 64, 1 or 2 blocks: 34 us whole, 45 cut; heads of 256, up to 7 blocks: 47 and
-    // 55; 4 observations of 64 blocks: 272 and 233; 1 of 126 blocks: 176 and 27.)
+    // Whole units take rounds of n_work; cut ones fill the last round, for the pieces' way through the workspace and a second kernel: the
+    // time of some 6 blocks, and of 10 more where the pieces are full tiles.
     const long long units = items * c.n_mt, nb = (max_len + XA_BKV - 1) / XA_BKV, rounds = (units + c.n_work - 1) / c.n_work;
-    const bool cut = (rounds * c.n_work - units) * nb > 6LL * c.n_work;
+    const bool cut = (rounds * c.n_work - units) * nb > (6LL + 10LL * c.ws_rows / 256) * c.n_work;
     c.ws_bytes = cut ? 2LL * c.n_work * c.ws_rows * (hd + 2) * 4 : 0;
     return c;
 }
