@@ -12,7 +12,7 @@
 //   loader warp      TMA: the unit's K tile and its query rows, chunks of at most NQ, through rings whose depths share 192 KB
 //   MMA warp         even CTA: D[256 keys][n rows] = K Q_chunk^T, n = the chunk's rows rounded up to 32 (one token: 32 columns), NB
 //                    accumulators; odd CTA: tells the even one what has landed
-//   16 sum warps     lane quarter = warp & 3, a quarter of the columns = warp >> 2: p = 2^(s c - lse'), two columns per FMA instruction
+//   16 sum warps     four per lane quarter, 128 columns of every second (heads of 256: fourth) chunk each: p = 2^(s c - lse')
 //
 // One query token: K streams once, HBM bounds it.  Many: the exponentials (heads of 64 and 128) or the product (256).
 #include <cuda_bf16.h>
@@ -24,7 +24,7 @@
 
 namespace vb {
 
-constexpr int KM_PARTS = 4;  // sum warps per lane quarter: each takes NQ / KM_PARTS columns of a chunk
+constexpr int KM_PARTS = 4;  // sum warps per lane quarter
 constexpr int KM_SUMS = 4 * KM_PARTS, KM_LOADER = KM_SUMS, KM_MMA = KM_SUMS + 1, KM_THREADS = 32 * (KM_SUMS + 2);
 
 struct KeyMassParams {
@@ -47,9 +47,9 @@ struct KeyMassSmem {
     static constexpr int Q_BYTES = CB * (NQ / 2) * 128;  // [CB][box_rows][128 B]: this CTA's half of a chunk
     static constexpr int RING = 192 * 1024;
     static constexpr int BAR_OFF = RING;
-    static constexpr int PART = NQ / KM_PARTS;        // columns of a sum warp
-    static constexpr int LSE_OFF = BAR_OFF + 512;     // float [2][KM_SUMS][PART]
-    static constexpr int SUM_OFF = LSE_OFF + 2 * KM_SUMS * PART * 4;  // float [2][KM_PARTS - 1][128]
+    static constexpr int PPC = NQ / 128, G = KM_PARTS / PPC;  // parts that share a chunk, 128 columns each; groups of them
+    static constexpr int LSE_OFF = BAR_OFF + 512;     // float [KM_SUMS][128]
+    static constexpr int SUM_OFF = LSE_OFF + KM_SUMS * 128 * 4;  // float [2][KM_PARTS - 1][128]
     static constexpr int TOTAL = SUM_OFF + 2 * (KM_PARTS - 1) * 128 * 4 + 1024;
     static_assert(2 * K_BYTES + 2 * Q_BYTES <= RING && TOTAL <= 227 * 1024, "shared memory");
 };
@@ -99,7 +99,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&a_full[i], 1);
-            mbar_init(&a_free[i], 2 * KM_SUMS);  // the sum warps of both CTAs (used in the even one)
+            mbar_init(&a_free[i], 2 * 4 * L::PPC);  // a chunk's sum warps in both CTAs (used in the even one)
             mbar_init(&meet[i], 32 * KM_PARTS);
         }
         *abort_flag = 0;
@@ -202,9 +202,13 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             }
         }
     } else {
-        const int qtr = warp & 3, part = warp >> 2;
-        constexpr int PART = L::PART, NBLK = PART / 32;
-        float *lse_s = reinterpret_cast<float *>(smem + L::LSE_OFF) + warp * PART;
+        // Parts in groups: a chunk is one group's, the next chunk the next group's, so that the groups are at different points of their work
+        // (all of them on every chunk, a quarter of its columns each, they waited and computed in step).  Which group begins a
+        // unit turns from unit to unit; `rel`, the group's place in that turn, says which chunks it adds up, and where its sum goes, so a
+        // unit's sums do not depend on what the pair did before.
+        constexpr int PPC = L::PPC, G = L::G, NBLK = 4;
+        const int qtr = warp & 3, part = warp >> 2, sub = part % PPC, group = part / PPC;
+        float *ls = reinterpret_cast<float *>(smem + L::LSE_OFF) + warp * 128;
         float *sum_s = reinterpret_cast<float *>(smem + L::SUM_OFF);
         const uint32_t lane_sel = (uint32_t)(qtr * 32) << 16;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
@@ -212,37 +216,39 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         auto fetch_lse = [&](bool there, const RaggedUnit &u, int c) {
 #pragma unroll
             for (int i = 0; i < NBLK; ++i) {
-                const int r = c * L::NQ + part * PART + i * 32 + lane;
-                lv[i] = there && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : INFINITY;
+                const int r = c * L::NQ + sub * 128 + i * 32 + lane;
+                lv[i] = there && c < p.n_chunks && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : INFINITY;
             }
         };
-        uint32_t qu = 0, un = 0;
-        KmStage ab;
+        uint32_t qu = 0, un = 0;  // chunks in front of this unit, units
         bool ok = true;
         int ui = cid;
         bool there = cursor.find(ui, unit);
-        fetch_lse(there, unit, 0);
+        fetch_lse(there, unit, group);
         while (ok && there) {
             const RaggedUnit now = unit;
             ui += ncl;
             there = cursor.find(ui, unit);
             const int item = now.obs * p.n_kv + now.kvh, key0 = now.block * 256 + (int)rank * 128, obs = now.obs;
+            const int rel = (int)((group + G - un % G) % G), rel_next = (rel + G - 1) % G;
             F2 acc[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i] = f2(0.0f, 0.0f);
-            for (int c = 0; c < p.n_chunks; ++c, ++qu) {
+            if (rel >= p.n_chunks) fetch_lse(there, unit, rel_next);
+            for (int c = rel; c < p.n_chunks; c += G) {
+                const uint32_t q = qu + (uint32_t)c, ab = q % L::NB;
                 // rows past the last, and rows that saw nothing (-inf), weigh nothing: 2^(s - inf)
-                float *ls = lse_s + (qu & 1u) * (KM_SUMS * PART);
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < NBLK; ++i) ls[i * 32 + lane] = lv[i] == -INFINITY ? -INFINITY : -1.4426950408889634f * lv[i];
                 __syncwarp();
-                if (c + 1 < p.n_chunks) fetch_lse(true, now, c + 1);
-                else fetch_lse(there, unit, 0);
-                ok = warp_wait(&a_full[ab.i], ab.ph, wc, DEV_TIMEOUT_ACCUM);
+                if (c + G < p.n_chunks) fetch_lse(true, now, c + G);
+                else fetch_lse(there, unit, rel_next);
+                ok = warp_wait(&a_full[ab], q / L::NB & 1u, wc, DEV_TIMEOUT_ACCUM);
                 if (!ok) break;
                 tc_fence_after();
-                const int n = min(p.R - c * L::NQ - part * PART, PART);  // of this warp's columns; may be 0 or less
-                const uint32_t d = tmem_base + lane_sel + ab.i * L::NQ + (uint32_t)(part * PART);
+                const int n = min(p.R - c * L::NQ - sub * 128, 128);  // of this warp's columns; may be 0 or less
+                const uint32_t d = tmem_base + lane_sel + ab * L::NQ + (uint32_t)(sub * 128);
 #pragma unroll
                 for (int b = 0; b < NBLK; ++b) {
                     uint32_t s[32];
@@ -254,8 +260,8 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
-                            if (rank == 0) mbar_arrive(&a_free[ab.i]);
-                            else mbar_arrive_cluster(&a_free[ab.i], 0);
+                            if (rank == 0) mbar_arrive(&a_free[ab]);
+                            else mbar_arrive_cluster(&a_free[ab], 0);
                         }
                     }
                     if (b * 32 >= n) continue;
@@ -277,22 +283,23 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                         }
                     }
                 }
-                ab.next(L::NB);
             }
             if (!ok) break;
+            qu += (uint32_t)p.n_chunks;
             float x[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) f2_get(acc[i], x[2 * i], x[2 * i + 1]);
             float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             // the parts of the columns meet; the slots are used in turn, so one meeting per unit is enough
             float *slot = sum_s + (un & 1u) * ((KM_PARTS - 1) * 128) + qtr * 32 + lane;
-            if (part) slot[(part - 1) * 128] = sum;
+            const int place = rel * PPC + sub;
+            if (place) slot[(place - 1) * 128] = sum;
             mbar_arrive(&meet[qtr]);
             ok = warp_wait(&meet[qtr], un & 1u, wc, DEV_TIMEOUT_MISC);
             if (!ok) break;
             ++un;
             const int key = key0 + qtr * 32 + lane;
-            if (!part && key < now.len) {
+            if (!place && key < now.len) {
 #pragma unroll
                 for (int i = 0; i < KM_PARTS - 1; ++i) sum += slot[i * 128];
                 if (p.pad && key >= p.pad[2 * obs] && key < p.pad[2 * obs + 1]) sum = 0.0f;
