@@ -174,6 +174,8 @@ VLAB200_API int32_t vlab200_denoise_attn_loop_host(const vlab200_kv_store *st, c
                                                    void *x_stage, void *out_host, void *stream);
 
 /* --------------------------------------------- a prefix cache whose observations differ in length */
+/* In this section a buffer that a call writes may not overlap one that it reads, or another one that it writes (VLAB200_ERR_ARG), but for
+ * mass_in and mass_out of vlab200_key_mass, which may be the same. */
 
 /* Angles per position of the rotated pairs of a head, and the factor on their cosines and sines (host only; needs no GPU).
  * freqs_host: double [rot_dim/2].  scaling 0 = none: f_i = base^(-2i/rot_dim); 1 = linear: f_i / factor; 2 = NTK-aware:
@@ -245,7 +247,7 @@ VLAB200_API int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, 
  * kept: int32 [n_layers][n_obs][n_kv][keep], the rows' indices in src, then -1.  mass_out (optional): float32
  * [n_layers][n_obs][n_kv][dst cap], their weights, then 0.  lens_out (optional): int32 [n_obs], min(n, keep).  Rows of dst behind
  * them are left as they were.  lens: int32 [n_obs], taken into [0, max_len], or NULL (max_len); max_len <= src cap, keep <= dst cap.  The
- * stores differ in nothing but cap and prefix_len, and no buffer that is written may overlap another of the call (VLAB200_ERR_ARG).
+ * stores differ in nothing but cap, prefix_len and memory.
  * A store of keep + suffix rows with prefix_len = keep then serves the calls above as the larger one did, with the suffix at its old
  * positions.  No counterpart in the reference. */
 VLAB200_API int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_kv_store *dst, const float *mass, const int32_t *lens,

@@ -17,17 +17,18 @@ def test_argument_checks_need_no_gpu():
     from vla_cpp_b200 import api
 
     def call(**kw):
-        st = api._KvStoreC(*(kw.pop(n, d) for n, d in (("k", 16), ("v", 16), ("layers", 1), ("obs", 2), ("n_kv", 1), ("hd", 64),
+        st = api._KvStoreC(*(kw.pop(n, d) for n, d in (("k", 1 << 20), ("v", 2 << 20), ("layers", 1), ("obs", 2), ("n_kv", 1), ("hd", 64),
                                                        ("cap", 8), ("prefix", 0))))
         g = lambda n, d: kw.pop(n, d)
         p = lambda v: C.c_void_p(v) if v else None
-        return api.lib().vlab200_cross_attention(C.byref(st), g("layer", 0), p(g("q", 16)), p(g("out", 32)), p(g("lse", 16)), g("S", 1), g("n_q", 2),
+        return api.lib().vlab200_cross_attention(C.byref(st), g("layer", 0), p(g("q", 3 << 20)), p(g("out", 4 << 20)), p(g("lse", 5 << 20)), g("S", 1), g("n_q", 2),
                                                  None, g("max_len", 8), None, C.c_float(g("scale", 0.0)), p(g("ws", None)),
                                                  C.c_int64(g("ws_bytes", 0)), None)
 
     for bad in (dict(k=None), dict(v=None), dict(q=None), dict(out=None), dict(layer=1), dict(layer=-1), dict(S=0), dict(n_q=0), dict(n_q=3, n_kv=2),
                 dict(max_len=9), dict(max_len=-1), dict(scale=-1.0), dict(scale=math.nan), dict(q=24), dict(k=8), dict(v=24), dict(out=40),
-                dict(ws=16, ws_bytes=1 << 30), dict(ws_bytes=-1), dict(obs=0), dict(cap=0)):
+                dict(ws=16, ws_bytes=1 << 30), dict(ws_bytes=-1), dict(obs=0), dict(cap=0),
+                dict(out=3 << 20), dict(out=1 << 20), dict(lse=4 << 20), dict(lse=(2 << 20) + 64)):
         assert call(**bad) == -1, bad
     assert call(hd=80) == -4
     st = api._KvStoreC(16, 16, 1, 2, 2, 64, 8, 0)
@@ -54,6 +55,9 @@ CASES = [
     (5, 300, 2, 2, 64, 1500, None, False),
     (3, 200, 4, 2, 128, 1500, None, True),
     (3, 100, 4, 1, 256, 1500, None, True),
+    (300, 2, 2, 2, 64, 200, None, True),                # more observations than are sorted
+    (270, 20, 8, 1, 256, 300, None, False),
+    (260, 70, 4, 1, 128, 150, None, True),
 ]
 
 
@@ -135,6 +139,28 @@ def test_lengths_by_default_and_out_of_range_and_a_scale(hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 256])
+def test_hidden_ranges_at_the_borders(hd):
+    """Ranges that are empty, turned round, reach out of the rows on either side, or hide everything; lengths at the blocks' borders."""
+    torch = require_cuda()
+    import vla_cpp_b200 as vb
+
+    lo_hi = [(0, 0), (9, 3), (-2 ** 31, 5), (250, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 1), (0, 128), (128, 256), (127, 129), (-7, -3), (2 ** 31 - 1, 2 ** 31 - 1)]
+    lens = [256, 255, 129, 256, 256, 128, 256, 129, 1, 127]
+    B = len(lens)
+    st, q, lens, _, g = make(torch, B, 3, 4, 2, hd, 256, lens, False, 17)
+    pads = torch.tensor(lo_hi, dtype=torch.int32, device="cuda")
+    out, lse = vb.cross_attention(st, 0, q, lens=lens, pad_ranges=pads)
+    assert vb.device_status() == 0
+    check(torch, st, 0, q, lens, pads.long(), out, lse)
+    mass = vb.key_mass(st, 0, q, lse, lens=lens, pad_ranges=pads)
+    seen = visible(torch, 256, lens, pads.long())
+    z = scores(st, 0, q).masked_fill(~seen[:, None, None], -math.inf)
+    want = torch.exp(z - lse.double().reshape(B, 2, -1, 1).nan_to_num(neginf=math.inf)).sum(2)
+    torch.testing.assert_close(mass.double(), want, rtol=1e-4, atol=0)
+
+
+@pytest.mark.gpu
 def test_refusals():
     torch = require_cuda()
     import vla_cpp_b200 as vb
@@ -143,7 +169,7 @@ def test_refusals():
     z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t, device="cuda")
     for kw in (dict(q=q.float()), dict(q=q.cpu()), dict(q=q[0]), dict(q=q.transpose(1, 2)), dict(q=q[:1]), dict(lens=z(2)), dict(lens=lens.cpu()),
                dict(pad_ranges=z(2, t=torch.int32)), dict(out=z(2, 3, 256)), dict(lse=z(2, 3, 4)), dict(max_len=21), dict(max_len=-1), dict(layer=2),
-               dict(scale=-1.0), dict(q=z(2, 3, 3, 64, t=torch.bfloat16)), dict(q=z(2, 4, 0, 64, t=torch.bfloat16))):
+               dict(scale=-1.0), dict(out=q.view(2, 3, 256)), dict(q=z(2, 3, 3, 64, t=torch.bfloat16)), dict(q=z(2, 4, 0, 64, t=torch.bfloat16))):
         kw = {**dict(q=q, layer=0), **kw}
         with pytest.raises(vb.VlaB200Error) as e:
             vb.cross_attention(st, kw.pop("layer"), kw.pop("q"), **kw)

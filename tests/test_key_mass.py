@@ -16,18 +16,19 @@ def test_argument_checks_need_no_gpu():
     from vla_cpp_b200 import api
 
     def call(**kw):
-        st = api._KvStoreC(*(kw.pop(n, d) for n, d in (("k", 16), ("v", 16), ("layers", 1), ("obs", 2), ("n_kv", 1), ("hd", 64),
+        st = api._KvStoreC(*(kw.pop(n, d) for n, d in (("k", 1 << 20), ("v", 2 << 20), ("layers", 1), ("obs", 2), ("n_kv", 1), ("hd", 64),
                                                        ("cap", 8), ("prefix", 0))))
         g = lambda n, d: kw.pop(n, d)
         p = lambda v: C.c_void_p(v) if v else None
-        return api.lib().vlab200_key_mass(C.byref(st), g("layer", 0), p(g("q", 16)), p(g("lse", 16)), p(g("mass", 16)), p(g("out", 16)),
+        return api.lib().vlab200_key_mass(C.byref(st), g("layer", 0), p(g("q", 3 << 20)), p(g("lse", 4 << 20)), p(g("mass", 5 << 20)), p(g("out", 6 << 20)),
                                           g("S", 1), g("n_q", 2), None, g("max_len", 0), None, C.c_float(g("scale", 0.0)),
                                           C.c_float(g("decay", 1.0)), None)
 
     assert call() == 0  # no rows
     for bad in (dict(k=None), dict(q=None), dict(lse=None), dict(out=None), dict(layer=1), dict(layer=-1), dict(S=0), dict(n_q=0),
                 dict(n_q=3, n_kv=2), dict(max_len=9), dict(max_len=-1), dict(scale=-1.0), dict(scale=math.nan), dict(decay=-0.5),
-                dict(decay=math.nan), dict(q=24), dict(k=8)):
+                dict(decay=math.nan), dict(q=24), dict(k=8), dict(max_len=8, out=3 << 20), dict(max_len=8, out=4 << 20), dict(max_len=8, out=1 << 20),
+                dict(max_len=8, out=(5 << 20) + 4)):
         assert call(**bad) == -1, bad
     assert call(hd=80) == -4
 
@@ -138,7 +139,7 @@ def test_refusals():
     st, q, lens, _, _ = make(torch, 2, 3, 4, 2, 64, 20, [20, 20], False, 7)
     lse = torch.zeros(2, 4, 3, device="cuda")
     z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t, device="cuda")
-    for kw in (dict(q=q.float()), dict(q=q.cpu()), dict(q=q[0]), dict(q=q.transpose(1, 2)), dict(q=q[:1]), dict(lse=lse.half()), dict(lse=z(2, 3, 4)),
+    for kw in (dict(out=lse.new_zeros(1).expand(80).reshape(2, 2, 20)[:1]), dict(q=q.float()), dict(q=q.cpu()), dict(q=q[0]), dict(q=q.transpose(1, 2)), dict(q=q[:1]), dict(lse=lse.half()), dict(lse=z(2, 3, 4)),
                dict(lens=z(2)), dict(lens=z(3, t=torch.int32)), dict(pad_ranges=z(2, t=torch.int32)), dict(mass=z(2, 2, 19)),
                dict(out=z(2, 2, 20, t=torch.bfloat16)), dict(max_len=21), dict(max_len=-1), dict(layer=2), dict(decay=-1.0),
                dict(q=z(2, 3, 3, 64, t=torch.bfloat16), lse=z(2, 3, 3))):
@@ -146,3 +147,6 @@ def test_refusals():
         with pytest.raises(vb.VlaB200Error) as e:
             vb.key_mass(st, kw.pop("layer"), kw.pop("q"), kw.pop("lse"), **kw)
         assert e.value.code == -1, kw
+    both = z(2 * 2 * 20 + 4)  # weights that overlap the ones they replace without being them
+    with pytest.raises(vb.VlaB200Error):
+        vb.key_mass(st, 0, q, lse, lens=lens, mass=both[:80].view(2, 2, 20), out=both[4:].view(2, 2, 20))

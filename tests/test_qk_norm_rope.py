@@ -207,7 +207,7 @@ def test_refusals():
            dict(S=S + 1), dict(n_q=3), dict(freqs=freqs.float()), dict(freqs=freqs.cpu()), dict(freqs=z(hd // 2 + 1, t=torch.float64)),
            dict(q_norm=z(hd + 1, t=torch.float32)), dict(k_norm=z(hd, t=torch.bfloat16)), dict(pos=z(B * S)), dict(row0=z(B, t=torch.int64)),
            dict(n_tok=z(B + 1)), dict(q_out=z(B, n_q, S, hd, t=torch.float32)), dict(q_out=z(B, S, n_q, hd, t=torch.bfloat16)),
-           dict(layer=1), dict(eps=-1.0)]
+           dict(layer=1), dict(eps=-1.0), dict(q_out=good["x"].view(-1)[:B * n_q * S * hd].view(B, n_q, S, hd))]
     for kw in bad:
         kw = {**good, "layer": 0, **kw}
         with pytest.raises(vb.VlaB200Error) as e:

@@ -37,6 +37,13 @@ def lib():
                 fn.restype = C.c_int32
         L.vlab200_kv_store_bytes.restype = C.c_int64
         L.vlab200_cross_attention_ws_bytes.restype = C.c_int64
+        # declared types: addresses, numbers and NULL go in as they are
+        vp, i32, f32 = C.c_void_p, C.c_int32, C.c_float
+        L.vlab200_cross_attention_ws_bytes.argtypes = [vp, i32, i32, i32]
+        L.vlab200_cross_attention.argtypes = [vp, i32, vp, vp, vp, i32, i32, vp, i32, vp, f32, vp, C.c_int64, vp]
+        L.vlab200_key_mass.argtypes = [vp, i32, vp, vp, vp, vp, i32, i32, vp, i32, vp, f32, f32, vp]
+        L.vlab200_kv_evict.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]
+        L.vlab200_qk_norm_rope_append.argtypes = [vp, i32, vp, vp]
         L.vlab200_engine_create.restype = C.c_void_p
         L.vlab200_engine_free.restype = None
         L.vlab200_prefill_create.restype = C.c_void_p
@@ -268,13 +275,13 @@ def _need(ok, what):
 def _need_tensor(t, name, dtype, shape, dev):
     """t is a contiguous tensor of this type and shape on cuda device `dev` (an index).  A call makes half a dozen of these checks, so the
     text of an error is put together only where there is one."""
-    import torch
-
-    if not isinstance(t, torch.Tensor):
-        raise VlaB200Error(ERR_ARG, f"{name}: a tensor is needed, not {type(t).__name__}")
-    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
-        raise VlaB200Error(ERR_ARG, f"{name}: a contiguous {dtype} tensor {tuple(shape)} on cuda:{dev} is needed, not {t.dtype} "
-                                    f"{tuple(t.shape)} (strides {t.stride()}) on {t.device}")
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+            return
+    except AttributeError:
+        raise VlaB200Error(ERR_ARG, f"{name}: a tensor is needed, not {type(t).__name__}") from None
+    raise VlaB200Error(ERR_ARG, f"{name}: a contiguous {dtype} tensor {tuple(shape)} on cuda:{dev} is needed, not {t.dtype} {tuple(t.shape)} "
+                                f"(strides {t.stride()}) on {t.device}")
 
 
 def _call_on(dev, fn, what, *args):
@@ -282,7 +289,7 @@ def _call_on(dev, fn, what, *args):
     import torch
 
     # the raw handle: making a Stream object of it took 3 us of a call's 16
-    stream = C.c_void_p(torch._C._cuda_getCurrentRawStream(dev))
+    stream = torch._C._cuda_getCurrentRawStream(dev)
     if torch.cuda.current_device() == dev:
         rc = fn(*args, stream)
     else:
@@ -304,7 +311,7 @@ def rope_freqs(rot_dim, base=10000.0, scaling="none", factor=1.0, original_len=0
     f, m = (C.c_double * (int(rot_dim) // 2))(), C.c_float()
     _check(lib().vlab200_rope_freqs(f, C.byref(m), int(rot_dim), C.c_double(base), ROPE_SCALING[scaling], C.c_double(factor),
                                     int(original_len)), "vlab200_rope_freqs")
-    return torch.tensor(list(f), dtype=torch.float64, device=device), m.value
+    return torch.frombuffer(bytearray(f), dtype=torch.float64).to(device), m.value
 
 
 class _QkNormRopeArgs(C.Structure):
@@ -404,10 +411,9 @@ def cross_attention(store, layer, q, lens=None, max_len=None, pad_ranges=None, s
             raise VlaB200Error(ERR_ARG, f"cross_attention: {n_q} query heads on {store.n_kv} kv heads, {S} tokens, {max_len} rows")
         if n > 0:
             ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
-    _call_on(dev, lib().vlab200_cross_attention, "vlab200_cross_attention", C.byref(store.c), layer, C.c_void_p(q.data_ptr()),
-             C.c_void_p(out.data_ptr()), C.c_void_p(lse.data_ptr()), S, n_q, C.c_void_p(lens.data_ptr()) if lens is not None else None, max_len,
-             C.c_void_p(pad_ranges.data_ptr()) if pad_ranges is not None else None, C.c_float(0.0 if scale is None else scale),
-             C.c_void_p(ws.data_ptr()) if ws is not None else None, C.c_int64(n))
+    _call_on(dev, lib().vlab200_cross_attention, "vlab200_cross_attention", C.byref(store.c), layer, q.data_ptr(), out.data_ptr(),
+             lse.data_ptr(), S, n_q, None if lens is None else lens.data_ptr(), max_len, None if pad_ranges is None else pad_ranges.data_ptr(),
+             0.0 if scale is None else scale, None if ws is None else ws.data_ptr(), n)
     return out, lse
 
 
@@ -429,11 +435,9 @@ def key_mass(store, layer, q, lse, lens=None, max_len=None, pad_ranges=None, sca
         out = torch.zeros(shape, dtype=torch.float32, device=q.device)
     else:
         _need_tensor(out, "out", torch.float32, shape, dev)
-    _call_on(dev, lib().vlab200_key_mass, "vlab200_key_mass", C.byref(store.c), layer, C.c_void_p(q.data_ptr()), C.c_void_p(lse.data_ptr()),
-             C.c_void_p(mass.data_ptr()) if mass is not None else None, C.c_void_p(out.data_ptr()), S, n_q,
-             C.c_void_p(lens.data_ptr()) if lens is not None else None, max_len,
-             C.c_void_p(pad_ranges.data_ptr()) if pad_ranges is not None else None, C.c_float(0.0 if scale is None else scale),
-             C.c_float(decay))
+    _call_on(dev, lib().vlab200_key_mass, "vlab200_key_mass", C.byref(store.c), layer, q.data_ptr(), lse.data_ptr(),
+             None if mass is None else mass.data_ptr(), out.data_ptr(), S, n_q, None if lens is None else lens.data_ptr(), max_len,
+             None if pad_ranges is None else pad_ranges.data_ptr(), 0.0 if scale is None else scale, decay)
     return out
 
 
@@ -467,9 +471,9 @@ def kv_evict(src, dst, mass, keep, lens=None, max_len=None, sink=0, recent=0, ma
         lens_out = torch.empty((src.n_obs,), dtype=torch.int32, device=src.k.device)
     else:
         _need_tensor(lens_out, "lens_out", torch.int32, (src.n_obs,), dev)
-    _call_on(dev, lib().vlab200_kv_evict, "vlab200_kv_evict", C.byref(src.c), C.byref(dst.c), C.c_void_p(mass.data_ptr()),
-             C.c_void_p(lens.data_ptr()) if lens is not None else None, src.cap if max_len is None else max_len, keep, sink, recent,
-             C.c_void_p(kept.data_ptr()), C.c_void_p(mass_out.data_ptr()), C.c_void_p(lens_out.data_ptr()))
+    _call_on(dev, lib().vlab200_kv_evict, "vlab200_kv_evict", C.byref(src.c), C.byref(dst.c), mass.data_ptr(),
+             None if lens is None else lens.data_ptr(), src.cap if max_len is None else max_len, keep, sink, recent, kept.data_ptr(),
+             mass_out.data_ptr(), lens_out.data_ptr())
     return lens_out, kept, mass_out
 
 

@@ -66,7 +66,7 @@ __device__ __forceinline__ float xa_max3(float a, float b, float c) {
 
 // The hidden range of an observation; (none, none) if it has none.
 __device__ __forceinline__ void xa_pad(const CrossParams &p, int obs, int &lo, int &hi) {
-    lo = p.pad ? p.pad[2 * obs] : 0;
+    lo = p.pad ? max(p.pad[2 * obs], 0) : 0;
     hi = p.pad ? p.pad[2 * obs + 1] : 0;
     if (hi <= lo) lo = hi = 0x7fffffff;
 }
@@ -1133,6 +1133,10 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
         vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 256 x 128 scores");
         return VLAB200_ERR_UNSUPPORTED;
     }
+    const long long q_b = items * R * hd * 2, pages_b = (long long)st->n_layers * items * st->cap * hd * 2;
+    const vb::MemRange written[] = {{out, q_b}, {lse, items * R * 4}, {ws, ws_bytes}};
+    const vb::MemRange read[] = {{q, q_b}, {st->k_pages, pages_b}, {st->v_pages, pages_b}, {lens, st->n_obs * 4LL}, {pad_ranges, st->n_obs * 8LL}};
+    if (vb::writes_overlap(written, 3, read, 5)) return VLAB200_ERR_ARG;
     const int n_sm = vb::sm_count();
     if (!n_sm) return vb::cuda_fail(cudaGetLastError(), "sm_count");
     const vb::CrossPlan plan = vb::cross_plan(hd, items, (int)R, max_len, n_sm);

@@ -84,6 +84,26 @@ static inline int launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 b
 // Asked of the driver once per (device, kernel, cluster).
 int max_active_clusters(const void *kernel, int threads, int smem, int cluster);
 
+// Device memory a call reads or writes; a null pointer or no bytes overlap nothing.
+struct MemRange {
+    const void *p;
+    long long bytes;
+};
+inline bool ranges_overlap(const MemRange &a, const MemRange &b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+// Does any of the n_out ranges that are written overlap one that is read, or another one that is written?
+inline bool writes_overlap(const MemRange *out, int n_out, const MemRange *in, int n_in) {
+    for (int o = 0; o < n_out; ++o) {
+        for (int i = 0; i < n_in; ++i)
+            if (ranges_overlap(out[o], in[i])) return true;
+        for (int q = 0; q < o; ++q)
+            if (ranges_overlap(out[o], out[q])) return true;
+    }
+    return false;
+}
+
 // Owning device allocation (move-only).
 struct DevBuf {
     void *p = nullptr;

@@ -364,6 +364,11 @@ extern "C" int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, c
         return VLAB200_ERR_UNSUPPORTED;
     }
     if (max_len == 0) return VLAB200_OK;
+    const long long q_b = (long long)st->n_obs * n_q * S * hd * 2, mass_b = (long long)st->n_obs * st->n_kv * st->cap * 4;
+    const vb::MemRange out[] = {{mass_out, mass_b}};
+    const vb::MemRange in[] = {{q, q_b}, {lse, (long long)st->n_obs * n_q * S * 4}, {st->k_pages, (long long)st->n_layers * mass_b / 4 * hd * 2},
+                               {lens, st->n_obs * 4LL}, {pad_ranges, st->n_obs * 8LL}, {mass_in == mass_out ? nullptr : mass_in, mass_b}};
+    if (vb::writes_overlap(out, 1, in, 6)) return VLAB200_ERR_ARG;
     vb::KeyMassParams p;
     p.lse = lse;
     p.mass_in = decay == 0.0f ? nullptr : mass_in;

@@ -256,24 +256,11 @@ extern "C" int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_k
         return VLAB200_ERR_UNSUPPORTED;
     }
     // rows are read while others are written: nothing that is written may overlap anything that is read, or one another
-    struct Range {
-        const void *p;
-        long long bytes;
-    };
     const long long src_b = pages * src->cap * hd * 2, dst_b = pages * dst->cap * hd * 2;
-    const Range in[4] = {{src->k_pages, src_b}, {src->v_pages, src_b}, {mass, pages * src->cap * 4}, {lens, lens ? src->n_obs * 4LL : 0}};
-    const Range out[5] = {{dst->k_pages, dst_b}, {dst->v_pages, dst_b}, {kept, pages * keep * 4}, {mass_out, mass_out ? pages * dst->cap * 4 : 0},
-                          {lens_out, lens_out ? src->n_obs * 4LL : 0}};
-    const auto overlap = [](const Range &a, const Range &b) {
-        const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-        return a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
-    };
-    for (int o = 0; o < 5; ++o) {
-        for (const Range &i : in)
-            if (overlap(out[o], i)) return VLAB200_ERR_ARG;
-        for (int q = 0; q < o; ++q)
-            if (overlap(out[o], out[q])) return VLAB200_ERR_ARG;
-    }
+    const vb::MemRange in[] = {{src->k_pages, src_b}, {src->v_pages, src_b}, {mass, pages * src->cap * 4}, {lens, src->n_obs * 4LL}};
+    const vb::MemRange out[] = {{dst->k_pages, dst_b}, {dst->v_pages, dst_b}, {kept, pages * keep * 4}, {mass_out, pages * dst->cap * 4},
+                                {lens_out, src->n_obs * 4LL}};
+    if (vb::writes_overlap(out, 5, in, 4)) return VLAB200_ERR_ARG;
     vb::EvictParams p;
     p.mass = mass;
     p.mass_out = mass_out;

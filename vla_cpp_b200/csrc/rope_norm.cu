@@ -474,6 +474,11 @@ int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, c
     vb::RopeNormParams p;
     const long long rows = (long long)st->n_obs * a->S;
     if (rows == 0) return VLAB200_OK;
+    const long long pages_b = a->with_kv ? (long long)st->n_layers * st->n_obs * st->n_kv * st->cap * hd * 2 : 0;
+    const vb::MemRange out[] = {{a->q_out, rows * a->n_q * hd * 2}, {st->k_pages, pages_b}, {st->v_pages, pages_b}};
+    const vb::MemRange in[] = {{a->x, ((rows - 1) * a->x_stride + n_heads * hd) * es}, {a->q_norm, hd * 4}, {a->k_norm, hd * 4},
+                               {a->freqs, a->rot_dim * 4LL}, {a->pos, rows * 4}, {a->row0, st->n_obs * 4LL}, {a->n_tok, st->n_obs * 4LL}};
+    if (vb::writes_overlap(out, 3, in, 7)) return VLAB200_ERR_ARG;
     if (rows > 0x7fffffffLL || (long long)a->S * hd > 0x7fffffffLL || n_heads > 2048 ||
         (long long)st->cap * hd > 0x7fffffffLL) {
         vb::set_last_error("qk_norm_rope_append: more than 2^31 - 1 rows or elements of a page, or 2,048 heads of a row");
