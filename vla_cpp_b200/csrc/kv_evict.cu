@@ -2,10 +2,10 @@
 // their order.  The first `sink` and the last `recent` rows of an observation stay in any case, then the rows of largest accumulated
 // attention weight (vlab200_key_mass), ties to the lower row.
 //
-// Two kernels.  The first finds the keep-th largest key of every page -- the weight's bits mapped so that they compare as whole numbers,
-// protected rows on top, no-numbers at the bottom -- and writes the kept rows' indices and weights in order: up to 1,024 rows a warp per
-// page, its keys in registers, bit by bit (1,152 pages of up to 816 rows: 5 us; a block per page and histograms 32); longer pages a block each,
-// 8 bits at a time from histograms.  The second copies K and V rows, 16 bytes per thread: all there is to move, HBM bounds it.
+// The keep-th largest key of a page decides -- the weight's bits mapped so that they compare as whole numbers, protected rows on top,
+// no-numbers at the bottom.  Pages of up to 1,024 rows: one kernel, a warp of every block finds it bit by bit with the keys in registers, then
+// the block copies its rows.  Longer pages: a block each finds it 8 bits at a time from histograms, a second kernel copies.  K and V rows go
+// 16 bytes per thread: all there is to move, HBM bounds it.
 #include "host_common.h"
 #include "tc5.cuh"
 
@@ -38,66 +38,98 @@ __device__ __forceinline__ uint32_t ev_key(const EvictParams &p, float mass, int
     return b & 0x80000000u ? ~b : b | 0x80000000u;  // in [2^23 - 1, 2^32 - 2^23]
 }
 
-// KPL keys per lane: pages of up to 32 KPL rows.
+// Rows [t0, n) of a page, every `stride`-th round of KE_THREADS / row_chunks rows, by the whole block; four rows of K and of V per thread in
+// flight (one of each: 5.0 TB/s of the 6.45 of a copy).
+__device__ __forceinline__ void ev_move(const EvictParams &p, long long page, const int32_t *rows, int n, int slice, int slices) {
+    constexpr int U = 4;
+    const int per = KE_THREADS / p.row_chunks, step = slices * per, col = threadIdx.x % p.row_chunks;
+    const long long from = page * p.src_cap * p.row_chunks + col, to = page * p.dst_cap * p.row_chunks + col;
+    for (int t = slice * per + threadIdx.x / p.row_chunks; t < n; t += U * step) {
+        int row[U];
+        uint4 a[U], b[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) row[i] = t + i * step < n ? rows[t + i * step] : -1;
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (row[i] >= 0) {
+                const long long src = from + (long long)row[i] * p.row_chunks;
+                a[i] = p.k[src];
+                b[i] = p.v[src];
+            }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (row[i] >= 0) {
+                const long long dst = to + (long long)(t + i * step) * p.row_chunks;
+                p.k_out[dst] = a[i];
+                p.v_out[dst] = b[i];
+            }
+    }
+}
+
+// KPL keys per lane: pages of up to 32 KPL rows.  Block (page, slice): its first warp selects, all of it moves its slice of the rows; what
+// other blocks move covers the selection.
 template <int KPL>
-__global__ void __launch_bounds__(128) kv_evict_select_warp_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(KE_THREADS) kv_evict_page_kernel(const EvictParams p) {
+    __shared__ int32_t s_rows[32 * KPL];
     pdl_launch_dependents();
     pdl_wait();
-    const long long page = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (page >= p.n_pages) return;
-    const int lane = threadIdx.x & 31;
+    const long long page = blockIdx.x;
     const int obs = (int)((unsigned)page / (unsigned)p.n_kv % (unsigned)p.n_obs);
     const int len = ev_len(p, obs), n = min(len, p.keep);
     const float *mass = p.mass + page * p.src_cap;
-    int32_t *kept = p.kept + page * p.keep;
-    float *mass_out = p.mass_out ? p.mass_out + page * p.dst_cap : nullptr;
-    if (p.lens_out && page < (long long)p.n_obs * p.n_kv && page % p.n_kv == 0 && lane == 0) p.lens_out[obs] = n;
-    float weight[KPL];
-    uint32_t key[KPL];
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        uint32_t key[KPL];
 #pragma unroll
-    for (int i = 0; i < KPL; ++i) weight[i] = i * 32 + lane < len ? mass[i * 32 + lane] : 0.0f;
+        for (int i = 0; i < KPL; ++i) {
+            const int r = i * 32 + lane;
+            key[i] = r < len ? __float_as_uint(mass[r]) : 0u;
+        }
 #pragma unroll
-    for (int i = 0; i < KPL; ++i) key[i] = i * 32 + lane < len ? ev_key(p, weight[i], i * 32 + lane, len) : 0u;
-    // the largest threshold that at least n keys reach; n keys that reach it exactly will do
-    uint32_t limit = 0;
-    if (len > n && n > 0) {
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t cand = limit | 1u << bit;
-            int part[4] = {0, 0, 0, 0};
+        for (int i = 0; i < KPL; ++i) {
+            const int r = i * 32 + lane;
+            key[i] = r < len ? ev_key(p, __uint_as_float(key[i]), r, len) : 0u;
+        }
+        // the largest threshold that at least n keys reach; n keys that reach it exactly will do
+        uint32_t limit = 0;
+        int left = n;  // rows at the threshold that are kept: the first ones
+        if (len > n && n > 0) {
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t cand = limit | 1u << bit;
+                int part[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < KPL; ++i) part[i & 3] += key[i] >= cand ? 1 : 0;
-            const int c = __reduce_add_sync(0xffffffffu, (part[0] + part[1]) + (part[2] + part[3]));
-            if (c >= n) limit = cand;
-            if (c == n) break;
+                for (int i = 0; i < KPL; ++i) part[i & 3] += key[i] >= cand ? 1 : 0;
+                const int c = __reduce_add_sync(0xffffffffu, (part[0] + part[1]) + (part[2] + part[3]));
+                if (c >= n) limit = cand;
+                if (c == n) break;
+            }
+            int above = 0;
+#pragma unroll
+            for (int i = 0; i < KPL; ++i) above += key[i] > limit ? 1 : 0;
+            left = n - __reduce_add_sync(0xffffffffu, above);
+        }
+        const unsigned before = (1u << lane) - 1u;
+        int done = 0, equals = 0;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            const int r = i * 32 + lane;
+            const bool above = r < len && (len <= n || key[i] > limit), equal = r < len && len > n && key[i] == limit;
+            const unsigned eq = __ballot_sync(0xffffffffu, equal);
+            const bool take = above || (equal && equals + __popc(eq & before) < left);
+            const unsigned tk = __ballot_sync(0xffffffffu, take);
+            if (take) s_rows[done + __popc(tk & before)] = r;
+            done += __popc(tk);
+            equals += __popc(eq);
         }
     }
-    int left = n;  // rows at the threshold that are kept: the first ones
-    if (len > n) {
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < KPL; ++i) c += key[i] > limit ? 1 : 0;
-        left = n - __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if (blockIdx.y == 0) {
+        if (p.lens_out && page < (long long)p.n_obs * p.n_kv && page % p.n_kv == 0 && threadIdx.x == 0) p.lens_out[obs] = n;
+        for (int i = threadIdx.x; i < p.keep; i += KE_THREADS) p.kept[page * p.keep + i] = i < n ? s_rows[i] : -1;
+        if (p.mass_out)
+            for (int i = threadIdx.x; i < p.dst_cap; i += KE_THREADS) p.mass_out[page * p.dst_cap + i] = i < n ? mass[s_rows[i]] : 0.0f;
     }
-    const unsigned before = (1u << lane) - 1u;
-    int done = 0, equals = 0;
-#pragma unroll
-    for (int i = 0; i < KPL; ++i) {
-        const int r = i * 32 + lane;
-        const bool above = r < len && (len <= n || key[i] > limit), equal = r < len && len > n && key[i] == limit;
-        const unsigned eq = __ballot_sync(0xffffffffu, equal);
-        const bool take = above || (equal && equals + __popc(eq & before) < left);
-        const unsigned tk = __ballot_sync(0xffffffffu, take);
-        if (take) {
-            const int at = done + __popc(tk & before);
-            kept[at] = r;
-            if (mass_out) mass_out[at] = weight[i];
-        }
-        done += __popc(tk);
-        equals += __popc(eq);
-    }
-    for (int i = n + lane; i < p.keep; i += 32) kept[i] = -1;
-    if (mass_out)
-        for (int i = n + lane; i < p.dst_cap; i += 32) mass_out[i] = 0.0f;
+    ev_move(p, page, s_rows, n, blockIdx.y, gridDim.y);
 }
 
 __global__ void __launch_bounds__(KE_THREADS) kv_evict_select_kernel(const EvictParams p) {
@@ -204,36 +236,9 @@ __global__ void __launch_bounds__(KE_THREADS) kv_evict_select_kernel(const Evict
 __global__ void __launch_bounds__(KE_THREADS) kv_evict_move_kernel(const EvictParams p) {
     pdl_launch_dependents();
     pdl_wait();
-    const int per = KE_THREADS / p.row_chunks;  // rows a block moves at a time
     const long long page = blockIdx.x;
     const int obs = (int)((unsigned)page / (unsigned)p.n_kv % (unsigned)p.n_obs);
-    const int n = min(ev_len(p, obs), p.keep);
-    const int32_t *kept = p.kept + page * p.keep;
-    const long long from = page * p.src_cap * p.row_chunks, to = page * p.dst_cap * p.row_chunks;
-    const int col = threadIdx.x % p.row_chunks;
-    // four rows of K and of V per thread in flight (one of each: 5.0 TB/s of the 6.45 of a copy)
-    constexpr int U = 4;
-    const int step = gridDim.y * per;
-    for (int t = blockIdx.y * per + threadIdx.x / p.row_chunks; t < n; t += U * step) {
-        int row[U];
-        uint4 a[U], b[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) row[i] = t + i * step < n ? kept[t + i * step] : -1;
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (row[i] >= 0) {
-                const long long src = from + (long long)row[i] * p.row_chunks + col;
-                a[i] = p.k[src];
-                b[i] = p.v[src];
-            }
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-            if (row[i] >= 0) {
-                const long long dst = to + (long long)(t + i * step) * p.row_chunks + col;
-                p.k_out[dst] = a[i];
-                p.v_out[dst] = b[i];
-            }
-    }
+    ev_move(p, page, p.kept + page * p.keep, min(ev_len(p, obs), p.keep), blockIdx.y, gridDim.y);
 }
 
 }  // namespace vb
@@ -284,15 +289,14 @@ extern "C" int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_k
     const int n_sm = vb::sm_count();
     if (!n_sm) return vb::cuda_fail(cudaGetLastError(), "sm_count");
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    const dim3 warp_grid((unsigned)((pages + 3) / 4));
-    const int rc = max_len <= 256    ? vb::launch_pdl(vb::kv_evict_select_warp_kernel<8>, warp_grid, dim3(128), 0, cs, p)
-                   : max_len <= 512  ? vb::launch_pdl(vb::kv_evict_select_warp_kernel<16>, warp_grid, dim3(128), 0, cs, p)
-                   : max_len <= 1024 ? vb::launch_pdl(vb::kv_evict_select_warp_kernel<32>, warp_grid, dim3(128), 0, cs, p)
-                                     : vb::launch_pdl(vb::kv_evict_select_kernel, dim3((unsigned)pages), dim3(vb::KE_THREADS), 0, cs, p);
-    if (rc) return rc;
     // enough blocks for eight on every SM, none with less than a round of rows
     const int rounds = (keep + vb::KE_THREADS / p.row_chunks - 1) / (vb::KE_THREADS / p.row_chunks);
     long long slices = (8LL * n_sm + pages - 1) / pages;
     if (slices > rounds) slices = rounds;
-    return vb::launch_pdl(vb::kv_evict_move_kernel, dim3((unsigned)pages, (unsigned)slices), dim3(vb::KE_THREADS), 0, cs, p);
+    const dim3 grid((unsigned)pages, (unsigned)slices), block(vb::KE_THREADS);
+    if (max_len <= 256) return vb::launch_pdl(vb::kv_evict_page_kernel<8>, grid, block, 0, cs, p);
+    if (max_len <= 512) return vb::launch_pdl(vb::kv_evict_page_kernel<16>, grid, block, 0, cs, p);
+    if (max_len <= 1024) return vb::launch_pdl(vb::kv_evict_page_kernel<32>, grid, block, 0, cs, p);
+    if (int rc = vb::launch_pdl(vb::kv_evict_select_kernel, dim3((unsigned)pages), block, 0, cs, p)) return rc;
+    return vb::launch_pdl(vb::kv_evict_move_kernel, grid, block, 0, cs, p);
 }
