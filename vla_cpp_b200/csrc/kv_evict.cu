@@ -289,9 +289,9 @@ extern "C" int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_k
     const int n_sm = vb::sm_count();
     if (!n_sm) return vb::cuda_fail(cudaGetLastError(), "sm_count");
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    // enough blocks for eight on every SM, none with less than a round of rows
+    // enough blocks for four on every SM, none with less than a round of rows
     const int rounds = (keep + vb::KE_THREADS / p.row_chunks - 1) / (vb::KE_THREADS / p.row_chunks);
-    long long slices = (8LL * n_sm + pages - 1) / pages;
+    long long slices = (4LL * n_sm + pages - 1) / pages;
     if (slices > rounds) slices = rounds;
     const dim3 grid((unsigned)pages, (unsigned)slices), block(vb::KE_THREADS);
     if (max_len <= 256) return vb::launch_pdl(vb::kv_evict_page_kernel<8>, grid, block, 0, cs, p);
