@@ -42,6 +42,7 @@ struct CrossParams {
     int S, n_q, n_kv, g, R, n_obs, max_len, page0;
     int n_mt, unit_rows; // units per item and their rows
     int n_work;          // CTAs (CTA pairs) the blocks are dealt to
+    int by_unit;         // cross_combine_kernel: a block per unit (and rows), not per CTA
     int out_al32;
     float scale_log2;
     int *status;
@@ -820,11 +821,16 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 else mbar_arrive_cluster(bar, 0);
             }
         };
+        auto is_live = [&](const XaSegment &sg) { return sg.mt * 256 + (int)rank * 128 + qtr * 32 < p.R; };  // has the warp rows
         // segment `u` is complete: O / l -> bf16 -> out, or the piece into the workspace
         auto drain = [&](uint32_t u, const XaSegment &sg, float m, float l_mine) -> bool {
-            xch[512 + half * 128 + my_slot] = l_mine;
             if (!warp_wait(o_done, u & 1u, wc, DEV_TIMEOUT_ACCUM)) return false;
             tc_fence_after();
+            if (!is_live(sg)) {
+                arrive_even(o_free);
+                return true;
+            }
+            xch[512 + half * 128 + my_slot] = l_mine;
             if (!pair_sync()) return false;
             const float l = l_mine + xch[512 + (half ^ 1) * 128 + my_slot];
             const int row = sg.mt * 256 + lr;
@@ -865,6 +871,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         float prev_m = 0.0f, prev_l = 0.0f;
         for (; ok && work.next(s); ++si) {
             const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
+            const bool live = is_live(s);
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units (the same in both halves), this half's part of the row sum
             for (int j = s.j0; j < s.j1; ++j, ++jb) {
                 const uint32_t sb = jb % NS;
@@ -872,6 +879,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 ok = warp_wait(&s_full[sb], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
                 if (!ok) break;
                 tc_fence_after();
+                if (live) {
                 uint32_t x[2][32];
                 tmem_ld32(s_addr + (uint32_t)(half * 64), x[0]);
                 tmem_ld32(s_addr + (uint32_t)(half * 64 + 32), x[1]);
@@ -937,6 +945,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 // P (128 rows of V, bf16) over the first 64 columns of S; both halves have read theirs: they met
                 tmem_st32(s_addr + (uint32_t)(half * 32), pk);
                 tmem_st_wait();
+                }
                 tc_fence_before();
                 arrive_even(&p_full[sb]);
                 if (j == s.j0 && si > 0) {
@@ -961,27 +970,48 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
 }
 
 // Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Block x
-// looks after the unit that CTA x began and did not finish.  TEAM warps share a row: 1 where a unit's rows are many (two pieces or three of each), 8 where they are few and the
-// pieces as many as there are CTAs (one token over 16,001 rows, a warp per row: 40 us).
+// looks after unit x, or, where there are more units than CTAs, after the one that CTA x began and did not finish.  TEAM warps share a row: 1 where a unit's rows are many (two pieces or three of each), 32 where they are few
+// and the pieces as many as there are CTAs (one token over 16,001 rows, a warp per row: 40 us).
 template <int HD, int TEAM>
-__global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p) {
-    __shared__ __align__(8) float s_o[8][TEAM > 1 ? HD : 1], s_l[8], s_m[8];
+__global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kernel(const CrossParams p) {
+    constexpr int WARPS = TEAM > 1 ? TEAM : 8;
+    __shared__ __align__(8) float s_o[WARPS][TEAM > 1 ? HD : 1], s_l[WARPS], s_m[WARPS];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c0 = blockIdx.x, total = xa_total_blocks(p), n = min(p.n_work, total);
-    if (c0 >= n) return;
-    const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
-    auto len_of = [&](int obs) { return xa_len(p, obs); };
-    RaggedCursor cur(len_of, p.n_obs, p.n_kv * p.n_mt, XA_BKV);
-    RaggedUnit u;
-    if (!cur.find(end - 1, u)) return;
-    const int nb = (u.len + XA_BKV - 1) / XA_BKV, first = end - 1 - u.block;  // of the unit of the CTA's last block
-    if (first < begin || first + nb <= end) return;                         // begun before this CTA, or whole
-    const int c1 = (int)(((long long)(first + nb) * n - 1) / total);        // the CTA that has the unit's last block
-    const int kvh = u.kvh / p.n_mt, row0 = (u.kvh - kvh * p.n_mt) * p.unit_rows, rows = min(p.R - row0, p.unit_rows);
+    const int total = xa_total_blocks(p), n = min(p.n_work, total), upo = p.n_kv * p.n_mt;  // units of an observation
+    if (total == 0) return;
+    int obs, u, nb, first, c0;  // the unit's observation, place in it and blocks; its first block in the list, the CTA that has that one
+    if (p.by_unit) {
+        obs = blockIdx.x / upo;
+        u = blockIdx.x - obs * upo;
+        nb = (xa_len(p, obs) + XA_BKV - 1) / XA_BKV;
+        if (nb == 0) return;
+        int before = 0;
+        for (int i = lane; i < obs; i += 32) before += (xa_len(p, i) + XA_BKV - 1) / XA_BKV;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+        first = before * upo + u * nb;
+        c0 = (int)(((long long)(first + 1) * n - 1) / total);
+    } else {
+        c0 = blockIdx.x;
+        if (c0 >= n) return;
+        const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
+        auto len_of = [&](int i) { return xa_len(p, i); };
+        RaggedCursor cur(len_of, p.n_obs, upo, XA_BKV);
+        RaggedUnit at;
+        if (!cur.find(end - 1, at)) return;
+        obs = at.obs;
+        u = at.kvh;
+        nb = (at.len + XA_BKV - 1) / XA_BKV;
+        first = end - 1 - at.block;
+        if (first < begin) return;  // begun before this CTA
+    }
+    const int c1 = (int)(((long long)(first + nb) * n - 1) / total);  // the CTA that has the unit's last block
+    if (c0 == c1) return;                                              // whole
+    const int kvh = u / p.n_mt, row0 = (u - kvh * p.n_mt) * p.unit_rows, rows = min(p.R - row0, p.unit_rows);
     constexpr int NV = HD / 64;  // pairs of columns per lane
-    for (int r0 = blockIdx.y * (8 / TEAM); r0 < rows; r0 += gridDim.y * (8 / TEAM)) {
+    for (int r0 = blockIdx.y * (WARPS / TEAM); r0 < rows; r0 += gridDim.y * (WARPS / TEAM)) {
         const int lr = r0 + warp / TEAM, member = warp % TEAM;
         if (TEAM == 1 && lr >= rows) return;
         auto slot_of = [&](int c) { return (long long)(2 * c + (c == c0 ? 1 : 0)) * p.ws_rows + lr; };
@@ -1017,7 +1047,7 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
             }
         }
         const int row = row0 + lr, head = kvh * p.g + row / p.S, tok = row % p.S;
-        __nv_bfloat16 *dst = p.out + (((long long)u.obs * p.S + tok) * p.n_q + head) * HD;
+        __nv_bfloat16 *dst = p.out + (((long long)obs * p.S + tok) * p.n_q + head) * HD;
         if (TEAM > 1) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) reinterpret_cast<float2 *>(s_o[warp])[k * 32 + lane] = acc[k];
@@ -1029,17 +1059,17 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
             l = 0.0f;
 #pragma unroll
             for (int w = 0; w < TEAM; ++w) M = fmaxf(M, s_m[w]);
-            float scale[TEAM];
+            float o = 0.0f;
+            const int col = threadIdx.x < HD ? threadIdx.x : 0;
 #pragma unroll
             for (int w = 0; w < TEAM; ++w) {
-                scale[w] = s_m[w] == -INFINITY ? 0.0f : xa_ex2(s_m[w] - M);
-                l = fmaf(s_l[w], scale[w], l);
+                const float scale = s_m[w] == -INFINITY ? 0.0f : xa_ex2(s_m[w] - M);
+                l = fmaf(s_l[w], scale, l);
+                o = fmaf(s_o[w][col], scale, o);
             }
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            for (int i = threadIdx.x; i < HD; i += 256) {
-                float o = 0.0f;
-#pragma unroll
-                for (int w = 0; w < TEAM; ++w) o = fmaf(s_o[w][i], scale[w], o);
+            if (threadIdx.x < HD) {
+                const int i = col;
                 dst[i] = __float2bfloat16_rn(o * inv);
             }
             __syncthreads();
@@ -1050,15 +1080,17 @@ __global__ void __launch_bounds__(256) cross_combine_kernel(const CrossParams p)
                 reinterpret_cast<__nv_bfloat162 *>(dst)[k * 32 + lane] = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv);
         }
         if (p.lse && lane == 0 && member == 0)
-            p.lse[((long long)u.obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+            p.lse[((long long)obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
     }
 }
 
 template <int HD>
-static int launch_combine(const CrossParams &p, cudaStream_t stream) {
-    const unsigned gx = (unsigned)p.n_work;
+static int launch_combine(CrossParams p, cudaStream_t stream) {
+    const int units = p.n_obs * p.n_kv * p.n_mt;
+    p.by_unit = units <= p.n_work ? 1 : 0;
+    const unsigned gx = (unsigned)(p.by_unit ? units : p.n_work);
     if (p.ws_rows <= 64)  // a row per block
-        return launch_pdl(cross_combine_kernel<HD, 8>, dim3(gx, (unsigned)p.ws_rows), dim3(256), 0, stream, p);
+        return launch_pdl(cross_combine_kernel<HD, 32>, dim3(gx, (unsigned)p.ws_rows), dim3(1024), 0, stream, p);
     return launch_pdl(cross_combine_kernel<HD, 1>, dim3(gx, 8), dim3(256), 0, stream, p);  // 32 rows per block
 }
 
