@@ -15,9 +15,15 @@
 // 1,024 clocks per tile and block at heads of 128; at 64 the exponentials bound it.  Blocks of 64 rows with two S buffers per tile were
 // slower: a product whose A comes from shared memory takes 64 clocks a step of 16 whether N is 64 or 128.
 //
-// Work is dealt out in blocks, not units: the units' blocks form one list and every CTA takes an equal piece of it, so neither ragged
-// lengths nor few units leave SMs idle.  A unit cut by a piece's border leaves un-normalised rows with their maximum and sum in the
-// workspace, at most two per CTA, and cross_combine_kernel merges them in order.  Without a workspace borders move to whole units.
+// Work is dealt out in one of two ways (cross_plan says which).  Whole: a CTA takes whole units, the longest observations first.  Cut: the
+// units' blocks form one list and every CTA takes an equal piece of it, so few units leave no SM idle; a unit cut by a piece's border
+// leaves un-normalised rows with their maximum and sum in the workspace, at most two pieces per CTA, and cross_combine_kernel merges them
+// in order.
+//
+// Measured (cold L2): 4 prompts of 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 rows 207 us = 991 TFLOP/s; there the chain of a
+// tile's block -- S, softmax, P V, some 3,500 clocks -- bounds it, of which the pipe computes 2,048 for the two tiles.  64 x 50 tokens, 15 / 5
+// heads of 64, over 113 to 241 rows 29 us, and 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 rows 37 us: a unit's fixed chain of
+// loads, first S, last P V and store, some 5 us, bounds those.
 #include <cuda_bf16.h>
 
 #include "f32x2.cuh"
@@ -969,9 +975,10 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     }
 }
 
-// Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Block x
-// looks after unit x, or, where there are more units than CTAs, after the one that CTA x began and did not finish.  TEAM warps share a row: 1 where a unit's rows are many (two pieces or three of each), 32 where they are few
-// and the pieces as many as there are CTAs (one token over 16,001 rows, a warp per row: 40 us).
+// Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Block x looks after unit x,
+// or, where there are more units than CTAs, after the one that CTA x began and did not finish.  TEAM warps share a row: 1 where a unit's rows
+// are many (two pieces or three of each), 32 where they are few and the pieces as many as there are CTAs (one token, 8 / 1 heads of 256,
+// over 16,001 rows, the whole call: 43 us with a warp per row, 24 so, 21 with the pages in L2).
 template <int HD, int TEAM>
 __global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kernel(const CrossParams p) {
     constexpr int WARPS = TEAM > 1 ? TEAM : 8;
@@ -1106,7 +1113,9 @@ static CrossPlan cross_plan(int hd, long long items, int R, int max_len, int n_s
     c.n_work = hd == 256 ? n_sm / 2 : n_sm;
     c.ws_rows = R < 256 ? R : 256;
     // Whole units take rounds of n_work; cut ones fill the last round, for the pieces' way through the workspace and a second kernel: the
-    // time of some 6 blocks, and of 10 more where the pieces are full tiles.
+    // time of some 6 blocks, and of 10 more where the pieces are full tiles.  Cut / whole, us: one token of 8 / 1 heads of 256 over 16,001
+    // rows 21 / 176; 4 x 816 tokens of 20 / 5 heads of 128 over 4,097 to 8,190 rows 221 / 207; 64 x 51 tokens of 8 / 1 heads of 256 over
+    // 304 to 816 rows 55 / 37; 64 x 50 tokens of 15 / 5 heads of 64 over 113 to 241 rows 45 / 31.
     const long long units = items * c.n_mt, nb = (max_len + XA_BKV - 1) / XA_BKV, rounds = (units + c.n_work - 1) / c.n_work;
     const bool cut = (rounds * c.n_work - units) * nb > (6LL + 10LL * c.ws_rows / 256) * c.n_work;
     c.ws_bytes = cut ? 2LL * c.n_work * c.ws_rows * (hd + 2) * 4 : 0;

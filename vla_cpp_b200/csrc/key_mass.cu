@@ -14,7 +14,10 @@
 //                    accumulators; odd CTA: tells the even one what has landed
 //   16 sum warps     four per lane quarter, 128 columns of every second (heads of 256: fourth) chunk each: p = 2^(s c - lse')
 //
-// One query token: K streams once, HBM bounds it.  Many: the exponentials (heads of 64 and 128) or the product (256).
+// One query token: K streams once, HBM bounds it.  Many: the exponentials (16 per clock and SM) at heads of 64 and 128, at 256 their sum
+// with the product's chain.  Measured (cold L2): 4 x 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 keys 145 us, 90 of them the
+// exponential unit's (a polynomial on the FMA pipe for every fourth or eighth of them was slower: the sum warps' issue slots are full);
+// 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 keys 27 us; one token over 16,001 keys 18 us, 13 with the pages in L2.
 #include <cuda_bf16.h>
 
 #include "f32x2.cuh"

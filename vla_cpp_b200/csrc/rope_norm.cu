@@ -6,10 +6,15 @@
 //                                                 interleaved: u, v = 2 i, 2 i + 1;  columns from r on stay
 //   one rounding to bf16; V is rounded only.
 //
-// The op reads and writes every element once and does some ten operations on it: HBM bounds it.  A warp takes a token and walks its
-// heads, 16 columns per lane, so the token's cosines and sines stay in registers (every lane computes r / 64 of them, they
-// are exchanged through shared memory once per token).  In the half layout a lane holds columns 8 j .. 8 j + 7 and their partners r / 2
-// further on, so the rotation needs no exchange.  Few tokens: a token's heads are dealt over several warps.
+// The op reads and writes every element once and does some ten operations on it.  A warp takes a token and walks its heads, 16 columns
+// per lane, so the products of norm weights with the token's cosines and sines stay in registers from head to head (the warp computes
+// the token's r / 2 of each once and exchanges them through shared memory).  In the half layout a lane holds columns 8 j .. 8 j + 7 and
+// their partners r / 2 further on, so the rotation needs no exchange.  Few tokens: a token's heads are dealt over several warps.
+//
+// Measured (cold L2): 33 prefixes of 306 to 816 tokens, 8 + 2 heads of 256 in bf16, 53 us = 4.2 TB/s of the 6.45 of a copy.  The rate at
+// which instructions issue bounds it, addresses about half of them: a table of the heads' places instead of arithmetic per step 59 -> 53 us,
+// rows straight to shared memory instead of through registers no change.  64 x 51 tokens of 15 + 10 heads of 64 in float32 interleaved
+// 17 us (launch and one wave), one token 7 us.
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -175,8 +180,8 @@ __global__ void __launch_bounds__(RN_WARPS * 32, 2) qk_norm_rope_kernel(const Ro
     tok.t = (int)(tok.m - (unsigned)tok.obs * (unsigned)p.S);
     tok.exists = tok.m < p.M;
     fetch(tok);
-    // The loads run DEPTH steps ahead through all of the warp's live tokens, each lane's own 2 x 8 columns straight to shared memory:
-    // in registers they left room for two steps (32 KB per SM in flight, a copy alone 47 us for 224 MB).
+    // The loads run DEPTH steps ahead through all of the warp's live tokens, each lane's own 2 x 8 columns straight to shared memory, so that
+    // no step waits for them at a token's border either.
     RnToken ld = tok;
     const int my_steps = (n_steps - part + p.parts - 1) / p.parts;
     const RnStep *const my_step0 = steps + part * HPW + lh;
