@@ -11,10 +11,11 @@
 // the token's r / 2 of each once and exchanges them through shared memory).  In the half layout a lane holds columns 8 j .. 8 j + 7 and
 // their partners r / 2 further on, so the rotation needs no exchange.  Few tokens: a token's heads are dealt over several warps.
 //
-// Measured (cold L2): 33 prefixes of 306 to 816 tokens, 8 + 2 heads of 256 in bf16, 53 us = 4.2 TB/s of the 6.45 of a copy.  The rate at
-// which instructions issue bounds it, addresses about half of them: a table of the heads' places instead of arithmetic per step 59 -> 53 us,
-// rows straight to shared memory instead of through registers no change.  64 x 51 tokens of 15 + 10 heads of 64 in float32 interleaved
-// 17 us (launch and one wave), one token 7 us.
+// Measured (cold L2): 33 prefixes of 306 to 816 tokens, 8 + 2 heads of 256 in bf16, 53 us = 4.2 TB/s of the 6.45 of a copy (an elementwise
+// kernel of torch moves as many bytes in 41).  Loads and stores alone take 47 us, arithmetic alone 40: 16 warps of 128 registers issue half
+// of the time and hide neither wholly.  A table of the heads' places instead of arithmetic per step 59 -> 53; no change from rows straight to
+// shared memory instead of through registers, nor from equal numbers of live tokens per warp; slower: 24 warps of 80 registers (57), two steps
+// at a time (56); whole rows by bulk copies of a loader warp 51, but 64 x 51 tokens of 15 + 10 heads of 64 in float32 22 instead of 17.
 #include <cuda_bf16.h>
 
 #include <cmath>
