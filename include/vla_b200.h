@@ -218,9 +218,9 @@ VLAB200_API int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int3
  * q: bf16 [n_obs][n_q][S][hd]; out: bf16 [n_obs][S][n_q*hd]; lse: float32 [n_obs][n_q][S] or NULL.  lens: int32 [n_obs], taken into
  * [0, max_len], or NULL (max_len for all); 0 <= max_len <= cap bounds the rows that may be read.  scale 0 = 1 / sqrt(hd).
  * ws: device memory of vlab200_cross_attention_ws_bytes() (32-byte aligned, nothing kept between calls, not shared by calls whose
- * kernels may overlap) lets the blocks of a call be dealt to the SMs evenly where that pays (0 bytes: it does not); NULL: units of 256 query rows
- * stay whole.  Results are the same from
- * run to run for the same lengths, and agree to rounding between the two.  The head widths are 64, 128 and 256.
+ * kernels may overlap) lets the blocks of a call be dealt to the SMs evenly where that pays (0 bytes: it does not); NULL: units of 256
+ * query rows stay whole.  Results are the same from run to run for the same lengths, and agree to rounding between the two.  The head
+ * widths are 64, 128 and 256.
  * Stands beside vlab200_attention, which has one key range for all observations (src/models/smolvla.cpp:870-881 are the reference's cross
  * layers). */
 VLAB200_API int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q,
