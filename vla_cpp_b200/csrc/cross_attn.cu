@@ -48,6 +48,7 @@ struct CrossParams {
     int S, n_q, n_kv, g, R, n_obs, max_len, page0;
     int n_mt, unit_rows; // units per item and their rows
     int n_work;          // CTAs (CTA pairs) the blocks are dealt to
+    int round_r, round_u, bin_shift;  // n_work in observations and units; see XaOrder
     int by_unit;         // cross_combine_kernel: a block per unit (and rows), not per CTA
     int out_al32;
     float scale_log2;
@@ -71,6 +72,11 @@ __device__ __forceinline__ float xa_max3(float a, float b, float c) {
     return d;
 }
 
+// A row of an item (g heads of S tokens): token * n_q + head.
+__device__ __forceinline__ int xa_place(const CrossParams &p, int row) {
+    const int head = row / p.S;
+    return (row - head * p.S) * p.n_q + head;
+}
 // The hidden range of an observation; (none, none) if it has none.
 __device__ __forceinline__ void xa_pad(const CrossParams &p, int obs, int &lo, int &hi) {
     lo = p.pad ? max(p.pad[2 * obs], 0) : 0;
@@ -92,77 +98,128 @@ struct XaSegment {  // a run of blocks [j0, j1) of one unit
     int pad_lo, pad_hi;                   // hidden rows
 };
 
-// Whole units of up to XA_SORT observations: longest observations first, dealt to the CTAs there and back, so that who has a long one first
+// Whole units of up to XA_SORT observations: those with most blocks first, dealt to the CTAs there and back, so that who has a long one first
 // has a short one next (64 observations of 3 to 7 blocks, two units each, on 74 pairs: 14 blocks for some pairs in the order of the
-// observations, 9 so; 8.5 on average).
-constexpr int XA_SORT = 256;
+// observations, 9 so; 8.5 on average).  Every CTA sorts for itself (a counting sort, the same in all of them): a bin per number of blocks, or
+// per 2^bin_shift of them, and the last for observations without rows.
+constexpr int XA_SORT = 256, XA_BINS = 64;
 struct XaOrder {
-    int len[XA_SORT], pad_lo[XA_SORT], pad_hi[XA_SORT];  // by observation
-    int obs[XA_SORT];                                    // by rank
-    int n_live;        // observations that have rows
+    int4 item[XA_SORT];                // observation, length, hidden range
+    int count[XA_SORT / 32][XA_BINS];  // by the warp that read them
+    int n_live;                        // observations that have rows
 };
-__device__ __forceinline__ void xa_sort(const CrossParams &p, XaOrder &o, int n_threads) {  // the whole block
-    if (p.ws_o != nullptr || p.n_obs > XA_SORT) return;
-    for (int i = threadIdx.x; i < p.n_obs; i += n_threads) {
-        o.len[i] = xa_len(p, i);
-        xa_pad(p, i, o.pad_lo[i], o.pad_hi[i]);
-    }
-    if (threadIdx.x == 0) o.n_live = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.n_obs; i += n_threads) {
-        const int mine = o.len[i];
-        int rank = 0;
-        for (int k = 0; k < p.n_obs; ++k) {
-            const int other = o.len[k];
-            rank += other > mine || (other == mine && k < i) ? 1 : 0;
+__device__ __forceinline__ void xa_sort_clear(XaOrder &o, int n_threads) {  // a barrier of the block later: xa_sort
+    for (int i = threadIdx.x; i < XA_SORT / 32 * XA_BINS; i += n_threads) (&o.count[0][0])[i] = 0;
+}
+__device__ __forceinline__ void xa_sort(const CrossParams &p, XaOrder &o) {  // the whole block: XA_SORT threads or more
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (p.n_obs + 31) >> 5;
+    int4 mine = make_int4((int)threadIdx.x, 0, 0, 0);
+    int bin = XA_BINS, rank = 0;  // (lanes without an observation share a bin that is not counted)
+    if (warp < warps) {
+        if ((int)threadIdx.x < p.n_obs) {
+            mine.y = xa_len(p, mine.x);
+            xa_pad(p, mine.x, mine.z, mine.w);
+            const int most = (p.max_len + XA_BKV - 1) / XA_BKV >> p.bin_shift;
+            bin = mine.y > 0 ? most - ((mine.y + XA_BKV - 1) / XA_BKV >> p.bin_shift) : XA_BINS - 1;
         }
-        o.obs[rank] = i;
-        if (mine > 0) atomicAdd(&o.n_live, 1);
+        const unsigned same = __match_any_sync(0xffffffffu, bin);
+        rank = __popc(same & ((1u << lane) - 1u));
+        if (bin < XA_BINS && rank == 0) o.count[warp][bin] = __popc(same);
+    }
+    __syncthreads();
+    if (warp < warps) {
+        int sum[2] = {0, 0}, before[2] = {0, 0};  // of this lane's two bins: all of them, those of the warps in front
+        for (int w = 0; w < warps; ++w) {
+            const int2 c = *reinterpret_cast<const int2 *>(&o.count[w][2 * lane]);
+            if (w == warp) {
+                before[0] = sum[0];
+                before[1] = sum[1];
+            }
+            sum[0] += c.x;
+            sum[1] += c.y;
+        }
+        int incl = sum[0] + sum[1];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += up;
+        }
+        const int at0 = incl - sum[0] - sum[1] + before[0], at1 = incl - sum[1] + before[1];
+        const int even = __shfl_sync(0xffffffffu, at0, bin >> 1), odd = __shfl_sync(0xffffffffu, at1, bin >> 1);
+        if (bin < XA_BINS) o.item[(bin & 1 ? odd : even) + rank] = mine;
+        if (warp == 0 && lane == 31) o.n_live = p.n_obs - sum[1];
     }
     __syncthreads();
 }
 
+// The segments of a CTA (pair): whole units in the order above, or (LIST) a piece of the list of all blocks.
+template <bool LIST, typename LenOf>
+struct XaWork;
 template <typename LenOf>
-struct XaWork {
-    RaggedCursor<LenOf> cur;
+struct XaWork<false, LenOf> {
     const XaOrder &order;
     const CrossParams &p;
-    int w, w1, c, n_mt, n_kv, n_work;  // sorted: w is the round, w1 the number of units
-    bool whole_units, sorted;
-    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, const XaOrder &o, int cta)
-        : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV, p.ws_o != nullptr || p.n_obs > XA_SORT), order(o), p(p) {
+    int upo, live;           // units of an observation, observations
+    int my_r, my_u;          // place of this CTA in a round, counted in observations and units
+    int base_r, base_u;      // of the round
+    bool back;
+    __device__ __forceinline__ XaWork(LenOf, const CrossParams &p, const XaOrder &o, int cta) : order(o), p(p) {
+        upo = p.n_kv * p.n_mt;
+        live = o.n_live;
+        my_r = cta / upo;
+        my_u = cta - my_r * upo;
+        base_r = base_u = 0;
+        back = false;
+    }
+    __device__ __forceinline__ bool next(XaSegment &s) {
+        int r = base_r + my_r, u = base_u + my_u;
+        base_r += p.round_r;
+        base_u += p.round_u;
+        if (base_u >= upo) {
+            base_u -= upo;
+            ++base_r;
+        }
+        if (back) {  // from the end of the round
+            r = base_r - my_r;
+            u = base_u - 1 - my_u;
+            if (u < 0) {
+                u += upo;
+                --r;
+            }
+        } else if (u >= upo) {
+            u -= upo;
+            ++r;
+        }
+        back = !back;
+        if (r >= live) return false;
+        const int4 it = order.item[r];
+        s.obs = it.x;
+        s.len = it.y;
+        s.pad_lo = it.z;
+        s.pad_hi = it.w;
+        s.kvh = p.n_mt == 1 ? u : u / p.n_mt;
+        s.mt = p.n_mt == 1 ? 0 : u - s.kvh * p.n_mt;
+        s.j0 = 0;
+        s.j1 = (it.y + XA_BKV - 1) / XA_BKV;
+        s.slot = -1;
+        return true;
+    }
+};
+template <typename LenOf>
+struct XaWork<true, LenOf> {
+    RaggedCursor<LenOf> cur;
+    const CrossParams &p;
+    int w, w1, c, n_mt;
+    bool whole_units;
+    __device__ __forceinline__ XaWork(LenOf f, const CrossParams &p, const XaOrder &, int cta) : cur(f, p.n_obs, p.n_kv * p.n_mt, XA_BKV), p(p) {
         c = cta;
         n_mt = p.n_mt;
-        n_kv = p.n_kv;
-        n_work = p.n_work;
         whole_units = p.ws_o == nullptr;
-        sorted = whole_units && p.n_obs <= XA_SORT;
-        if (sorted) {
-            w = 0;
-            w1 = o.n_live * p.n_kv * p.n_mt;
-        } else {
-            const int total = xa_total_blocks(p), n = min(p.n_work, total);
-            w = cta < n ? xa_border(cta, n, total) : total;
-            w1 = cta < n ? xa_border(cta + 1, n, total) : total;
-        }
+        const int total = xa_total_blocks(p), n = min(p.n_work, total);
+        w = cta < n ? xa_border(cta, n, total) : total;
+        w1 = cta < n ? xa_border(cta + 1, n, total) : total;
     }
     __device__ __forceinline__ bool next(XaSegment &s) {  // whole warp
-        if (sorted) {
-            const int k = w * n_work + (w & 1 ? n_work - 1 - c : c);
-            if (k >= w1) return false;
-            ++w;
-            const int upo = n_kv * n_mt, r = k / upo, u = k - r * upo;
-            s.obs = order.obs[r];
-            s.len = order.len[s.obs];
-            s.pad_lo = order.pad_lo[s.obs];
-            s.pad_hi = order.pad_hi[s.obs];
-            s.kvh = u / n_mt;
-            s.mt = u - s.kvh * n_mt;
-            s.j0 = 0;
-            s.j1 = (s.len + XA_BKV - 1) / XA_BKV;
-            s.slot = -1;
-            return true;
-        }
         RaggedUnit u;
         while (w < w1 && cur.find(w, u)) {
             const int nb = (u.len + XA_BKV - 1) / XA_BKV;
@@ -197,11 +254,12 @@ struct CrossSmem {
     static_assert(S_COL + 2 * BKV <= 512 && TOTAL <= 227 * 1024, "TMEM, shared memory");
 };
 
-// Rows of empty observations: 0 and -inf.  CTA (pair) c looks after every n_work-th observation.
-template <int HD>
-__device__ __forceinline__ void xa_fill_empty(const CrossParams &p, int c, int tid, int n_threads) {
-    for (int obs = c; obs < p.n_obs; obs += p.n_work) {
-        if (xa_len(p, obs) > 0) continue;
+// Rows of empty observations: 0 and -inf.  CTA (pair) c looks after every n_work-th of them (LIST: of all observations).
+template <int HD, bool LIST>
+__device__ __forceinline__ void xa_fill_empty(const CrossParams &p, const XaOrder &order, int c, int tid, int n_threads) {
+    for (int i = (LIST ? 0 : order.n_live) + c; i < p.n_obs; i += p.n_work) {
+        if (LIST && xa_len(p, i) > 0) continue;
+        const int obs = LIST ? i : order.item[i].x;
         const long long n = (long long)p.n_q * p.S;
         uint4 *out = reinterpret_cast<uint4 *>(p.out + obs * n * HD);
         for (long long i = tid; i < n * (HD / 8); i += n_threads) out[i] = make_uint4(0, 0, 0, 0);
@@ -243,17 +301,14 @@ __device__ __forceinline__ void xa_clean_blocks(XaSegment &s, bool &ok, uint32_t
     }
 }
 
-// -inf over the hidden ones of 32 columns that begin at row c0; groups that hide nothing cost nothing (all 128 columns of a block tested for
-// length and range took 2,000 clocks).
+// -inf over the hidden ones of 32 columns that begin at row c0.  Which those are is the same for all rows: one word of bits, and groups that hide
+// nothing cost nothing (every column of a block tested for length and range took 2,000 clocks, of the groups concerned 1,000).
+__device__ __forceinline__ uint32_t xa_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 __device__ __forceinline__ void xa_mask32(uint32_t (&x)[32], int c0, int len, int pad_lo, int pad_hi) {
-    const int lim = len - c0, lo = pad_lo - c0, hi = pad_hi - c0;
-    if (lim < 32) {
+    const uint32_t seen = xa_below(len - c0) & ~(xa_below(pad_hi - c0) & ~xa_below(pad_lo - c0));
+    if (seen != 0xffffffffu) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = e < lim ? x[e] : 0xff800000u;
-    }
-    if (lo < 32 && hi > 0) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = e < lo || e >= hi ? x[e] : 0xff800000u;
+        for (int e = 0; e < 32; ++e) x[e] = seen & (1u << e) ? x[e] : 0xff800000u;
     }
 }
 
@@ -277,7 +332,7 @@ __device__ __forceinline__ void xa_store32(__nv_bfloat16 *dst, const uint32_t (&
     }
 }
 
-template <int HD>
+template <int HD, bool LIST>
 __global__ void __launch_bounds__(XA_THREADS, 1)
 cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
@@ -295,6 +350,8 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{abort_flag, p.status};
+    XaOrder &order = *reinterpret_cast<XaOrder *>(smem + L::ORDER_OFF);
+    if (!LIST) xa_sort_clear(order, XA_THREADS);
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < QS; ++i) {
@@ -334,10 +391,9 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
     pdl_wait();
 
     auto len_of = [&](int obs) { return xa_len(p, obs); };
-    XaOrder &order = *reinterpret_cast<XaOrder *>(smem + L::ORDER_OFF);
-    xa_sort(p, order, XA_THREADS);
-    if (warp < XA_LOADER) xa_fill_empty<HD>(p, blockIdx.x, threadIdx.x, 32 * XA_LOADER);
-    XaWork work(len_of, p, order, blockIdx.x);
+    if (!LIST) xa_sort(p, order);
+    if (warp < XA_LOADER) xa_fill_empty<HD, LIST>(p, order, blockIdx.x, threadIdx.x, 32 * XA_LOADER);
+    XaWork<LIST, decltype(len_of)> work(len_of, p, order, blockIdx.x);
     XaSegment s;
     bool ok = true;
 
@@ -397,26 +453,36 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         };
         uint32_t si = 0, jb = 0;
         uint32_t blk[2] = {0, 0}, seg[2] = {0, 0};  // blocks and segments of each tile so far
-        for (; ok && work.next(s); ++si) {
-            const int tiles = p.R > s.mt * 256 + 128 ? 2 : 1;
-            const uint32_t qs = si % QS;
-            ok = warp_wait(&q_full[qs], si / QS & 1u, wc, DEV_TIMEOUT_FULL);
-            if (ok) ok = warp_wait(&k_full[jb % NS], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-            if (!ok) break;
-            tc_fence_after();
-            // a tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order
-            for (int t = 0; t < tiles; ++t) issue_s(qs, t, jb % NS);
-            if (elect_one()) {
-                tc_commit(&k_free[jb % NS]);
-                if (s.j1 - s.j0 == 1) tc_commit(&q_free[qs]);
+        // S of a segment's first block follows the P V of the segment before: by tile where its Q has its own stage, behind both otherwise.
+        // A tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order.
+        auto tiles_of = [&](const XaSegment &g) { return p.R > g.mt * 256 + 128 ? 2 : 1; };
+        XaSegment after;
+        bool here = work.next(s);
+        if (here) {
+            ok = warp_wait(&q_full[0], 0, wc, DEV_TIMEOUT_FULL);
+            if (ok) ok = warp_wait(&k_full[0], 0, wc, DEV_TIMEOUT_FULL);
+            if (ok) {
+                tc_fence_after();
+                for (int t = 0; t < tiles_of(s); ++t) issue_s(0, t, 0);
+                if (elect_one()) {
+                    tc_commit(&k_free[0]);
+                    if (s.j1 - s.j0 == 1) tc_commit(&q_free[0]);
+                }
             }
+        }
+        for (; ok && here; ++si) {
+            const int tiles = tiles_of(s);
+            const uint32_t qs = si % QS, qn = (si + 1) % QS;
+            const bool next = work.next(after);
+            const int tiles_n = next ? tiles_of(after) : 0;
             for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
                 const uint32_t st = jb % NS, sn = (jb + 1) % NS;
                 const uint64_t v = v_desc0 + (uint64_t)(st * (L::KV_BYTES >> 4));
-                const bool more = j + 1 < s.j1;
+                const bool more = j + 1 < s.j1, early = QS > 1 && !more && next;
                 // what comes early is waited for before the softmax is
                 ok = warp_wait(&v_full[st], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-                if (ok && more) ok = warp_wait(&k_full[sn], ((jb + 1) / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                if (ok && (more || early)) ok = warp_wait(&k_full[sn], ((jb + 1) / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                if (ok && early) ok = warp_wait(&q_full[qn], (si + 1) / QS & 1u, wc, DEV_TIMEOUT_FULL);
                 for (int t = 0; ok && t < tiles; ++t) {
                     if (j == s.j0) ok = warp_wait(&o_free[t], (seg[t] & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
                     if (ok) ok = warp_wait(&p_full[2 * t], blk[t] & 1u, wc, DEV_TIMEOUT_FULL);
@@ -438,15 +504,29 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                         tc_commit(&pv_done[t]);
                     }
                     if (more) issue_s(qs, t, sn);
+                    else if (early && t < tiles_n) issue_s(qn, t, sn);
                     ++blk[t];
                 }
-                if (ok && elect_one()) {
-                    tc_commit(&v_free[st]);
-                    if (more) tc_commit(&k_free[sn]);
-                    if (j + 2 == s.j1) tc_commit(&q_free[qs]);  // the segment's last S blocks have been issued
+                if (!ok) break;
+                if (elect_one()) tc_commit(&v_free[st]);
+                if (!more && next) {  // the S blocks of the next segment that are not issued yet
+                    if (!early) {
+                        ok = warp_wait(&k_full[sn], ((jb + 1) / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                        if (ok) ok = warp_wait(&q_full[qn], (si + 1) / QS & 1u, wc, DEV_TIMEOUT_FULL);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    for (int t = early ? tiles : 0; t < tiles_n; ++t) issue_s(qn, t, sn);
+                }
+                if (elect_one()) {
+                    if (more || next) tc_commit(&k_free[sn]);
+                    if (j + 2 == s.j1) tc_commit(&q_free[qs]);  // a segment's last S blocks have been issued
+                    if (!more && next && after.j1 - after.j0 == 1) tc_commit(&q_free[qn]);
                 }
             }
             for (int t = 0; t < tiles; ++t) ++seg[t];
+            s = after;
+            here = next;
         }
     } else if (warp > XA_CLEANER) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_REST));
@@ -457,9 +537,16 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         const uint32_t s_addr = tmem_base + L::S_COL + t * BKV + lane_sel, o_addr = tmem_base + t * HD + lane_sel;
         const F2 scale2 = f2(p.scale_log2, p.scale_log2);
         uint32_t blk = 0;  // blocks of this tile so far
-        while (ok && work.next(s)) {
+        auto next = [&](XaSegment &g) {  // with rows in this tile
+            do {
+                if (!work.next(g)) return false;
+            } while (t == 1 && g.mt * 256 + 128 >= p.R);
+            return true;
+        };
+        XaSegment after;
+        int mt_of_place = -1, place = 0;  // of this thread's row: token * n_q + head of the kv head's group
+        for (bool here = next(s); ok && here; s = after) {
             const int row0 = s.mt * 256 + t * 128;
-            if (t == 1 && row0 >= p.R) continue;
             const int lr = t * 128 + qtr * 32 + lane, row = s.mt * 256 + lr;  // in the unit, in the item
             const bool live = row0 + qtr * 32 < p.R;                          // of the warp
             const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
@@ -552,15 +639,19 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                 l_sum += (u0 + u1) + (u2 + u3);
             }
             if (!ok) break;
-            // ---- O / l -> bf16 -> out, or the piece into the workspace ----
+            // ---- O / l -> bf16 -> out, or the piece into the workspace; what comes next and the rows' places are worked out meanwhile ----
+            here = next(after);
+            const bool row_ok = row < p.R;
+            if (s.mt != mt_of_place) {
+                mt_of_place = s.mt;
+                place = xa_place(p, row);
+            }
+            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
+            __nv_bfloat16 *dst = p.out + ((long long)s.obs * p.S * p.n_q + s.kvh * p.g + place) * HD;
+            float *wo = p.ws_o + ((long long)s.slot * p.ws_rows + lr) * HD;
             ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
             if (!ok) break;
             tc_fence_after();
-            const bool row_ok = row < p.R;
-            const int head = row_ok ? s.kvh * p.g + row / p.S : 0, tok = row_ok ? row % p.S : 0;
-            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
-            __nv_bfloat16 *dst = p.out + (((long long)s.obs * p.S + tok) * p.n_q + head) * HD;
-            float *wo = p.ws_o + ((long long)s.slot * p.ws_rows + lr) * HD;
             if (live) {
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
@@ -586,7 +677,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                 if (s.slot >= 0)
                     *reinterpret_cast<float2 *>(p.ws_ml + ((long long)s.slot * p.ws_rows + lr) * 2) = make_float2(m_used, l_sum);
                 else if (p.lse)
-                    p.lse[((long long)s.obs * p.n_q + head) * p.S + tok] = l_sum == 0.0f ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
+                    p.lse[((long long)s.obs * p.n_kv + s.kvh) * p.R + row] = l_sum == 0.0f ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
             }
         }
     }
@@ -617,6 +708,7 @@ struct CrossPairSmem {
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
+template <bool LIST>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XP_THREADS, 1)
 cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map, const CrossParams p) {
@@ -638,6 +730,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     const uint32_t rank = cluster_ctarank();
     const WaitCtx wc{abort_flag, p.status};
     const uint32_t both = rank == 0 ? 2u : 1u;  // even CTA: its own TMA and the odd CTA's word
+    XaOrder &order = *reinterpret_cast<XaOrder *>(smem + L::ORDER_OFF);
+    if (!LIST) xa_sort_clear(order, XP_THREADS);
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, both);
@@ -681,10 +775,9 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     pdl_wait();
 
     auto len_of = [&](int obs) { return xa_len(p, obs); };
-    XaOrder &order = *reinterpret_cast<XaOrder *>(smem + L::ORDER_OFF);
-    xa_sort(p, order, XP_THREADS);
-    if (warp < XP_LOADER) xa_fill_empty<HD>(p, blockIdx.x >> 1, rank * 32 * XP_LOADER + threadIdx.x, 64 * XP_LOADER);
-    XaWork work(len_of, p, order, blockIdx.x >> 1);
+    if (!LIST) xa_sort(p, order);
+    if (warp < XP_LOADER) xa_fill_empty<HD, LIST>(p, order, blockIdx.x >> 1, rank * 32 * XP_LOADER + threadIdx.x, 64 * XP_LOADER);
+    XaWork<LIST, decltype(len_of)> work(len_of, p, order, blockIdx.x >> 1);
     XaSegment s;
     bool ok = true;
     uint32_t si = 0, jb = 0;  // segments and blocks so far
@@ -827,6 +920,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 else mbar_arrive_cluster(bar, 0);
             }
         };
+        int mt_of_place = -1, place = 0;  // of this thread's row: token * n_q + head of the kv head's group
         auto is_live = [&](const XaSegment &sg) { return sg.mt * 256 + (int)rank * 128 + qtr * 32 < p.R; };  // has the warp rows
         // segment `u` is complete: O / l -> bf16 -> out, or the piece into the workspace
         auto drain = [&](uint32_t u, const XaSegment &sg, float m, float l_mine) -> bool {
@@ -841,9 +935,12 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             const float l = l_mine + xch[512 + (half ^ 1) * 128 + my_slot];
             const int row = sg.mt * 256 + lr;
             const bool row_ok = row < p.R;
-            const int head = row_ok ? sg.kvh * p.g + row / p.S : 0, tok = row_ok ? row % p.S : 0;
+            if (sg.mt != mt_of_place) {
+                mt_of_place = sg.mt;
+                place = xa_place(p, row);
+            }
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            __nv_bfloat16 *dst = p.out + (((long long)sg.obs * p.S + tok) * p.n_q + head) * HD;
+            __nv_bfloat16 *dst = p.out + ((long long)sg.obs * p.S * p.n_q + sg.kvh * p.g + place) * HD;
             float *wo = p.ws_o + ((long long)sg.slot * p.ws_rows + lr) * HD;
 #pragma unroll 1
             for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
@@ -869,7 +966,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 if (sg.slot >= 0)
                     *reinterpret_cast<float2 *>(p.ws_ml + ((long long)sg.slot * p.ws_rows + lr) * 2) = make_float2(m, l);
                 else if (p.lse)
-                    p.lse[((long long)sg.obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                    p.lse[((long long)sg.obs * p.n_kv + sg.kvh) * p.R + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
             }
             return true;  // (the row-sum slots are next written after at least one more meeting of the pair)
         };
@@ -1134,11 +1231,13 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
     if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     if constexpr (HD == 256) {
-        if ((rc = ensure_dyn_smem(cross_attn_pair_kernel, CrossPairSmem::TOTAL))) return rc;
-        rc = launch_pdl(cross_attn_pair_kernel, dim3(2 * (unsigned)plan.n_work), dim3(XP_THREADS), CrossPairSmem::TOTAL, stream, qmap, kmap, vmap, p);
+        const auto kernel = p.ws_o || p.n_obs > XA_SORT ? cross_attn_pair_kernel<true> : cross_attn_pair_kernel<false>;
+        if ((rc = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), CrossPairSmem::TOTAL))) return rc;
+        rc = launch_pdl(kernel, dim3(2 * (unsigned)plan.n_work), dim3(XP_THREADS), CrossPairSmem::TOTAL, stream, qmap, kmap, vmap, p);
     } else {
-        if ((rc = ensure_dyn_smem(cross_attn_kernel<HD>, CrossSmem<HD>::TOTAL))) return rc;
-        rc = launch_pdl(cross_attn_kernel<HD>, dim3((unsigned)plan.n_work), dim3(XA_THREADS), CrossSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
+        const auto kernel = p.ws_o || p.n_obs > XA_SORT ? cross_attn_kernel<HD, true> : cross_attn_kernel<HD, false>;
+        if ((rc = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), CrossSmem<HD>::TOTAL))) return rc;
+        rc = launch_pdl(kernel, dim3((unsigned)plan.n_work), dim3(XA_THREADS), CrossSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
     }
     if (rc || !p.ws_o) return rc;
     return launch_combine<HD>(p, stream);
@@ -1198,6 +1297,11 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     p.n_mt = plan.n_mt;
     p.unit_rows = plan.unit_rows;
     p.n_work = plan.n_work;
+    const long long upo = (long long)p.n_kv * p.n_mt;
+    p.round_r = (int)(p.n_work / upo);
+    p.round_u = (int)(p.n_work % upo);
+    p.bin_shift = 0;
+    while (((max_len + 127LL) / 128 >> p.bin_shift) > vb::XA_BINS - 2) ++p.bin_shift;
     p.out_al32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0 ? 1 : 0;
     p.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)hd));
     p.status = vb::device_status_ptr();
