@@ -37,8 +37,9 @@ constexpr int XA_BKV = 128;      // rows of K / V per block
 constexpr int XA_THREADS = 384;  // warps 0-3 tile 0, 4-7 tile 1, 8 loader, 9 MMA, 10 V cleaner, 11 fills the warpgroup that gives up registers
 constexpr int XA_LOADER = 8, XA_MMA = 9, XA_CLEANER = 10;
 constexpr int XA_EARLY = 96;     // of a block's rows: their P V runs beside the softmax of the others
-// Registers of a thread: 384 x 168 at launch = 64,512; 2 x 128 x 208 + 128 x 88 = 64,512 after the split.
-constexpr int XA_REGS_SOFTMAX = 208, XA_REGS_REST = 88;
+// Registers of a thread: 384 x 168 at launch = 64,512; 2 x 128 x 192 + 128 x 120 = 64,512 after the split.  With 208 + 88 the issuing warp kept its
+// descriptors and the next unit in local memory: 64 x 50 tokens over 113 to 241 rows 24.6 us instead of 22.6, the longest case 203 instead of 199.
+constexpr int XA_REGS_SOFTMAX = 192, XA_REGS_REST = 120;
 constexpr float XA_RAISE = 8.0f; // the running maximum is raised, and O rescaled, only by blocks that exceed it by more than 2^8
 
 struct CrossParams {
@@ -312,22 +313,42 @@ __device__ __forceinline__ void xa_mask32(uint32_t (&x)[32], int c0, int len, in
     }
 }
 
-// 32 columns of O of one row, divided and rounded, to 32 bf16 at dst.
-__device__ __forceinline__ void xa_store32(__nv_bfloat16 *dst, const uint32_t (&o)[32], float inv, int al32) {
+// COLS columns of O of one row per thread, out of TMEM: divided and rounded to dst, or (ws) as they are.  The loads of 32 N columns are in flight
+// at once: one at a time 32 columns took 870 clocks.  `out_of_tmem` runs when all have been read.
+template <int COLS, int N, typename F>
+__device__ __forceinline__ void xa_drain(uint32_t o_addr, bool row_ok, __nv_bfloat16 *dst, float inv, int al32, float *ws, F out_of_tmem) {
+    const F2 inv2 = f2(inv, inv);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        uint32_t w[8];
+    for (int c0 = 0; c0 < COLS; c0 += 32 * N) {
+        uint32_t o[N][32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[16 * q + 2 * e]) * inv, __uint_as_float(o[16 * q + 2 * e + 1]) * inv);
-            w[e] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        if (al32) {
-            st_global_v8(dst + 16 * q, w);
-        } else {
-            uint4 *d4 = reinterpret_cast<uint4 *>(dst + 16 * q);
-            d4[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            d4[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int i = 0; i < N; ++i) tmem_ld32(o_addr + (uint32_t)(c0 + 32 * i), o[i]);
+        tmem_ld_wait();
+        if (c0 + 32 * N == COLS) out_of_tmem();
+        if (!row_ok) continue;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) {
+            const uint32_t(&v)[32] = o[i / 2];
+            const int h = 16 * (i & 1), at = c0 + 16 * i;
+            uint32_t w[8];
+            if (ws) {
+#pragma unroll
+                for (int q = 0; q < 16; q += 8) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = v[h + q + e];
+                    st_global_v8(ws + at + q, w);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = f2_bf16(f2_mul(f2(__uint_as_float(v[h + 2 * e]), __uint_as_float(v[h + 2 * e + 1])), inv2));
+            if (al32) {
+                st_global_v8(dst + at, w);
+            } else {
+                uint4 *d4 = reinterpret_cast<uint4 *>(dst + at);
+                d4[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                d4[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
         }
     }
 }
@@ -648,37 +669,23 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
             }
             const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
             __nv_bfloat16 *dst = p.out + ((long long)s.obs * p.S * p.n_q + s.kvh * p.g + place) * HD;
-            float *wo = p.ws_o + ((long long)s.slot * p.ws_rows + lr) * HD;
-            ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
-            if (!ok) break;
-            tc_fence_after();
-            if (live) {
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t ov[32];
-                    tmem_ld32(o_addr + (uint32_t)c, ov);
-                    tmem_ld_wait();
-                    if (!row_ok) continue;
-                    if (s.slot < 0) {
-                        xa_store32(dst + c, ov, inv, p.out_al32);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            const uint32_t w[8] = {ov[e], ov[e + 1], ov[e + 2], ov[e + 3], ov[e + 4], ov[e + 5], ov[e + 6], ov[e + 7]};
-                            st_global_v8(wo + c + e, w);
-                        }
-                    }
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[t]);
+            float *wo = LIST && s.slot >= 0 ? p.ws_o + ((long long)s.slot * p.ws_rows + lr) * HD : nullptr;
             if (row_ok) {
-                if (s.slot >= 0)
+                if (wo)
                     *reinterpret_cast<float2 *>(p.ws_ml + ((long long)s.slot * p.ws_rows + lr) * 2) = make_float2(m_used, l_sum);
                 else if (p.lse)
                     p.lse[((long long)s.obs * p.n_kv + s.kvh) * p.R + row] = l_sum == 0.0f ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
             }
+            ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
+            if (!ok) break;
+            tc_fence_after();
+            auto out_of_tmem = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_free[t]);
+            };
+            if (live) xa_drain<HD, 1>(o_addr, row_ok, dst, inv, p.out_al32, wo, out_of_tmem);
+            else out_of_tmem();
         }
     }
     tc_fence_before();
@@ -924,50 +931,37 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         auto is_live = [&](const XaSegment &sg) { return sg.mt * 256 + (int)rank * 128 + qtr * 32 < p.R; };  // has the warp rows
         // segment `u` is complete: O / l -> bf16 -> out, or the piece into the workspace
         auto drain = [&](uint32_t u, const XaSegment &sg, float m, float l_mine) -> bool {
-            if (!warp_wait(o_done, u & 1u, wc, DEV_TIMEOUT_ACCUM)) return false;
-            tc_fence_after();
-            if (!is_live(sg)) {
-                arrive_even(o_free);
-                return true;
-            }
-            xch[512 + half * 128 + my_slot] = l_mine;
-            if (!pair_sync()) return false;
-            const float l = l_mine + xch[512 + (half ^ 1) * 128 + my_slot];
+            const bool live = is_live(sg);
             const int row = sg.mt * 256 + lr;
             const bool row_ok = row < p.R;
-            if (sg.mt != mt_of_place) {
-                mt_of_place = sg.mt;
-                place = xa_place(p, row);
-            }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            __nv_bfloat16 *dst = p.out + ((long long)sg.obs * p.S * p.n_q + sg.kvh * p.g + place) * HD;
-            float *wo = p.ws_o + ((long long)sg.slot * p.ws_rows + lr) * HD;
-#pragma unroll 1
-            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
-                uint32_t ov[32];
-                tmem_ld32(tmem_base + lane_sel + (uint32_t)c, ov);
-                tmem_ld_wait();
-                if (c + 32 == (half + 1) * (HD / 2)) {  // O is out of TMEM
-                    tc_fence_before();
-                    arrive_even(o_free);
+            float inv = 0.0f, *wo = nullptr;
+            __nv_bfloat16 *dst = nullptr;
+            if (live) {  // while the last P V runs
+                xch[512 + half * 128 + my_slot] = l_mine;
+                if (!pair_sync()) return false;
+                const float l = l_mine + xch[512 + (half ^ 1) * 128 + my_slot];
+                if (sg.mt != mt_of_place) {
+                    mt_of_place = sg.mt;
+                    place = xa_place(p, row);
                 }
-                if (!row_ok) continue;
-                if (sg.slot < 0) {
-                    xa_store32(dst + c, ov, inv, p.out_al32);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        const uint32_t w[8] = {ov[e], ov[e + 1], ov[e + 2], ov[e + 3], ov[e + 4], ov[e + 5], ov[e + 6], ov[e + 7]};
-                        st_global_v8(wo + c + e, w);
-                    }
+                inv = l == 0.0f ? 0.0f : 1.0f / l;
+                dst = p.out + ((long long)sg.obs * p.S * p.n_q + sg.kvh * p.g + place) * HD + half * (HD / 2);
+                if (LIST && sg.slot >= 0) wo = p.ws_o + ((long long)sg.slot * p.ws_rows + lr) * HD + half * (HD / 2);
+                if (row_ok && half == 0) {
+                    if (wo)
+                        *reinterpret_cast<float2 *>(p.ws_ml + ((long long)sg.slot * p.ws_rows + lr) * 2) = make_float2(m, l);
+                    else if (p.lse)
+                        p.lse[((long long)sg.obs * p.n_kv + sg.kvh) * p.R + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                 }
             }
-            if (row_ok && half == 0) {
-                if (sg.slot >= 0)
-                    *reinterpret_cast<float2 *>(p.ws_ml + ((long long)sg.slot * p.ws_rows + lr) * 2) = make_float2(m, l);
-                else if (p.lse)
-                    p.lse[((long long)sg.obs * p.n_kv + sg.kvh) * p.R + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-            }
+            if (!warp_wait(o_done, u & 1u, wc, DEV_TIMEOUT_ACCUM)) return false;
+            tc_fence_after();
+            auto out_of_tmem = [&]() {
+                tc_fence_before();
+                arrive_even(o_free);
+            };
+            if (live) xa_drain<HD / 2, LIST ? 2 : 4>(tmem_base + lane_sel + (uint32_t)(half * (HD / 2)), row_ok, dst, inv, p.out_al32, wo, out_of_tmem);
+            else out_of_tmem();
             return true;  // (the row-sum slots are next written after at least one more meeting of the pair)
         };
         XaSegment prev;
