@@ -67,6 +67,12 @@ __device__ __forceinline__ float xa_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// log2 of a row sum, off by 2^-22: the fast logarithm's error is that of a whole number plus it, once its argument lies in [0.75, 1.5).
+__device__ __forceinline__ float xa_log2(float x) {
+    const int bits = __float_as_int(x), k = (bits - 0x3f400000) >> 23;
+    const float r = (float)k + __log2f(__int_as_float(bits - (k << 23)));
+    return x < INFINITY ? r : x;  // infinite or no number: as it is
+}
 __device__ __forceinline__ float xa_max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -667,14 +673,14 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                 mt_of_place = s.mt;
                 place = xa_place(p, row);
             }
-            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
+            const float inv = l_sum == 0.0f ? 0.0f : __fdividef(1.0f, l_sum);
             __nv_bfloat16 *dst = p.out + ((long long)s.obs * p.S * p.n_q + s.kvh * p.g + place) * HD;
             float *wo = LIST && s.slot >= 0 ? p.ws_o + ((long long)s.slot * p.ws_rows + lr) * HD : nullptr;
             if (row_ok) {
                 if (wo)
                     *reinterpret_cast<float2 *>(p.ws_ml + ((long long)s.slot * p.ws_rows + lr) * 2) = make_float2(m_used, l_sum);
                 else if (p.lse)
-                    p.lse[((long long)s.obs * p.n_kv + s.kvh) * p.R + row] = l_sum == 0.0f ? -INFINITY : (m_used + log2f(l_sum)) * 0.6931471805599453f;
+                    p.lse[((long long)s.obs * p.n_kv + s.kvh) * p.R + row] = l_sum == 0.0f ? -INFINITY : (m_used + xa_log2(l_sum)) * 0.6931471805599453f;
             }
             ok = warp_wait(&pv_done[t], (blk - 1) & 1u, wc, DEV_TIMEOUT_ACCUM);
             if (!ok) break;
@@ -944,14 +950,14 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     mt_of_place = sg.mt;
                     place = xa_place(p, row);
                 }
-                inv = l == 0.0f ? 0.0f : 1.0f / l;
+                inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
                 dst = p.out + ((long long)sg.obs * p.S * p.n_q + sg.kvh * p.g + place) * HD + half * (HD / 2);
                 if (LIST && sg.slot >= 0) wo = p.ws_o + ((long long)sg.slot * p.ws_rows + lr) * HD + half * (HD / 2);
                 if (row_ok && half == 0) {
                     if (wo)
                         *reinterpret_cast<float2 *>(p.ws_ml + ((long long)sg.slot * p.ws_rows + lr) * 2) = make_float2(m, l);
                     else if (p.lse)
-                        p.lse[((long long)sg.obs * p.n_kv + sg.kvh) * p.R + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                        p.lse[((long long)sg.obs * p.n_kv + sg.kvh) * p.R + row] = l == 0.0f ? -INFINITY : (m + xa_log2(l)) * 0.6931471805599453f;
                 }
             }
             if (!warp_wait(o_done, u & 1u, wc, DEV_TIMEOUT_ACCUM)) return false;
@@ -1165,20 +1171,20 @@ __global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kern
                 l = fmaf(s_l[w], scale, l);
                 o = fmaf(s_o[w][col], scale, o);
             }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
             if (threadIdx.x < HD) {
                 const int i = col;
                 dst[i] = __float2bfloat16_rn(o * inv);
             }
             __syncthreads();
         } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
 #pragma unroll
             for (int k = 0; k < NV; ++k)
                 reinterpret_cast<__nv_bfloat162 *>(dst)[k * 32 + lane] = __floats2bfloat162_rn(acc[k].x * inv, acc[k].y * inv);
         }
         if (p.lse && lane == 0 && member == 0)
-            p.lse[((long long)obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+            p.lse[((long long)obs * p.n_q + head) * p.S + tok] = l == 0.0f ? -INFINITY : (M + xa_log2(l)) * 0.6931471805599453f;
     }
 }
 
