@@ -17,7 +17,7 @@
 // One query token: K streams once, HBM bounds it.  Many: the exponentials (16 per clock and SM) at heads of 64 and 128, at 256 their sum
 // with the product's chain.  Measured (cold L2): 4 x 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 keys 145 us, 90 of them the
 // exponential unit's (a polynomial on the FMA pipe for every fourth or eighth of them was slower: the sum warps' issue slots are full);
-// 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 keys 27 us; one token over 16,001 keys 18 us, 13 with the pages in L2.
+// 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 keys 26 us; one token over 16,001 keys 14 us, 10.5 with the pages in L2.
 #include <cuda_bf16.h>
 
 #include "f32x2.cuh"
@@ -40,10 +40,10 @@ struct KeyMassParams {
     int *status;
 };
 
-template <int HD>
+template <int HD, int NQ_>
 struct KeyMassSmem {
     static constexpr int CB = HD / 64;                // 64-element column blocks
-    static constexpr int NQ = HD == 256 ? 128 : 256;  // query rows per chunk
+    static constexpr int NQ = NQ_;                    // query rows per chunk
     static constexpr int NB = 512 / NQ;               // accumulators
     static constexpr int MAX_STAGES = 6;
     static constexpr int K_BYTES = CB * 128 * 128;    // [CB][128 keys][128 B]
@@ -54,6 +54,7 @@ struct KeyMassSmem {
     static constexpr int LSE_OFF = BAR_OFF + 512;     // float [KM_SUMS][128]
     static constexpr int SUM_OFF = LSE_OFF + KM_SUMS * 128 * 4;  // float [2][KM_PARTS - 1][128]
     static constexpr int TOTAL = SUM_OFF + 2 * (KM_PARTS - 1) * 128 * 4 + 1024;
+    static_assert(NB == G, "a group of sum warps has an accumulator of its own");
     static_assert(2 * K_BYTES + 2 * Q_BYTES <= RING && TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -74,10 +75,10 @@ struct KmStage {
     }
 };
 
-template <int HD>
+template <int HD, int NQ>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(KM_THREADS, 1)
 key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const KeyMassParams p) {
-    using L = KeyMassSmem<HD>;
+    using L = KeyMassSmem<HD, NQ>;
     extern __shared__ uint8_t km_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(km_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
@@ -208,7 +209,10 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         // Parts in groups: a chunk is one group's, the next chunk the next group's, so that the groups are at different points of their work
         // (all of them on every chunk, a quarter of its columns each, they waited and computed in step).  Which group begins a
         // unit turns from unit to unit; `rel`, the group's place in that turn, says which chunks it adds up, and where its sum goes, so a
-        // unit's sums do not depend on what the pair did before.
+        // unit's sums do not depend on what the pair did before.  The groups meet at a unit's end: going on to the next one, with the sums handed to
+        // the group that ends last, was slower (4 x 816 tokens, heads of 128, 141 us instead of 136 with the pages in L2), since the
+        // accumulators are filled in order and either group's delay is the other's.  A unit that is one part's alone needs no
+        // meeting and its group takes every G-th (one token over 16,001 rows 14 us, 16 with one unit at a time).
         constexpr int PPC = L::PPC, G = L::G, NBLK = 4;
         const int qtr = warp & 3, part = warp >> 2, sub = part % PPC, group = part / PPC;
         float *ls = reinterpret_cast<float *>(smem + L::LSE_OFF) + warp * 128;
@@ -223,17 +227,20 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                 lv[i] = there && c < p.n_chunks && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : INFINITY;
             }
         };
-        uint32_t qu = 0, un = 0;  // chunks in front of this unit, units
+        const bool alone = PPC == 1 && p.n_chunks == 1;
+        uint32_t un = alone ? (uint32_t)group : 0u;  // units of the pair
+        auto rel_of = [&](uint32_t u) { return alone ? 0 : (int)(((uint32_t)group + G - u % G) % G); };
         bool ok = true;
-        int ui = cid;
-        bool there = cursor.find(ui, unit);
-        fetch_lse(there, unit, group);
+        bool there = cursor.find(cid + (int)un * ncl, unit);
+        fetch_lse(there, unit, rel_of(un));
         while (ok && there) {
             const RaggedUnit now = unit;
-            ui += ncl;
-            there = cursor.find(ui, unit);
+            const uint32_t qu = un * (uint32_t)p.n_chunks, turn = un & 1u;  // chunks in front of this unit
+            const int rel = rel_of(un);
+            un += alone ? (uint32_t)G : 1u;
+            const int rel_next = rel_of(un);
+            there = cursor.find(cid + (int)un * ncl, unit);
             const int item = now.obs * p.n_kv + now.kvh, key0 = now.block * 256 + (int)rank * 128, obs = now.obs;
-            const int rel = (int)((group + G - un % G) % G), rel_next = (rel + G - 1) % G;
             F2 acc[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i] = f2(0.0f, 0.0f);
@@ -288,23 +295,25 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                 }
             }
             if (!ok) break;
-            qu += (uint32_t)p.n_chunks;
             float x[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) f2_get(acc[i], x[2 * i], x[2 * i + 1]);
             float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             // the parts of the columns meet; the slots are used in turn, so one meeting per unit is enough
-            float *slot = sum_s + (un & 1u) * ((KM_PARTS - 1) * 128) + qtr * 32 + lane;
+            float *slot = sum_s + turn * ((KM_PARTS - 1) * 128) + qtr * 32 + lane;
             const int place = rel * PPC + sub;
-            if (place) slot[(place - 1) * 128] = sum;
-            mbar_arrive(&meet[qtr]);
-            ok = warp_wait(&meet[qtr], un & 1u, wc, DEV_TIMEOUT_MISC);
-            if (!ok) break;
-            ++un;
+            if (!alone) {
+                if (place) slot[(place - 1) * 128] = sum;
+                mbar_arrive(&meet[qtr]);
+                ok = warp_wait(&meet[qtr], turn, wc, DEV_TIMEOUT_MISC);
+                if (!ok) break;
+            }
             const int key = key0 + qtr * 32 + lane;
             if (!place && key < now.len) {
+                if (!alone) {
 #pragma unroll
-                for (int i = 0; i < KM_PARTS - 1; ++i) sum += slot[i * 128];
+                    for (int i = 0; i < KM_PARTS - 1; ++i) sum += slot[i * 128];
+                }
                 if (p.pad && key >= p.pad[2 * obs] && key < p.pad[2 * obs + 1]) sum = 0.0f;
                 const long long at = (long long)item * p.cap + key;
                 p.mass_out[at] = p.mass_in ? fmaf(p.decay, p.mass_in[at], sum) : sum;
@@ -320,14 +329,14 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
     }
 }
 
-template <int HD>
+template <int HD, int NQ>
 static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassParams &p, int max_units, cudaStream_t stream) {
-    using L = KeyMassSmem<HD>;
+    using L = KeyMassSmem<HD, NQ>;
     p.n_chunks = (p.R + L::NQ - 1) / L::NQ;
     p.box_rows = p.R >= L::NQ ? L::NQ / 2 : ((p.R + 31) & ~31) / 2;  // a multiple of 8: whole swizzle groups
     // A unit that takes its query rows in one chunk streams keys: the ring goes to K.  More chunks: K stays, query rows stream.
     const int q_stage = L::CB * p.box_rows * 128;
-    p.q_stages = p.n_chunks == 1 ? 2 : (L::RING - 2 * L::K_BYTES) / q_stage;
+    p.q_stages = p.n_chunks > 1 ? (L::RING - 2 * L::K_BYTES) / q_stage : (L::RING - 4 * q_stage) / L::K_BYTES == (L::RING - 2 * q_stage) / L::K_BYTES ? 4 : 2;
     if (p.q_stages > L::MAX_STAGES) p.q_stages = L::MAX_STAGES;
     p.k_stages = (L::RING - p.q_stages * q_stage) / L::K_BYTES;
     if (p.k_stages > L::MAX_STAGES) p.k_stages = L::MAX_STAGES;
@@ -345,9 +354,9 @@ static int launch_key_mass(const vlab200_kv_store *st, const void *q, KeyMassPar
         if (int rc = make_tensor_map(&kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->k_pages, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
     }
-    if (int rc = ensure_dyn_smem(key_mass_kernel<HD>, L::TOTAL)) return rc;
+    if (int rc = ensure_dyn_smem(key_mass_kernel<HD, NQ>, L::TOTAL)) return rc;
     const int pairs = sm_count() / 2;
-    return launch_pdl(key_mass_kernel<HD>, dim3(2 * (max_units < pairs ? max_units : pairs)), dim3(KM_THREADS), L::TOTAL, stream, qmap, kmap, p);
+    return launch_pdl(key_mass_kernel<HD, NQ>, dim3(2 * (max_units < pairs ? max_units : pairs)), dim3(KM_THREADS), L::TOTAL, stream, qmap, kmap, p);
 }
 
 }  // namespace vb
@@ -389,7 +398,8 @@ extern "C" int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, c
     p.status = vb::device_status_ptr();
     if (!p.status) return vb::cuda_fail(cudaGetLastError(), "device_status_ptr");
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (hd == 64) return vb::launch_key_mass<64>(st, q, p, (int)units, cs);
-    if (hd == 128) return vb::launch_key_mass<128>(st, q, p, (int)units, cs);
-    return vb::launch_key_mass<256>(st, q, p, (int)units, cs);
+    // Rows that fill one chunk of 128 are one group's alone: four units at a time in four accumulators, instead of two in two.
+    if (hd == 64) return R <= 128 ? vb::launch_key_mass<64, 128>(st, q, p, (int)units, cs) : vb::launch_key_mass<64, 256>(st, q, p, (int)units, cs);
+    if (hd == 128) return R <= 128 ? vb::launch_key_mass<128, 128>(st, q, p, (int)units, cs) : vb::launch_key_mass<128, 256>(st, q, p, (int)units, cs);
+    return vb::launch_key_mass<256, 128>(st, q, p, (int)units, cs);
 }
