@@ -58,6 +58,13 @@ CASES = [
     (300, 2, 2, 2, 64, 200, None, True),                # more observations than are sorted
     (270, 20, 8, 1, 256, 300, None, False),
     (260, 70, 4, 1, 128, 150, None, True),
+    (3, 2, 8, 1, 256, 700, None, True),                 # 16 rows: the most that the kernel of few rows takes
+    (2, 17, 2, 2, 128, 300, None, True),                # 17
+    (5, 1, 4, 4, 128, 65, [65, 64, 63, 1, 0], False),   # its blocks of 64 rows
+    (200, 5, 6, 2, 64, 200, None, True),                # several units per CTA
+    (150, 1, 8, 1, 256, 700, None, True),
+    (160, 2, 4, 2, 128, 500, None, False),
+    (150, 2, 1, 1, 64, 8300, None, True),               # more blocks than the sort has bins
 ]
 
 
@@ -120,6 +127,21 @@ def test_growing_keys_rescale(hd):
     for split in (True, False):
         out, lse = vb.cross_attention(st, 0, q, lens=lens, split=split)
         check(torch, st, 0, q, lens, None, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_growing_keys_under_one_token(hd):
+    """The same with few query rows: every block of 64 rows raises each warp's maximum."""
+    torch = require_cuda()
+    import vla_cpp_b200 as vb
+
+    st, q, lens, pads, g = make(torch, 2, 1, 8, 2, hd, 1600, [1600, 1111], True, 6)
+    st.k.mul_(torch.linspace(0.05, 6.0, 1600, device="cuda").bfloat16()[:, None])
+    for split in (True, False):
+        out, lse = vb.cross_attention(st, 0, q, lens=lens, pad_ranges=pads, split=split)
+        assert vb.device_status() == 0
+        check(torch, st, 0, q, lens, pads, out, lse)
 
 
 @pytest.mark.gpu

@@ -4,6 +4,7 @@
 //
 // visible: row < len[b], not in the observation's hidden range [lo, hi).  A row that sees nothing gives 0 and -inf, whatever the pages hold.
 //
+// Up to 16 query rows per kv head: cross_few_kernel, below.
 // Heads of 64 and 128, a unit = (observation, kv head, 256 of the g S stacked query rows), one CTA:
 //   loader warp       TMA: the two 128-row Q tiles of a unit, K and V in blocks of 128 rows through rings
 //   MMA warp          O_t += P_t V_j with P_t read from TMEM, XA_EARLY of the block's rows while the softmax is at the others, then
@@ -20,10 +21,10 @@
 // leaves un-normalised rows with their maximum and sum in the workspace, at most two pieces per CTA, and cross_combine_kernel merges them
 // in order.
 //
-// Measured (cold L2): 4 prompts of 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 rows 207 us = 991 TFLOP/s; there the chain of a
-// tile's block -- S, softmax, P V, some 3,500 clocks -- bounds it, of which the pipe computes 2,048 for the two tiles.  64 x 50 tokens, 15 / 5
-// heads of 64, over 113 to 241 rows 29 us, and 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 rows 37 us: a unit's fixed chain of
-// loads, first S, last P V and store, some 5 us, bounds those.
+// Measured (cold L2): 4 prompts of 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 rows 199 us = 1,030 TFLOP/s; there the chain of a
+// tile's block -- S, softmax, P V, some 3,400 clocks -- bounds it, of which the pipe computes 2,048 for the two tiles.  64 x 50 tokens, 15 / 5
+// heads of 64, over 113 to 241 rows 22 us, and 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 rows 35 us: the chain of a unit's blocks
+// (2,400 to 3,000 clocks each), of the first loads (5,000 to 8,000 with the launch) and of the store bounds those.
 #include <cuda_bf16.h>
 
 #include "f32x2.cuh"
@@ -98,7 +99,13 @@ __device__ __forceinline__ int xa_total_blocks(const CrossParams &p) {  // whole
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum * p.n_kv * p.n_mt;
 }
-__device__ __forceinline__ int xa_border(int c, int n, int total) { return (int)((long long)c * total / n); }
+__device__ __forceinline__ int xa_div(unsigned long long a, unsigned b) {  // a 64-bit division takes 500 clocks
+    return a >> 32 ? (int)(a / b) : (int)((unsigned)a / b);
+}
+__device__ __forceinline__ int xa_border(int c, int n, int total) { return xa_div((unsigned long long)c * (unsigned)total, (unsigned)n); }
+__device__ __forceinline__ int xa_cta_of(int block, int n, int total) {  // whose piece a block is in
+    return xa_div((unsigned long long)(block + 1u) * (unsigned)n - 1u, (unsigned)total);
+}
 
 struct XaSegment {  // a run of blocks [j0, j1) of one unit
     int obs, kvh, mt, j0, j1, len, slot;  // slot: of the workspace; -1: the unit is whole
@@ -112,33 +119,43 @@ struct XaSegment {  // a run of blocks [j0, j1) of one unit
 constexpr int XA_SORT = 256, XA_BINS = 64;
 struct XaOrder {
     int4 item[XA_SORT];                // observation, length, hidden range
-    int count[XA_SORT / 32][XA_BINS];  // by the warp that read them
+    int count[XA_SORT / 32][XA_BINS];  // by groups of 32 observations
     int n_live;                        // observations that have rows
 };
 __device__ __forceinline__ void xa_sort_clear(XaOrder &o, int n_threads) {  // a barrier of the block later: xa_sort
     for (int i = threadIdx.x; i < XA_SORT / 32 * XA_BINS; i += n_threads) (&o.count[0][0])[i] = 0;
 }
-__device__ __forceinline__ void xa_sort(const CrossParams &p, XaOrder &o) {  // the whole block: XA_SORT threads or more
+template <int THREADS>
+__device__ __forceinline__ void xa_sort(const CrossParams &p, XaOrder &o) {  // the whole block
+    constexpr int N = (XA_SORT + THREADS - 1) / THREADS, W = THREADS / 32;  // observations per thread
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (p.n_obs + 31) >> 5;
-    int4 mine = make_int4((int)threadIdx.x, 0, 0, 0);
-    int bin = XA_BINS, rank = 0;  // (lanes without an observation share a bin that is not counted)
-    if (warp < warps) {
-        if ((int)threadIdx.x < p.n_obs) {
-            mine.y = xa_len(p, mine.x);
-            xa_pad(p, mine.x, mine.z, mine.w);
+    int4 mine[N];
+    int bin[N], rank[N];  // (lanes without an observation share a bin that is not counted)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int g = warp + i * W;  // of the groups of 32 observations
+        mine[i] = make_int4(g * 32 + lane, 0, 0, 0);
+        bin[i] = XA_BINS;
+        if (g >= warps) continue;
+        if (mine[i].x < p.n_obs) {
+            mine[i].y = xa_len(p, mine[i].x);
+            xa_pad(p, mine[i].x, mine[i].z, mine[i].w);
             const int most = (p.max_len + XA_BKV - 1) / XA_BKV >> p.bin_shift;
-            bin = mine.y > 0 ? most - ((mine.y + XA_BKV - 1) / XA_BKV >> p.bin_shift) : XA_BINS - 1;
+            bin[i] = mine[i].y > 0 ? most - ((mine[i].y + XA_BKV - 1) / XA_BKV >> p.bin_shift) : XA_BINS - 1;
         }
-        const unsigned same = __match_any_sync(0xffffffffu, bin);
-        rank = __popc(same & ((1u << lane) - 1u));
-        if (bin < XA_BINS && rank == 0) o.count[warp][bin] = __popc(same);
+        const unsigned same = __match_any_sync(0xffffffffu, bin[i]);
+        rank[i] = __popc(same & ((1u << lane) - 1u));
+        if (bin[i] < XA_BINS && rank[i] == 0) o.count[g][bin[i]] = __popc(same);
     }
     __syncthreads();
-    if (warp < warps) {
-        int sum[2] = {0, 0}, before[2] = {0, 0};  // of this lane's two bins: all of them, those of the warps in front
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int g = warp + i * W;
+        if (g >= warps) continue;
+        int sum[2] = {0, 0}, before[2] = {0, 0};  // of this lane's two bins: all of them, those of the groups in front
         for (int w = 0; w < warps; ++w) {
             const int2 c = *reinterpret_cast<const int2 *>(&o.count[w][2 * lane]);
-            if (w == warp) {
+            if (w == g) {
                 before[0] = sum[0];
                 before[1] = sum[1];
             }
@@ -152,9 +169,9 @@ __device__ __forceinline__ void xa_sort(const CrossParams &p, XaOrder &o) {  // 
             if (lane >= d) incl += up;
         }
         const int at0 = incl - sum[0] - sum[1] + before[0], at1 = incl - sum[1] + before[1];
-        const int even = __shfl_sync(0xffffffffu, at0, bin >> 1), odd = __shfl_sync(0xffffffffu, at1, bin >> 1);
-        if (bin < XA_BINS) o.item[(bin & 1 ? odd : even) + rank] = mine;
-        if (warp == 0 && lane == 31) o.n_live = p.n_obs - sum[1];
+        const int even = __shfl_sync(0xffffffffu, at0, bin[i] >> 1), odd = __shfl_sync(0xffffffffu, at1, bin[i] >> 1);
+        if (bin[i] < XA_BINS) o.item[(bin[i] & 1 ? odd : even) + rank[i]] = mine[i];
+        if (g == 0 && lane == 31) o.n_live = p.n_obs - sum[1];
     }
     __syncthreads();
 }
@@ -414,11 +431,11 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         tma_prefetch_desc(&k_map);
         tma_prefetch_desc(&v_map);
     }
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();  // after the wait: cross_combine_kernel reads the lengths before its own
 
     auto len_of = [&](int obs) { return xa_len(p, obs); };
-    if (!LIST) xa_sort(p, order);
+    if (!LIST) xa_sort<XA_THREADS>(p, order);
     if (warp < XA_LOADER) xa_fill_empty<HD, LIST>(p, order, blockIdx.x, threadIdx.x, 32 * XA_LOADER);
     XaWork<LIST, decltype(len_of)> work(len_of, p, order, blockIdx.x);
     XaSegment s;
@@ -784,11 +801,11 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         tma_prefetch_desc(&k_map);
         tma_prefetch_desc(&v_map);
     }
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();  // after the wait: cross_combine_kernel reads the lengths before its own
 
     auto len_of = [&](int obs) { return xa_len(p, obs); };
-    if (!LIST) xa_sort(p, order);
+    if (!LIST) xa_sort<XP_THREADS>(p, order);
     if (warp < XP_LOADER) xa_fill_empty<HD, LIST>(p, order, blockIdx.x >> 1, rank * 32 * XP_LOADER + threadIdx.x, 64 * XP_LOADER);
     XaWork<LIST, decltype(len_of)> work(len_of, p, order, blockIdx.x >> 1);
     XaSegment s;
@@ -1072,16 +1089,264 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     }
 }
 
+// ------------------------------------------------------------------ few query rows --
+// Units of up to 16 rows (a token, of every head of a group): K and V are read once and next to nothing is computed, so what counts is bytes in
+// flight and a short chain behind them.  Tiles of 128 or 256 rows would be empty for the most part, and TMEM, its allocation and the pair's
+// launch cost more than the products; 16 rows are what mma.sync (16 x 8 x 16) takes.  Measured: see cross_plan.
+//   loader warp   TMA: Q (16 rows), K and V in blocks of 64 rows, one barrier for both, running ahead over the segments
+//   4 warps       16 of a block's rows each, with a maximum, a sum and an O of their own; a warp zeroes its hidden rows of V itself.
+//                 A segment's end: their O meet in shared memory and are added by all
+constexpr int XF_ROWS = 16, XF_WARPS = 4, XF_THREADS = 32 * (XF_WARPS + 1), XF_BKV = 16 * XF_WARPS;
+
+template <int HD>
+struct CrossFewSmem {
+    static constexpr int CB = HD / 64, PER_SM = HD == 256 ? 1 : 2;                        // CTAs
+    static constexpr int STAGES = HD == 64 ? 4 : 2, QS = HD == 128 ? 1 : 2;               // blocks of K and V; segments' Q
+    static constexpr int Q_BYTES = CB * XF_ROWS * 128, KV_BYTES = CB * XF_BKV * 128;      // [CB][rows][128 B]
+    static constexpr int Q_OFF = STAGES * 2 * KV_BYTES, O_OFF = Q_OFF + QS * Q_BYTES, O_STRIDE = HD + 8;
+    static constexpr int ML_OFF = O_OFF + XF_WARPS * XF_ROWS * O_STRIDE * 4;              // float O [warp][row][O_STRIDE], float2 [warp][row]
+    static constexpr int BAR_OFF = ML_OFF + XF_WARPS * XF_ROWS * 8, ORDER_OFF = BAR_OFF + 128, TOTAL = ORDER_OFF + (int)sizeof(XaOrder) + 1024;
+    static_assert(ORDER_OFF % 16 == 0 && TOTAL <= 227 * 1024 && PER_SM * (TOTAL + 1024) <= 228 * 1024, "shared memory");
+};
+__device__ __forceinline__ void xf_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void xf_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void xf_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <int HD, bool LIST>
+__global__ void __launch_bounds__(XF_THREADS, CrossFewSmem<HD>::PER_SM)
+cross_few_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                 const CrossParams p) {
+    using L = CrossFewSmem<HD>;
+    constexpr uint32_t NS = L::STAGES, QS = L::QS;
+    extern __shared__ uint8_t xf_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(xf_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF);
+    uint64_t *full = bars, *free_ = bars + 4, *q_full = bars + 8, *q_free = bars + 10, *o_full = bars + 12, *o_free = bars + 13;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 14);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtx wc{abort_flag, p.status};
+    XaOrder &order = *reinterpret_cast<XaOrder *>(smem + L::ORDER_OFF);
+    if (!LIST) xa_sort_clear(order, XF_THREADS);
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < NS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&free_[i], XF_WARPS);
+        }
+        for (uint32_t i = 0; i < QS; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_free[i], XF_WARPS);
+        }
+        mbar_init(o_full, XF_WARPS);
+        mbar_init(o_free, XF_WARPS);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&q_map);
+        tma_prefetch_desc(&k_map);
+        tma_prefetch_desc(&v_map);
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();  // after the wait: cross_combine_kernel reads the lengths before its own
+    auto len_of = [&](int obs) { return xa_len(p, obs); };
+    if (!LIST) xa_sort<XF_THREADS>(p, order);
+    XaWork<LIST, decltype(len_of)> work(len_of, p, order, blockIdx.x);
+    XaSegment s;
+    bool ok = true;
+    uint32_t it = 0, si = 0;  // blocks of 64 rows and segments so far
+    auto begin_of = [&]() { return s.j0 * (XA_BKV / XF_BKV); };
+    auto end_of = [&]() { return min(s.j1 * (XA_BKV / XF_BKV), (s.len + XF_BKV - 1) / XF_BKV); };
+    if (warp == XF_WARPS) {
+        for (; ok && work.next(s); ++si) {
+            const int item = s.obs * p.n_kv + s.kvh;
+            const uint32_t qs = si % QS;
+            ok = warp_wait(&q_free[qs], (si / QS & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+            if (!ok) break;
+            if (elect_one()) {
+                mbar_expect_tx(&q_full[qs], L::Q_BYTES);
+                for (int cb = 0; cb < L::CB; ++cb)
+                    tma_load_3d(smem + L::Q_OFF + qs * L::Q_BYTES + cb * (XF_ROWS * 128), &q_map, &q_full[qs], cb * 64, 0, item);
+            }
+            const int end = end_of();
+            for (int i = begin_of(); i < end; ++i, ++it) {
+                const uint32_t st = it % NS;
+                ok = warp_wait(&free_[st], (it / NS & 1u) ^ 1u, wc, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                if (elect_one()) {
+                    uint8_t *stage = smem + st * (2 * L::KV_BYTES);
+                    mbar_expect_tx(&full[st], 2 * L::KV_BYTES);
+                    for (int cb = 0; cb < L::CB; ++cb) tma_load_3d(stage + cb * (XF_BKV * 128), &k_map, &full[st], cb * 64, i * XF_BKV, p.page0 + item);
+                    for (int cb = 0; cb < L::CB; ++cb)
+                        tma_load_3d(stage + L::KV_BYTES + cb * (XF_BKV * 128), &v_map, &full[st], cb * 64, i * XF_BKV, p.page0 + item);
+                }
+            }
+        }
+    } else {
+        const int r = lane >> 2, t = lane & 3;
+        float *const s_o = reinterpret_cast<float *>(smem + L::O_OFF);
+        float2 *const s_ml = reinterpret_cast<float2 *>(smem + L::ML_OFF);
+        // rows of the 8 x 8 matrices that this lane gives ldmatrix the addresses of, and which 16-byte chunk (swizzled by the row)
+        const int row_a = (lane & 7) + (lane >> 3 & 1) * 8, chunk_a = lane >> 4;  // A, and V transposed
+        const int row_b = (lane & 7) + (lane >> 4) * 8, chunk_b = lane >> 3 & 1;  // K
+        const int swz = lane & 7;
+        const uint32_t base = smem_u32(smem);
+        for (; ok && work.next(s); ++si) {
+            const uint32_t qs = si % QS;
+            ok = warp_wait(&q_full[qs], si / QS & 1u, wc, DEV_TIMEOUT_FULL);
+            if (!ok) break;
+            const uint32_t q_at = base + L::Q_OFF + qs * L::Q_BYTES + (uint32_t)(row_a * 128);
+            float acc[HD / 8][4];
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // of query rows r and r + 8; l: of this lane's columns
+            const int end = end_of();
+            for (int i = begin_of(); i < end; ++i, ++it) {
+                const uint32_t st = it % NS, k_at = base + st * (2 * L::KV_BYTES) + (uint32_t)(warp * 16 * 128), v_at = k_at + L::KV_BYTES;
+                ok = warp_wait(&full[st], it / NS & 1u, wc, DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                const int first = i * XF_BKV + warp * 16;
+                auto seen = [&](int row) { return row < s.len && (row < s.pad_lo || row >= s.pad_hi); };
+                const bool dirty = first + 16 > s.len || (first < s.pad_hi && first + 16 > s.pad_lo);
+                if (dirty) {  // hidden rows of V meet weights of 0, and 0 times what stands there need not be 0
+                    uint4 *v = reinterpret_cast<uint4 *>(smem + st * (2 * L::KV_BYTES) + L::KV_BYTES) + warp * 16 * 8;
+                    for (int n = lane; n < 16 * 8; n += 32)
+                        if (!seen(first + n / 8))
+                            for (int cb = 0; cb < L::CB; ++cb) v[cb * (XF_BKV * 8) + n] = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                float c[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    uint32_t a[4], b[4];
+                    xf_ldmatrix(a, q_at + (uint32_t)((kk >> 2) * (XF_ROWS * 128) + (((kk & 3) * 2 + chunk_a) ^ swz) * 16));
+                    xf_ldmatrix(b, k_at + (uint32_t)((kk >> 2) * (XF_BKV * 128) + row_b * 128 + (((kk & 3) * 2 + chunk_b) ^ swz) * 16));
+                    xf_mma(c[0], a, b[0], b[1]);
+                    xf_mma(c[1], a, b[2], b[3]);
+                }
+                // c[n][e]: query row r + 8 (e / 2), cached row first + 8 n + 2 t + e % 2
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[n][e] = !dirty || seen(first + 8 * n + 2 * t + (e & 1)) ? c[n][e] * p.scale_log2 : -INFINITY;
+                float f[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float top = fmaxf(fmaxf(c[0][2 * h], c[0][2 * h + 1]), fmaxf(c[1][2 * h], c[1][2 * h + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    top = fmaxf(top, m[h]);
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    f[h] = m[h] == -INFINITY ? 0.0f : xa_ex2(m[h] - ref);
+                    m[h] = top;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        c[n][2 * h] = xa_ex2(c[n][2 * h] - ref);
+                        c[n][2 * h + 1] = xa_ex2(c[n][2 * h + 1] - ref);
+                    }
+                    l[h] = l[h] * f[h] + ((c[0][2 * h] + c[0][2 * h + 1]) + (c[1][2 * h] + c[1][2 * h + 1]));
+                }
+                if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) {
+                        acc[n][0] *= f[0];
+                        acc[n][1] *= f[0];
+                        acc[n][2] *= f[1];
+                        acc[n][3] *= f[1];
+                    }
+                }
+                // weights are rounded to 8 bits for the product, their sum is not
+                const uint32_t w[4] = {f2_bf16(f2(c[0][0], c[0][1])), f2_bf16(f2(c[0][2], c[0][3])), f2_bf16(f2(c[1][0], c[1][1])),
+                                       f2_bf16(f2(c[1][2], c[1][3]))};
+#pragma unroll
+                for (int n = 0; n < HD / 16; ++n) {
+                    uint32_t b[4];
+                    xf_ldmatrix_t(b, v_at + (uint32_t)((n >> 2) * (XF_BKV * 128) + row_a * 128 + (((n & 3) * 2 + chunk_a) ^ swz) * 16));
+                    xf_mma(acc[2 * n], w, b[0], b[1]);
+                    xf_mma(acc[2 * n + 1], w, b[2], b[3]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&free_[st]);
+            }
+            if (!ok) break;
+            if (lane == 0) mbar_arrive(&q_free[qs]);
+            ok = warp_wait(o_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_MISC);  // the segment before has been read
+            if (!ok) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                if (t == 0) s_ml[warp * XF_ROWS + r + 8 * h] = make_float2(m[h], l[h]);
+                if (r + 8 * h < p.R) {
+                    float2 *o = reinterpret_cast<float2 *>(s_o + (warp * XF_ROWS + r + 8 * h) * L::O_STRIDE + 2 * t);
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) o[4 * n] = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_full);
+            ok = warp_wait(o_full, si & 1u, wc, DEV_TIMEOUT_MISC);
+            if (!ok) break;
+            for (int row = warp; row < p.R; row += XF_WARPS) {
+                float f[XF_WARPS], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < XF_WARPS; ++w) {
+                    f[w] = s_ml[w * XF_ROWS + row].x;
+                    top = fmaxf(top, f[w]);
+                }
+                F2 o[HD / 64];  // two columns in 64
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c) o[c] = f2(0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < XF_WARPS; ++w) {
+                    f[w] = f[w] == -INFINITY ? 0.0f : xa_ex2(f[w] - top);
+                    sum = fmaf(s_ml[w * XF_ROWS + row].y, f[w], sum);
+                    const float2 *x = reinterpret_cast<const float2 *>(s_o + (w * XF_ROWS + row) * L::O_STRIDE) + lane;
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c) o[c] = f2_fma(f2(x[32 * c].x, x[32 * c].y), f2(f[w], f[w]), o[c]);
+                }
+                if (LIST && s.slot >= 0) {
+                    const long long piece = (long long)s.slot * p.ws_rows + row;
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c) {
+                        float x, y;
+                        f2_get(o[c], x, y);
+                        reinterpret_cast<float2 *>(p.ws_o + piece * HD)[32 * c + lane] = make_float2(x, y);
+                    }
+                    if (lane == 0) *reinterpret_cast<float2 *>(p.ws_ml + piece * 2) = make_float2(top, sum);
+                    continue;
+                }
+                const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
+                uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + ((long long)s.obs * p.S * p.n_q + s.kvh * p.g + xa_place(p, row)) * HD) + lane;
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c) dst[32 * c] = f2_bf16(f2_mul(o[c], f2(inv, inv)));
+                if (p.lse && lane == 0)
+                    p.lse[((long long)s.obs * p.n_kv + s.kvh) * p.R + row] = sum == 0.0f ? -INFINITY : (top + xa_log2(sum)) * 0.6931471805599453f;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+        }
+        xa_fill_empty<HD, LIST>(p, order, blockIdx.x, threadIdx.x, 32 * XF_WARPS);
+    }
+    __syncthreads();
+}
+
 // Rows of units that were cut: M = max m_i, O = sum O_i 2^(m_i - M), l = sum l_i 2^(m_i - M), pieces in order.  Block x looks after unit x,
 // or, where there are more units than CTAs, after the one that CTA x began and did not finish.  TEAM warps share a row: 1 where a unit's rows
 // are many (two pieces or three of each), 32 where they are few and the pieces as many as there are CTAs (one token, 8 / 1 heads of 256,
-// over 16,001 rows, the whole call: 43 us with a warp per row, 24 so, 21 with the pages in L2).
+// over 16,001 rows, the whole call with tiles of 256 rows: 43 us with a warp per row, 24 so).
 template <int HD, int TEAM>
 __global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kernel(const CrossParams p) {
     constexpr int WARPS = TEAM > 1 ? TEAM : 8;
     __shared__ __align__(8) float s_o[WARPS][TEAM > 1 ? HD : 1], s_l[WARPS], s_m[WARPS];
     pdl_launch_dependents();
-    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int total = xa_total_blocks(p), n = min(p.n_work, total), upo = p.n_kv * p.n_mt;  // units of an observation
     if (total == 0) return;
@@ -1096,7 +1361,7 @@ __global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kern
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
         first = before * upo + u * nb;
-        c0 = (int)(((long long)(first + 1) * n - 1) / total);
+        c0 = xa_cta_of(first, n, total);
     } else {
         c0 = blockIdx.x;
         if (c0 >= n) return;
@@ -1111,8 +1376,9 @@ __global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kern
         first = end - 1 - at.block;
         if (first < begin) return;  // begun before this CTA
     }
-    const int c1 = (int)(((long long)(first + nb) * n - 1) / total);  // the CTA that has the unit's last block
+    const int c1 = xa_cta_of(first + nb - 1, n, total);  // the CTA that has the unit's last block
     if (c0 == c1) return;                                              // whole
+    pdl_wait();  // for the pieces; the lengths were complete before the kernel in front let this one begin
     const int kvh = u / p.n_mt, row0 = (u - kvh * p.n_mt) * p.unit_rows, rows = min(p.R - row0, p.unit_rows);
     constexpr int NV = HD / 64;  // pairs of columns per lane
     for (int r0 = blockIdx.y * (WARPS / TEAM); r0 < rows; r0 += gridDim.y * (WARPS / TEAM)) {
@@ -1201,41 +1467,54 @@ static int launch_combine(CrossParams p, cudaStream_t stream) {
 // Units, workers and workspace of a call; the same for the size query and the launch.
 struct CrossPlan {
     int unit_rows, n_mt, n_work, ws_rows;
+    bool few;            // up to 16 query rows: cross_few_kernel
     long long ws_bytes;  // 0: no unit is cut
 };
 static CrossPlan cross_plan(int hd, long long items, int R, int max_len, int n_sm) {
     CrossPlan c;
     c.unit_rows = 256;
     c.n_mt = (R + 255) / 256;
-    c.n_work = hd == 256 ? n_sm / 2 : n_sm;
+    c.few = R <= XF_ROWS;
+    c.n_work = c.few ? (hd == 256 ? CrossFewSmem<256>::PER_SM : hd == 128 ? CrossFewSmem<128>::PER_SM : CrossFewSmem<64>::PER_SM) * n_sm : hd == 256 ? n_sm / 2 : n_sm;
     c.ws_rows = R < 256 ? R : 256;
     // Whole units take rounds of n_work; cut ones fill the last round, for the pieces' way through the workspace and a second kernel: the
     // time of some 6 blocks, and of 10 more where the pieces are full tiles.  Cut / whole, us: one token of 8 / 1 heads of 256 over 16,001
-    // rows 21 / 176; 4 x 816 tokens of 20 / 5 heads of 128 over 4,097 to 8,190 rows 221 / 207; 64 x 51 tokens of 8 / 1 heads of 256 over
-    // 304 to 816 rows 55 / 37; 64 x 50 tokens of 15 / 5 heads of 64 over 113 to 241 rows 45 / 31.
+    // rows 21 / 233; 4 x 816 tokens of 20 / 5 heads of 128 over 4,097 to 8,190 rows 219 / 199; 64 x 51 tokens of 8 / 1 heads of 256 over
+    // 304 to 816 rows 55 / 37; 64 x 50 tokens of 15 / 5 heads of 64 over 113 to 241 rows 45 / 31.  Few rows: only where there are fewer units
+    // than CTAs (320 units of one token, heads of 128, 304 to 816 rows: 70 / 35).
+    // Few rows against tiles of 256 (cold / pages in L2): one token over 16,001 rows, heads of 256 20.5 / 14.6 against 24.6 / 20.4, of 128 24.6 /
+    // 16.6 against 30.7 / 23.8, of 64 20.5 / 13.6 against 26.7 / 20.8; 256 observations of 200 to 400 rows, heads of 256 30.8 / 19.1 against
+    // 36.9 / 28.9, of 128 55 / 44 against 68 / 60, of 64 36.9 / 28.9 against 57 / 55; 64 observations of 408 to 816 rows, heads of 256, the
+    // same (24.6 / 18.6 against 24.6 / 18.7).
     const long long units = items * c.n_mt, nb = (max_len + XA_BKV - 1) / XA_BKV, rounds = (units + c.n_work - 1) / c.n_work;
-    const bool cut = (rounds * c.n_work - units) * nb > (6LL + 10LL * c.ws_rows / 256) * c.n_work;
+    const bool cut = (!c.few || units < c.n_work) && (rounds * c.n_work - units) * nb > (6LL + 10LL * c.ws_rows / 256) * c.n_work;
     c.ws_bytes = cut ? 2LL * c.n_work * c.ws_rows * (hd + 2) * 4 : 0;
     return c;
 }
 
 template <int HD>
 static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &p, const CrossPlan &plan, cudaStream_t stream) {
+    const bool list = p.ws_o || p.n_obs > XA_SORT;
     const uint64_t pages = (uint64_t)st->n_layers * st->n_obs * st->n_kv;
     CUtensorMap qmap, kmap, vmap;
     const uint64_t qdims[3] = {(uint64_t)HD, (uint64_t)p.R, (uint64_t)st->n_obs * st->n_kv}, qstr[2] = {(uint64_t)HD * 2, (uint64_t)p.R * HD * 2};
     const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)(p.max_len > 0 ? p.max_len : 1), pages}, str[2] = {(uint64_t)HD * 2, (uint64_t)st->cap * HD * 2};
-    const uint32_t box[3] = {64, 128, 1}, kbox[3] = {64, HD == 256 ? 64 : 128, 1};  // a CTA of a pair stages half of a block's K rows
-    int rc = make_tensor_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, qdims, qstr, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint32_t few = XF_BKV, qbox[3] = {64, plan.few ? (uint32_t)XF_ROWS : 128u, 1}, vbox[3] = {64, plan.few ? few : 128u, 1};
+    const uint32_t kbox[3] = {64, plan.few ? few : HD == 256 ? 64u : 128u, 1};  // a CTA of a pair stages half of a block's K rows
+    int rc = make_tensor_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, qdims, qstr, qbox, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = make_tensor_map(&kmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->k_pages, dims, str, kbox, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_tensor_map(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, st->v_pages, dims, str, vbox, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    if constexpr (HD == 256) {
-        const auto kernel = p.ws_o || p.n_obs > XA_SORT ? cross_attn_pair_kernel<true> : cross_attn_pair_kernel<false>;
+    if (plan.few) {
+        const auto kernel = list ? cross_few_kernel<HD, true> : cross_few_kernel<HD, false>;
+        if ((rc = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), CrossFewSmem<HD>::TOTAL))) return rc;
+        rc = launch_pdl(kernel, dim3((unsigned)plan.n_work), dim3(XF_THREADS), CrossFewSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
+    } else if constexpr (HD == 256) {
+        const auto kernel = list ? cross_attn_pair_kernel<true> : cross_attn_pair_kernel<false>;
         if ((rc = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), CrossPairSmem::TOTAL))) return rc;
         rc = launch_pdl(kernel, dim3(2 * (unsigned)plan.n_work), dim3(XP_THREADS), CrossPairSmem::TOTAL, stream, qmap, kmap, vmap, p);
     } else {
-        const auto kernel = p.ws_o || p.n_obs > XA_SORT ? cross_attn_kernel<HD, true> : cross_attn_kernel<HD, false>;
+        const auto kernel = list ? cross_attn_kernel<HD, true> : cross_attn_kernel<HD, false>;
         if ((rc = ensure_dyn_smem(reinterpret_cast<const void *>(kernel), CrossSmem<HD>::TOTAL))) return rc;
         rc = launch_pdl(kernel, dim3((unsigned)plan.n_work), dim3(XA_THREADS), CrossSmem<HD>::TOTAL, stream, qmap, kmap, vmap, p);
     }
