@@ -337,7 +337,8 @@ __device__ __forceinline__ void xa_mask32(uint32_t (&x)[32], int c0, int len, in
 }
 
 // COLS columns of O of one row per thread, out of TMEM: divided and rounded to dst, or (ws) as they are.  The loads of 32 N columns are in flight
-// at once: one at a time 32 columns took 870 clocks.  `out_of_tmem` runs when all have been read.
+// at once (N = 2 at heads of 256; 64 and 128 have no registers for it: 64 x 50 tokens 20.7 us instead of 18.7).  `out_of_tmem` runs when all have
+// been read.
 template <int COLS, int N, typename F>
 __device__ __forceinline__ void xa_drain(uint32_t o_addr, bool row_ok, __nv_bfloat16 *dst, float inv, int al32, float *ws, F out_of_tmem) {
     const F2 inv2 = f2(inv, inv);
@@ -983,22 +984,26 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 tc_fence_before();
                 arrive_even(o_free);
             };
-            if (live) xa_drain<HD / 2, LIST ? 2 : 4>(tmem_base + lane_sel + (uint32_t)(half * (HD / 2)), row_ok, dst, inv, p.out_al32, wo, out_of_tmem);
+            if (live) xa_drain<HD / 2, 2>(tmem_base + lane_sel + (uint32_t)(half * (HD / 2)), row_ok, dst, inv, p.out_al32, wo, out_of_tmem);
             else out_of_tmem();
             return true;  // (the row-sum slots are next written after at least one more meeting of the pair)
         };
         XaSegment prev;
         float prev_m = 0.0f, prev_l = 0.0f;
-        for (; ok && work.next(s); ++si) {
+        for (bool here = true; ok && here; ++si) {
+            here = work.next(s);
+            if (!here) s.j0 = s.mt = 0, s.j1 = 1;  // behind the last segment: its drain alone, by the same instructions (a copy of them would not be cached)
             const int pad_lo = s.pad_lo, pad_hi = s.pad_hi;
-            const bool live = is_live(s);
+            const bool live = here && is_live(s);
             float m_used = -INFINITY, l_sum = 0.0f;  // running maximum in log2 units (the same in both halves), this half's part of the row sum
             for (int j = s.j0; j < s.j1; ++j, ++jb) {
                 const uint32_t sb = jb % NS;
                 const uint32_t s_addr = tmem_base + HD + sb * BKV + lane_sel;
-                ok = warp_wait(&s_full[sb], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
-                if (!ok) break;
-                tc_fence_after();
+                if (here) {
+                    ok = warp_wait(&s_full[sb], (jb / NS) & 1u, wc, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
                 if (live) {
                 uint32_t x[2][32];
                 tmem_ld32(s_addr + (uint32_t)(half * 64), x[0]);
@@ -1066,8 +1071,10 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 tmem_st32(s_addr + (uint32_t)(half * 32), pk);
                 tmem_st_wait();
                 }
-                tc_fence_before();
-                arrive_even(&p_full[sb]);
+                if (here) {
+                    tc_fence_before();
+                    arrive_even(&p_full[sb]);
+                }
                 if (j == s.j0 && si > 0) {
                     ok = drain(si - 1, prev, prev_m, prev_l);
                     if (!ok) break;
@@ -1078,7 +1085,6 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             prev_m = m_used;
             prev_l = l_sum;
         }
-        if (ok && si > 0) ok = drain(si - 1, prev, prev_m, prev_l);
     }
     tc_fence_before();
     __syncthreads();
