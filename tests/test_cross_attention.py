@@ -65,6 +65,10 @@ CASES = [
     (150, 1, 8, 1, 256, 700, None, True),
     (160, 2, 4, 2, 128, 500, None, False),
     (150, 2, 1, 1, 64, 8300, None, True),               # more blocks than the sort has bins
+    (40, 1, 3, 3, 64, 3000, None, True),                # cut units of more than 32 observations
+    (20, 260, 4, 4, 64, 2600, None, True),              # cut, and more units than CTAs
+    (40, 40, 8, 2, 256, 2400, None, True),
+    (100, 17, 2, 2, 128, 2500, None, True),
 ]
 
 
