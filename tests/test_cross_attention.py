@@ -200,3 +200,20 @@ def test_refusals():
         with pytest.raises(vb.VlaB200Error) as e:
             vb.cross_attention(st, kw.pop("layer"), kw.pop("q"), **kw)
         assert e.value.code == -1, kw
+
+
+def test_no_block_leaves_before_it_has_waited():
+    """A block that ends without griddepcontrol.wait lets the next kernel take this one's end for the end of the one in front, whose results it
+    may then read too early: no kernel that waits returns before it does."""
+    import glob
+    import os
+
+    from tests.test_dependent_launch_sources import CSRC, functions, strip_comments
+
+    waiting = 0
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu"))):
+        for name, _, body in functions(strip_comments(open(path).read()), r"__global__"):
+            if "pdl_wait" in body:
+                waiting += 1
+                assert "return;" not in body[:body.index("pdl_wait")], f"{os.path.basename(path)}: {name}"
+    assert waiting > 20

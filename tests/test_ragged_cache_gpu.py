@@ -128,6 +128,86 @@ def test_captured_replayed_and_on_two_streams():
     assert vb.device_status() == 0
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_one_token_replayed_while_the_cache_grows(hd):
+    """A captured step -- rotate and append at row0, attend over row0 + 1 rows -- replayed as the lengths move on, against the calls."""
+    torch = require_cuda()
+    import vla_cpp_b200 as vb
+
+    B, n_q, n_kv, cap = 3, 8, 2, 4000
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    st, other = vb.KvStore(1, B, n_kv, hd, 0, cap), vb.KvStore(1, B, n_kv, hd, 0, cap)
+    for t in (st.k, st.v):
+        t.normal_(0, 1, generator=g)
+    other.k.copy_(st.k)
+    other.v.copy_(st.v)
+    freqs, m = vb.rope_freqs(hd)
+    x = torch.empty(B, (n_q + 2 * n_kv) * hd, dtype=torch.bfloat16, device="cuda")
+    row0, lens = (torch.zeros(B, dtype=torch.int32, device="cuda") for _ in range(2))
+    mass = torch.zeros(B, n_kv, cap, device="cuda")
+
+    def step(store, weights):
+        q = vb.qk_norm_rope_append(store, 0, x, 1, n_q, freqs, row0=row0)
+        out, lse = vb.cross_attention(store, 0, q, lens=lens)
+        vb.key_mass(store, 0, q, lse, lens=lens, mass=weights, out=weights)
+        return out, lse
+
+    x.zero_()
+    for store in (st, other):  # the first call is not captured; it writes row 0 of both
+        step(store, mass.clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(st, mass)
+    mine = torch.zeros_like(mass)
+    for at in ([0, 0, 63], [1, 64, 64], [127, 128, 700], [3999, 1, 2047], [3999, 3998, 3997]):
+        x.normal_(0, 1, generator=g)
+        row0.copy_(torch.tensor(at, dtype=torch.int32))
+        lens.copy_(row0 + 1)
+        if at == [1, 64, 64]:
+            lens[0] = 0  # an idle observation
+        graph.replay()
+        want = step(other, mine)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(mass, mine)
+        assert torch.equal(st.k, other.k) and torch.equal(st.v, other.v)
+        seen = torch.arange(cap, device="cuda")[None] < lens[:, None]
+        q = vb.qk_norm_rope_append(other, 0, x, 1, n_q, freqs, row0=row0)
+        z = (q.double().reshape(B, n_kv, -1, hd) @ other.k[0].double().transpose(-1, -2) * hd ** -0.5).masked_fill(~seen[:, None, None], -float("inf"))
+        ref = torch.logsumexp(z, -1).reshape(B, n_q, 1)
+        assert torch.equal(ref == -float("inf"), got[1] == -float("inf"))
+        torch.testing.assert_close(got[1].double().nan_to_num(neginf=0), ref.nan_to_num(neginf=0), rtol=1e-5, atol=1e-5)
+    assert vb.device_status() == 0
+
+
+@pytest.mark.parametrize("hd,S", [(64, 1), (128, 40), (256, 1)])
+def test_what_follows_a_call_whose_pieces_are_all_whole(hd, S):
+    """max_len asks for cut units, the lengths leave none cut: nothing to merge, and the next call still sees what the first one wrote."""
+    torch = require_cuda()
+    import vla_cpp_b200 as vb
+
+    B, n_q, n_kv, cap = 20, 6, 2, 6000
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    st = vb.KvStore(1, B, n_kv, hd, 0, cap)
+    st.k.normal_(0, 1, generator=g)
+    st.v.normal_(0, 1, generator=g)
+    q = torch.randn(B, n_q, S, hd, device="cuda", generator=g).bfloat16()
+    lens = torch.full((B,), 128, dtype=torch.int32, device="cuda")
+    out, lse = vb.cross_attention(st, 0, q, lens=lens)
+    torch.cuda.synchronize()
+    want = vb.key_mass(st, 0, q, lse, lens=lens)
+    mass = torch.zeros_like(want)
+    again = torch.empty_like(lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        vb.cross_attention(st, 0, q, lens=lens, out=out, lse=again)
+        vb.key_mass(st, 0, q, again, lens=lens, out=mass)
+    for _ in range(20):
+        again.fill_(3.0)
+        mass.zero_()
+        graph.replay()
+        assert torch.equal(again, lse) and torch.equal(mass, want)
+    assert vb.device_status() == 0
+
+
 def test_denoise_attention_over_an_evicted_cache():
     """The isolated denoise-attention op runs on the smaller store, its action tokens at their old positions."""
     torch = require_cuda()

@@ -1355,36 +1355,37 @@ __global__ void __launch_bounds__(TEAM > 1 ? 32 * TEAM : 256) cross_combine_kern
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int total = xa_total_blocks(p), n = min(p.n_work, total), upo = p.n_kv * p.n_mt;  // units of an observation
-    if (total == 0) return;
-    int obs, u, nb, first, c0;  // the unit's observation, place in it and blocks; its first block in the list, the CTA that has that one
-    if (p.by_unit) {
-        obs = blockIdx.x / upo;
-        u = blockIdx.x - obs * upo;
-        nb = (xa_len(p, obs) + XA_BKV - 1) / XA_BKV;
-        if (nb == 0) return;
-        int before = 0;
-        for (int i = lane; i < obs; i += 32) before += (xa_len(p, i) + XA_BKV - 1) / XA_BKV;
+    int obs = 0, u = 0, nb = 0, first = 0, c0 = 0, c1 = 0;  // the unit's observation, place in it and blocks; its first block in the list, the
+    if (total > 0) {                                        // CTAs that have that one and the last (the same one: whole, nothing to merge)
+        if (p.by_unit) {
+            obs = blockIdx.x / upo;
+            u = blockIdx.x - obs * upo;
+            nb = (xa_len(p, obs) + XA_BKV - 1) / XA_BKV;
+            int before = 0;
+            for (int i = lane; i < obs; i += 32) before += (xa_len(p, i) + XA_BKV - 1) / XA_BKV;
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
-        first = before * upo + u * nb;
-        c0 = xa_cta_of(first, n, total);
-    } else {
-        c0 = blockIdx.x;
-        if (c0 >= n) return;
-        const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
-        auto len_of = [&](int i) { return xa_len(p, i); };
-        RaggedCursor cur(len_of, p.n_obs, upo, XA_BKV);
-        RaggedUnit at;
-        if (!cur.find(end - 1, at)) return;
-        obs = at.obs;
-        u = at.kvh;
-        nb = (at.len + XA_BKV - 1) / XA_BKV;
-        first = end - 1 - at.block;
-        if (first < begin) return;  // begun before this CTA
+            for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+            first = before * upo + u * nb;
+            if (nb > 0) c0 = xa_cta_of(first, n, total);
+        } else if ((int)blockIdx.x < n) {
+            c0 = blockIdx.x;
+            const int begin = xa_border(c0, n, total), end = xa_border(c0 + 1, n, total);
+            auto len_of = [&](int i) { return xa_len(p, i); };
+            RaggedCursor cur(len_of, p.n_obs, upo, XA_BKV);
+            RaggedUnit at;
+            if (cur.find(end - 1, at) && end - 1 - at.block >= begin) {  // (begun before this CTA: the one that began it merges it)
+                obs = at.obs;
+                u = at.kvh;
+                nb = (at.len + XA_BKV - 1) / XA_BKV;
+                first = end - 1 - at.block;
+            }
+        }
+        c1 = nb > 0 ? xa_cta_of(first + nb - 1, n, total) : c0;
     }
-    const int c1 = xa_cta_of(first + nb - 1, n, total);  // the CTA that has the unit's last block
-    if (c0 == c1) return;                                              // whole
-    pdl_wait();  // for the pieces; the lengths were complete before the kernel in front let this one begin
+    // For the pieces; the lengths were complete before the kernel in front let this one begin.  Every block waits, those without work too: who
+    // follows this kernel takes its end for the end of the one in front.
+    pdl_wait();
+    if (c0 == c1) return;
     const int kvh = u / p.n_mt, row0 = (u - kvh * p.n_mt) * p.unit_rows, rows = min(p.R - row0, p.unit_rows);
     constexpr int NV = HD / 64;  // pairs of columns per lane
     for (int r0 = blockIdx.y * (WARPS / TEAM); r0 < rows; r0 += gridDim.y * (WARPS / TEAM)) {
