@@ -5,6 +5,7 @@ library's kernels.  Argument meaning and error behaviour follow the reference en
 points named in include/vla_b200.h.
 """
 import ctypes as C
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -396,6 +397,18 @@ def _ragged_args(store, q, lens, max_len, pad_ranges):
     return dev, S, n_q, store.cap if max_len is None else max_len
 
 
+@functools.lru_cache(maxsize=1024)
+def _cross_ws_bytes(dev, n_obs, n_kv, head_dim, cap, S, n_q, max_len):
+    """vlab200_cross_attention_ws_bytes, asked once per shape (1 us of a call's 14); it depends on nothing else."""
+    import torch
+
+    with torch.cuda.device(dev):
+        n = lib().vlab200_cross_attention_ws_bytes(C.byref(_KvStoreC(None, None, 1, n_obs, n_kv, head_dim, cap, 0)), S, n_q, max_len)
+    if n < 0:  # (an exception is not kept)
+        raise VlaB200Error(ERR_ARG, f"cross_attention: {n_q} query heads on {n_kv} kv heads, {S} tokens, {max_len} rows")
+    return n
+
+
 def cross_attention(store, layer, q, lens=None, max_len=None, pad_ranges=None, scale=None, out=None, lse=None, split=True):
     """Attention of query tokens to each observation's own number of cached rows -> (out, lse).
 
@@ -415,13 +428,7 @@ def cross_attention(store, layer, q, lens=None, max_len=None, pad_ranges=None, s
         _need_tensor(lse, "lse", torch.float32, (store.n_obs, n_q, S), dev)
     ws, n = None, 0
     if split:
-        if torch.cuda.current_device() == dev:
-            n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q, max_len)
-        else:
-            with torch.cuda.device(dev):
-                n = lib().vlab200_cross_attention_ws_bytes(C.byref(store.c), S, n_q, max_len)
-        if n < 0:
-            raise VlaB200Error(ERR_ARG, f"cross_attention: {n_q} query heads on {store.n_kv} kv heads, {S} tokens, {max_len} rows")
+        n = _cross_ws_bytes(dev, store.n_obs, store.n_kv, store.head_dim, store.cap, S, n_q, max_len)
         if n > 0:
             ws = _new((n,), torch.uint8, q.device)
     _call_on(dev, lib().vlab200_cross_attention, "vlab200_cross_attention", C.byref(store.c), layer, q.data_ptr(), out.data_ptr(),
