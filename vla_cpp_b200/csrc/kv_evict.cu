@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(KE_THREADS) kv_evict_select_kernel(const Evict
         }
     }
     // kept rows in order: those above the keep-th key, and the first `left` of its equals
-    int done = 0, equals = 0;  // kept rows and rows equal to it in front of this round
+    int done = 0, equals = 0;  // kept rows and rows equal to it in front of these
     for (int r0 = 0; r0 < len; r0 += KE_THREADS) {
         const int r = r0 + tid;
         bool above = false, equal = false;
