@@ -734,8 +734,9 @@ struct CrossPairSmem {
     static constexpr int STAGES = 2, NS = 2;
     static constexpr int Q_BYTES = CB * 128 * 128, K_BYTES = CB * 64 * 128, V_BYTES = CBH * 128 * 128;
     static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + STAGES * K_BYTES, BAR_OFF = V_OFF + STAGES * V_BYTES;
-    static constexpr int XCH_OFF = BAR_OFF + 256;  // float [2][2 halves][128]: block maxima, used in turn; then the row sums
-    static constexpr int ORDER_OFF = XCH_OFF + 3 * 2 * 128 * 4, TOTAL = ORDER_OFF + (int)sizeof(XaOrder) + 1024;
+    static constexpr int SUM_SETS = 2;             // of row-sum slots
+    static constexpr int XCH_OFF = BAR_OFF + 256;  // float [2][2 halves][128]: block maxima, used in turn; then [SUM_SETS][2 halves][128]: row sums
+    static constexpr int ORDER_OFF = XCH_OFF + (2 + SUM_SETS) * 2 * 128 * 4, TOTAL = ORDER_OFF + (int)sizeof(XaOrder) + 1024;
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -961,9 +962,12 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             float inv = 0.0f, *wo = nullptr;
             __nv_bfloat16 *dst = nullptr;
             if (live) {  // while the last P V runs
-                xch[512 + half * 128 + my_slot] = l_mine;
+                // Two sets of slots, used in turn.  One was not enough: a last segment of one block is drained right behind the drain before
+                // it, and a warp could write its sum while the other, late out of their meeting, had yet to read the one that stood there.
+                float *sums = xch + 512 + (u % L::SUM_SETS) * 256;
+                sums[half * 128 + my_slot] = l_mine;
                 if (!pair_sync()) return false;
-                const float l = l_mine + xch[512 + (half ^ 1) * 128 + my_slot];
+                const float l = l_mine + sums[(half ^ 1) * 128 + my_slot];
                 if (sg.mt != mt_of_place) {
                     mt_of_place = sg.mt;
                     place = xa_place(p, row);
@@ -986,7 +990,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             };
             if (live) xa_drain<HD / 2, 2>(tmem_base + lane_sel + (uint32_t)(half * (HD / 2)), row_ok, dst, inv, p.out_al32, wo, out_of_tmem);
             else out_of_tmem();
-            return true;  // (the row-sum slots are next written after at least one more meeting of the pair)
+            return true;  // (this set is next written behind segment u + 1's meeting, or that of segment u + 2's first block)
         };
         XaSegment prev;
         float prev_m = 0.0f, prev_l = 0.0f;
