@@ -68,7 +68,7 @@ def test_one_set_is_not_enough():
     assert unordered(events([(3, True), (2, True)]), 1) == []
 
 
-@pytest.mark.parametrize("path,struct,with_empty", [("cross_attn.cu", "CrossPairSmem", True)])
+@pytest.mark.parametrize("path,struct,with_empty", [("cross_attn.cu", "CrossPairSmem", True), ("attn_flash.cu", "FlashPairSmem", False)])
 def test_every_write_is_behind_a_meeting(path, struct, with_empty):
     sets = sets_of(path, struct)
     for segments in sequences(with_empty):
@@ -100,3 +100,29 @@ def test_segments_of_one_block(B, S, n_q, n_kv, cap, lens):
         for _ in range(20):
             again = vb.cross_attention(st, 0, q, lens=lens, split=split)
             assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,rows", [(256, 128), (256, 100), (128, 97), (256, 129)])
+def test_units_of_one_key_block(hd, rows):
+    """vlab200_attention over CTA pairs that each walk several units of one block.  Bound: one bf16 rounding of the value, one of each weight
+    (2^-8 each), and 2^-16 of the weighted |v| for all that is done in 32 bits (scores up to 2^5, a few hundred additions: below 2^-17)."""
+    from tests.gpu_util import require_cuda
+
+    torch = require_cuda()
+    import vla_cpp_b200 as vb
+
+    B, n_q, S = 190, 4, 50  # 200 rows: two tiles, 190 units on 74 pairs
+    g = torch.Generator(device="cuda").manual_seed(hd + rows)
+    st = vb.KvStore(1, B, 1, hd, rows, 0)
+    st.k.normal_(0, 1, generator=g)
+    st.v.normal_(0, 1, generator=g)
+    q = (torch.randn(B, n_q, S, hd, device="cuda", generator=g) * torch.linspace(0.1, 1.5, B, device="cuda")[:, None, None, None]).bfloat16()
+    out = vb.attention(st, 0, q, S, n_q, rows, vb.MASK_NONE)
+    p = torch.softmax(q.double() @ st.k[0].double().transpose(-1, -2) * hd ** -0.5, -1)
+    fold = lambda t: t.transpose(1, 2).reshape(B, S, n_q * hd)
+    want, size = fold(p @ st.v[0].double()), fold(p @ st.v[0].double().abs())
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -16) * size).all())
+    for _ in range(20):
+        assert torch.equal(vb.attention(st, 0, q, S, n_q, rows, vb.MASK_NONE), out)
+    assert vb.device_status() == 0

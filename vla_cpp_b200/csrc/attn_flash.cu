@@ -413,8 +413,9 @@ struct FlashPairSmem {
     static constexpr int V_BYTES = CBH * FP_BKV * 128;       // [CBH][128 keys][128 B]: this CTA's half of the head dimension
     static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + STAGES * K_BYTES;
     static constexpr int BAR_OFF = V_OFF + STAGES * V_BYTES;
-    static constexpr int XCH_OFF = BAR_OFF + 512;      // float [2 halves][128 rows] block maxima, then row sums, then the maxima of odd blocks
-    static constexpr int TOTAL = XCH_OFF + 3072 + 1024;
+    static constexpr int SUM_SETS = 2;                 // of row-sum slots
+    static constexpr int XCH_OFF = BAR_OFF + 512;      // float [2 sets, used in turn][block maxima, then row sums][2 halves][128 rows]
+    static constexpr int TOTAL = XCH_OFF + SUM_SETS * 2048 + 1024;
     static constexpr int O_COLS = HD;
     static constexpr int TMEM_COLS = 512;              // O [0, HD), then NS S buffers of 128 columns
     static_assert(HD + NS * FP_BKV <= 512 && NS >= 2, "TMEM");
@@ -654,11 +655,14 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         // The O drain of a unit runs AFTER the first S block of the next unit: that block only needs its S buffer, and the
         // ~2000 cycles between a unit's last P and "O complete" (its last P V) are spent on it instead of on waiting.
         auto drain = [&](uint32_t u, float l_mine, __nv_bfloat16 *dst, bool row_ok) -> bool {
-            xch[256 + half * 128 + my_slot] = l_mine;
+            // Two sets of slots, used in turn: with a single key block the last unit is drained right behind the drain before it, and a
+            // warp could write its sum while the other, late out of their meeting, had yet to read the one that stood there.
+            float *sums = xch + 256 + (u % L::SUM_SETS) * 512;
+            sums[half * 128 + my_slot] = l_mine;
             if (!mbar_wait(o_done, u & 1u, wc, DEV_TIMEOUT_ACCUM)) return false;
             tc_fence_after();
             if (!pair_sync()) return false;
-            const float inv = 1.0f / (l_mine + xch[256 + (half ^ 1) * 128 + my_slot]);
+            const float inv = 1.0f / (l_mine + sums[(half ^ 1) * 128 + my_slot]);
             for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                 uint32_t ov[32];
                 tmem_ld32(tmem_base + lane_sel + (uint32_t)c, ov);
@@ -688,7 +692,7 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     }
                 }
             }
-            // (the row-sum slots are next written after at least two more meetings of the pair)
+            // (this set is next written behind unit u + 1's meeting here)
             return true;
         };
         uint32_t ui = 0, jb = 0;
