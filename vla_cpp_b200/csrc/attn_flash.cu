@@ -437,7 +437,7 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     uint64_t *pair_bar = bars + 32;  // [4] the two softmax warps of a lane quarter meet here (64 arrivals)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 36);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    volatile uint32_t *pv_issued = reinterpret_cast<volatile uint32_t *>(tmem_slot + 2);  // P V blocks issued so far (even CTA)
+    uint32_t *pv_issued = tmem_slot + 2;  // P V blocks issued so far (even CTA)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -551,9 +551,9 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             // ~500 cycles between the block's last MMA and the moment this thread saw the barrier flip.
             auto ready_s = [&](uint32_t jbx) -> bool {
                 bool r = mbar_wait(&k_full[jbx % FP_STAGES], (jbx / FP_STAGES) & 1u, wc, DEV_TIMEOUT_FULL);
-                if (r && jbx >= FP_NS && *pv_issued < jbx - FP_NS + 1u) {
+                if (r && jbx >= FP_NS && ld_acquire_cta(pv_issued) < jbx - FP_NS + 1u) {
                     const long long t0 = clock64();
-                    for (uint32_t it = 1; *pv_issued < jbx - FP_NS + 1u; ++it) {
+                    for (uint32_t it = 1; ld_acquire_cta(pv_issued) < jbx - FP_NS + 1u; ++it) {
                         if ((it & 63u) == 0) {
                             if (*abort_flag) return false;
                             if (clock64() - t0 > wc.budget) {
@@ -620,7 +620,8 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                         for (int k16 = 0; k16 < FP_BKV / 16; ++k16)
                             mma_f16_tmem_a_pair(tmem_base, p_tmem + (uint32_t)(k16 * 8), v_desc + (uint64_t)(k16 * 128), idesc_o,
                                                 (j | k16) != 0 ? 1u : 0u);
-                        *pv_issued = jb + 1u;
+                        tc_fence_before();
+                        st_release_cta(pv_issued, jb + 1u);
                         tc_commit_pair(&pv_done[sb], 3);
                         tc_commit_pair(&v_free[st], 3);
                     }

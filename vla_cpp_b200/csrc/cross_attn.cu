@@ -757,7 +757,7 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     uint64_t *v_raw = bars + 22;                                                               // [ST]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    volatile uint32_t *pv_issued = reinterpret_cast<volatile uint32_t *>(tmem_slot + 2);  // P V blocks issued so far (even CTA)
+    uint32_t *pv_issued = tmem_slot + 2;  // P V blocks issued so far (even CTA)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const WaitCtx wc{abort_flag, p.status};
@@ -858,9 +858,9 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
                     ok = warp_wait(&k_full[jb % ST], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
                     // the P V of the block that used this S buffer has to be in the pipe
-                    if (ok && jb >= NS && *pv_issued < jb - NS + 1u) {
+                    if (ok && jb >= NS && ld_acquire_cta(pv_issued) < jb - NS + 1u) {
                         const long long t0 = clock64();
-                        for (uint32_t it = 1; *pv_issued < jb - NS + 1u; ++it) {
+                        for (uint32_t it = 1; ld_acquire_cta(pv_issued) < jb - NS + 1u; ++it) {
                             if ((it & 63u) == 0) {
                                 if (*abort_flag) {
                                     ok = false;
@@ -926,7 +926,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                         for (int kk = 0; kk < BKV / 16; ++kk)
                             mma_f16_tmem_a_pair(tmem_base, p_tmem + (uint32_t)(kk * 8), v_desc + (uint64_t)(kk * 128), idesc_o,
                                                 j != s.j0 || kk != 0 ? 1u : 0u);
-                        *pv_issued = jb + 1u;
+                        tc_fence_before();
+                        st_release_cta(pv_issued, jb + 1u);
                         tc_commit_pair(&pv_done[sb], 3);
                         tc_commit_pair(&v_free[st], 3);
                         if (j + 1 == s.j1) tc_commit_pair(o_done, 3);
