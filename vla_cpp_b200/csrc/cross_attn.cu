@@ -1230,7 +1230,6 @@ cross_few_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     for (int n = lane; n < 16 * 8; n += 32)
                         if (!seen(first + n / 8))
                             for (int cb = 0; cb < L::CB; ++cb) v[cb * (XF_BKV * 8) + n] = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
                     __syncwarp();
                 }
                 float c[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -1283,11 +1282,14 @@ cross_few_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     xf_mma(acc[2 * n], w, b[0], b[1]);
                     xf_mma(acc[2 * n + 1], w, b[2], b[3]);
                 }
+                // What this lane read of the stage (and of Q), and the zeros it wrote, come before the fill that follows the arrival; the reads have
+                // arrived, the products in front of the fence take them.
+                fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&free_[st]);
             }
             if (!ok) break;
-            if (lane == 0) mbar_arrive(&q_free[qs]);
+            if (lane == 0) mbar_arrive(&q_free[qs]);  // (fenced with the segment's last block; a segment has at least one)
             ok = warp_wait(o_free, (si & 1u) ^ 1u, wc, DEV_TIMEOUT_MISC);  // the segment before has been read
             if (!ok) break;
 #pragma unroll
