@@ -224,7 +224,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
 #pragma unroll
             for (int i = 0; i < NBLK; ++i) {
                 const int r = c * L::NQ + sub * 128 + i * 32 + lane;
-                lv[i] = there && c < p.n_chunks && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : INFINITY;
+                lv[i] = there && c < p.n_chunks && r < p.R ? p.lse[(long long)(u.obs * p.n_kv + u.kvh) * p.R + r] : -INFINITY;
             }
         };
         const bool alone = PPC == 1 && p.n_chunks == 1;
@@ -247,10 +247,16 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
             if (rel >= p.n_chunks) fetch_lse(there, unit, rel_next);
             for (int c = rel; c < p.n_chunks; c += G) {
                 const uint32_t q = qu + (uint32_t)c, ab = q % L::NB;
-                // rows past the last, and rows that saw nothing (-inf), weigh nothing: 2^(s - inf)
+                // Rows past the last, and rows that saw nothing (-inf), weigh nothing: 2^(0 - inf).  Their scores may be anything (a column that
+                // no row stands behind, a query that nobody wrote), so they are taken as 0: lane i keeps which ones of 32-column block i.
+                unsigned unseen = 0;
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < NBLK; ++i) ls[i * 32 + lane] = lv[i] == -INFINITY ? -INFINITY : -1.4426950408889634f * lv[i];
+                for (int i = 0; i < NBLK; ++i) {
+                    const unsigned of_block = __ballot_sync(0xffffffffu, lv[i] == -INFINITY);
+                    unseen = lane == i ? of_block : unseen;
+                    ls[i * 32 + lane] = lv[i] == -INFINITY ? -INFINITY : -1.4426950408889634f * lv[i];
+                }
                 __syncwarp();
                 if (c + G < p.n_chunks) fetch_lse(true, now, c + G);
                 else fetch_lse(there, unit, rel_next);
@@ -275,9 +281,10 @@ key_mass_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                         }
                     }
                     if (b * 32 >= n) continue;
-                    if (n < b * 32 + 32) {  // columns that no row stands behind hold anything
+                    const unsigned none = __shfl_sync(0xffffffffu, unseen, b);
+                    if (none) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = b * 32 + e < n ? s[e] : 0u;
+                        for (int e = 0; e < 32; ++e) s[e] = none & (1u << e) ? 0u : s[e];
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
