@@ -1536,6 +1536,12 @@ static int launch_cross(const vlab200_kv_store *st, const void *q, CrossParams &
     return launch_combine<HD>(p, stream);
 }
 
+// More query rows per kv head, pages or blocks of 256 x 128 scores than are counted in 32 bits?
+static bool cross_too_large(const vlab200_kv_store *st, int S, int n_q, int max_len) {
+    const long long R = (long long)(n_q / st->n_kv) * S;
+    return R > 0x7fffff00LL || size_product({st->n_obs, st->n_kv, st->n_layers}) > 0x7fffff00LL ||
+           size_product({st->n_obs, st->n_kv, (R + 255) / 256, (max_len + 127LL) / 128}) > 0x7fffff00LL;
+}
 static bool cross_shape_ok(const vlab200_kv_store *st, int S, int n_q) {
     return st && st->n_layers > 0 && st->n_obs > 0 && st->n_kv > 0 && st->cap > 0 && S > 0 && n_q > 0 && n_q % st->n_kv == 0;
 }
@@ -1545,7 +1551,7 @@ static bool cross_shape_ok(const vlab200_kv_store *st, int S, int n_q) {
 extern "C" {
 
 int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q, int32_t max_len) {
-    if (!vb::cross_shape_ok(st, S, n_q) || max_len < 0 || max_len > st->cap || (long long)(n_q / st->n_kv) * S > 0x7fffff00LL) return -1;
+    if (!vb::cross_shape_ok(st, S, n_q) || max_len < 0 || max_len > st->cap || vb::cross_too_large(st, S, n_q, max_len)) return -1;
     const int n_sm = vb::sm_count();
     return n_sm ? vb::cross_plan(st->head_dim, (long long)st->n_obs * st->n_kv, (n_q / st->n_kv) * S, max_len, n_sm).ws_bytes : -1;
 }
@@ -1560,13 +1566,12 @@ int32_t vlab200_cross_attention(const vlab200_kv_store *st, int32_t layer, const
     if ((al & 15) || (reinterpret_cast<uintptr_t>(ws) & 31)) return VLAB200_ERR_ARG;
     const int hd = st->head_dim;
     if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
-    const long long R = (long long)(n_q / st->n_kv) * S, items = (long long)st->n_obs * st->n_kv;
-    const long long blocks = items * ((R + 255) / 256) * ((max_len + 127LL) / 128);
-    if (R > 0x7fffff00LL || items * st->n_layers > 0x7fffff00LL || blocks > 0x7fffff00LL) {
+    if (vb::cross_too_large(st, S, n_q, max_len)) {
         vb::set_last_error("cross_attention: more than 2^31 query rows per kv head, pages or blocks of 256 x 128 scores");
         return VLAB200_ERR_UNSUPPORTED;
     }
-    const long long q_b = items * R * hd * 2, pages_b = (long long)st->n_layers * items * st->cap * hd * 2;
+    const long long R = (long long)(n_q / st->n_kv) * S, items = (long long)st->n_obs * st->n_kv;
+    const long long q_b = vb::size_product({items, R, hd, 2}), pages_b = vb::size_product({st->n_layers, items, st->cap, hd, 2});
     const vb::MemRange written[] = {{out, q_b}, {lse, items * R * 4}, {ws, ws_bytes}};
     const vb::MemRange read[] = {{q, q_b}, {st->k_pages, pages_b}, {st->v_pages, pages_b}, {lens, st->n_obs * 4LL}, {pad_ranges, st->n_obs * 8LL}};
     if (vb::writes_overlap(written, 3, read, 5)) return VLAB200_ERR_ARG;

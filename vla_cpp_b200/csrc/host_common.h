@@ -3,7 +3,9 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <climits>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/vla_b200.h"
 
@@ -83,6 +85,17 @@ static inline int launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 b
 // How many clusters of `cluster` CTAs of a kernel (its shared memory already opted into) the current device holds at once; 0 on failure.
 // Asked of the driver once per (device, kernel, cluster).
 int max_active_clusters(const void *kernel, int threads, int smem, int cluster);
+
+// Product of sizes (none negative); LLONG_MAX where it does not fit.
+inline long long size_product(std::initializer_list<long long> sizes) {
+    bool fits = true;
+    long long n = 1;
+    for (const long long s : sizes) {
+        if (s == 0) return 0;
+        fits = fits && !__builtin_mul_overflow(n, s, &n);
+    }
+    return fits ? n : LLONG_MAX;
+}
 
 // Device memory a call reads or writes; a null pointer or no bytes overlap nothing.
 struct MemRange {

@@ -377,15 +377,15 @@ extern "C" int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, c
     if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(st->k_pages) & 15)) return VLAB200_ERR_ARG;
     const int hd = st->head_dim;
     if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
-    const long long R = (long long)(n_q / st->n_kv) * S, tiles = (max_len + 255LL) / 256, units = (long long)st->n_obs * st->n_kv * tiles;
-    if (R > 0x7fffff00LL || units > 0x7fffff00LL || (long long)st->n_layers * st->n_obs * st->n_kv > 0x7fffff00LL) {
+    const long long R = (long long)(n_q / st->n_kv) * S, tiles = (max_len + 255LL) / 256, units = vb::size_product({st->n_obs, st->n_kv, tiles});
+    if (R > 0x7fffff00LL || units > 0x7fffff00LL || vb::size_product({st->n_layers, st->n_obs, st->n_kv}) > 0x7fffff00LL) {
         vb::set_last_error("key_mass: more than 2^31 query rows per kv head, pages or key tiles");
         return VLAB200_ERR_UNSUPPORTED;
     }
     if (max_len == 0) return VLAB200_OK;
-    const long long q_b = (long long)st->n_obs * n_q * S * hd * 2, mass_b = (long long)st->n_obs * st->n_kv * st->cap * 4;
+    const long long items = (long long)st->n_obs * st->n_kv, q_b = vb::size_product({items, R, hd, 2}), mass_b = vb::size_product({items, st->cap, 4});
     const vb::MemRange out[] = {{mass_out, mass_b}};
-    const vb::MemRange in[] = {{q, q_b}, {lse, (long long)st->n_obs * n_q * S * 4}, {st->k_pages, (long long)st->n_layers * mass_b / 4 * hd * 2},
+    const vb::MemRange in[] = {{q, q_b}, {lse, vb::size_product({items, R, 4})}, {st->k_pages, vb::size_product({st->n_layers, items, st->cap, hd, 2})},
                                {lens, st->n_obs * 4LL}, {pad_ranges, st->n_obs * 8LL}, {mass_in == mass_out ? nullptr : mass_in, mass_b}};
     if (vb::writes_overlap(out, 1, in, 6)) return VLAB200_ERR_ARG;
     vb::KeyMassParams p;

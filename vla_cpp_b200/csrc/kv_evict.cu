@@ -257,13 +257,13 @@ extern "C" int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_k
     const uintptr_t al = reinterpret_cast<uintptr_t>(src->k_pages) | reinterpret_cast<uintptr_t>(src->v_pages) |
                          reinterpret_cast<uintptr_t>(dst->k_pages) | reinterpret_cast<uintptr_t>(dst->v_pages);
     if (al & 15) return VLAB200_ERR_ARG;
-    const long long pages = (long long)src->n_layers * src->n_obs * src->n_kv;
+    const long long pages = vb::size_product({src->n_layers, src->n_obs, src->n_kv});
     if (pages > 0x7fffffffLL) {
         vb::set_last_error("kv_evict: more than 2^31 - 1 pages");
         return VLAB200_ERR_UNSUPPORTED;
     }
     // rows are read while others are written: nothing that is written may overlap anything that is read, or one another
-    const long long src_b = pages * src->cap * hd * 2, dst_b = pages * dst->cap * hd * 2;
+    const long long src_b = vb::size_product({pages, src->cap, hd, 2}), dst_b = vb::size_product({pages, dst->cap, hd, 2});
     const vb::MemRange in[] = {{src->k_pages, src_b}, {src->v_pages, src_b}, {mass, pages * src->cap * 4}, {lens, src->n_obs * 4LL}};
     const vb::MemRange out[] = {{dst->k_pages, dst_b}, {dst->v_pages, dst_b}, {kept, pages * keep * 4}, {mass_out, pages * dst->cap * 4},
                                 {lens_out, src->n_obs * 4LL}};

@@ -471,25 +471,26 @@ int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int32_t layer, c
     const int hd = st->head_dim;
     if (hd != 64 && hd != 128 && hd != 256) return VLAB200_ERR_UNSUPPORTED;
     if (a->rot_dim < 0 || a->rot_dim % 2 || a->rot_dim > hd || !(a->eps >= 0.0f)) return VLAB200_ERR_ARG;
-    const int n_heads = a->n_q + (a->with_kv ? 2 * st->n_kv : 0);
+    const long long heads = a->n_q + (a->with_kv ? 2LL * st->n_kv : 0), rows = (long long)st->n_obs * a->S;
     const int es = a->x_is_f32 ? 4 : 2;
-    if (a->x_stride < (int64_t)n_heads * hd || a->x_stride * es % 16) return VLAB200_ERR_ARG;
+    if (a->x_stride < heads * hd || a->x_stride % (16 / es)) return VLAB200_ERR_ARG;
     const uintptr_t al = reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->q_out) |
                          (a->with_kv ? reinterpret_cast<uintptr_t>(st->k_pages) | reinterpret_cast<uintptr_t>(st->v_pages) : 0);
     if (al & 15) return VLAB200_ERR_ARG;
     vb::RopeNormParams p;
-    const long long rows = (long long)st->n_obs * a->S;
     if (rows == 0) return VLAB200_OK;
-    const long long pages_b = a->with_kv ? (long long)st->n_layers * st->n_obs * st->n_kv * st->cap * hd * 2 : 0;
+    if (rows > 0x7fffffffLL || (long long)a->S * hd > 0x7fffffffLL || heads > 2048 || (long long)st->cap * hd > 0x7fffffffLL ||
+        (a->with_kv && vb::size_product({st->n_layers, st->n_obs, st->n_kv}) > 0x7fffffffLL) ||
+        vb::size_product({rows, a->x_stride, es}) == LLONG_MAX) {
+        vb::set_last_error("qk_norm_rope_append: more than 2^31 - 1 rows, pages or elements of a page, 2,048 heads of a row, or 2^63 bytes of x");
+        return VLAB200_ERR_UNSUPPORTED;
+    }
+    const int n_heads = (int)heads;
+    const long long pages_b = a->with_kv ? vb::size_product({st->n_layers, st->n_obs, st->n_kv, st->cap, hd, 2}) : 0;
     const vb::MemRange out[] = {{a->q_out, rows * a->n_q * hd * 2}, {st->k_pages, pages_b}, {st->v_pages, pages_b}};
     const vb::MemRange in[] = {{a->x, ((rows - 1) * a->x_stride + n_heads * hd) * es}, {a->q_norm, hd * 4}, {a->k_norm, hd * 4},
                                {a->freqs, a->rot_dim * 4LL}, {a->pos, rows * 4}, {a->row0, st->n_obs * 4LL}, {a->n_tok, st->n_obs * 4LL}};
     if (vb::writes_overlap(out, 3, in, 7)) return VLAB200_ERR_ARG;
-    if (rows > 0x7fffffffLL || (long long)a->S * hd > 0x7fffffffLL || n_heads > 2048 ||
-        (long long)st->cap * hd > 0x7fffffffLL) {
-        vb::set_last_error("qk_norm_rope_append: more than 2^31 - 1 rows or elements of a page, or 2,048 heads of a row");
-        return VLAB200_ERR_UNSUPPORTED;
-    }
     p.M = (unsigned)rows;
     const long long page0 = (long long)layer * st->n_obs * st->n_kv * st->cap * hd;
     p.x = a->x;
