@@ -353,7 +353,7 @@ def qk_norm_rope_append(store, layer, x, S, n_q, freqs=None, q_norm=None, k_norm
     if S < 0 or n_q <= 0 or x.dim() != 2 or x.shape[0] != B * S or x.shape[1] < width or x.stride(1) != 1:
         raise VlaB200Error(ERR_ARG, f"x: [{B * S}, >= {width}] with adjacent columns is needed, not {tuple(x.shape)}")
     if freqs is not None:
-        _need_tensor(freqs, "freqs", torch.float64, (freqs.numel(),), dev)
+        _need_tensor(freqs, "freqs", torch.float64, (freqs.numel() if isinstance(freqs, torch.Tensor) else 0,), dev)
     if q_norm is not None:
         _need_tensor(q_norm, "q_norm", f32, (hd,), dev)
     if k_norm is not None:
