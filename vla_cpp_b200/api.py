@@ -474,8 +474,8 @@ def kv_evict(src, dst, mass, keep, lens=None, max_len=None, sink=0, recent=0, ma
     pages = (src.n_layers, src.n_obs, src.n_kv)
     if dst.k.get_device() != dev:
         raise VlaB200Error(ERR_ARG, f"the stores are on {src.k.device} and {dst.k.device}")
-    if keep <= 0:
-        raise VlaB200Error(ERR_ARG, f"keep: {keep} rows")
+    if keep <= 0 or keep > dst.cap:
+        raise VlaB200Error(ERR_ARG, f"keep: {keep} rows, dst has {dst.cap}")
     _need_tensor(mass, "mass", torch.float32, (*pages, src.cap), dev)
     if lens is not None:
         _need_tensor(lens, "lens", torch.int32, (src.n_obs,), dev)
