@@ -221,6 +221,8 @@ VLAB200_API int32_t vlab200_qk_norm_rope_append(const vlab200_kv_store *st, int3
  * kernels may overlap) lets the blocks of a call be dealt to the SMs evenly where that pays (0 bytes: it does not); NULL: units of 256
  * query rows stay whole.  Results are the same from run to run for the same lengths, and agree to rounding between the two.  The head
  * widths are 64, 128 and 256.
+ * How work is dealt goes by max_len and the number of units -- the host does not see lens -- so a bound near the longest observation is
+ * the fast one: pages with much room and max_len = cap are cut up for rows that nobody has.
  * Stands beside vlab200_attention, which has one key range for all observations (src/models/smolvla.cpp:870-881 are the reference's cross
  * layers). */
 VLAB200_API int64_t vlab200_cross_attention_ws_bytes(const vlab200_kv_store *st, int32_t S, int32_t n_q,
@@ -249,7 +251,11 @@ VLAB200_API int32_t vlab200_key_mass(const vlab200_kv_store *st, int32_t layer, 
  * them are left as they were.  lens: int32 [n_obs], taken into [0, max_len], or NULL (max_len); max_len <= src cap, keep <= dst cap.  The
  * stores differ in nothing but cap, prefix_len and memory.
  * A store of keep + suffix rows with prefix_len = keep then serves the calls above as the larger one did, with the suffix at its old
- * positions.  No counterpart in the reference. */
+ * positions.  Where an observation kept fewer than keep rows, nobody wrote the rows between lens_out[b] and keep: its suffix goes to
+ * row0 = lens_out and lens says where it ends, and vlab200_attention and the denoise loop, which know one length, need keep rows of every
+ * observation.  Hidden rows (pad_ranges) are rows of weight 0 here: one that is protected, or that fewer than keep rows outweigh, is kept,
+ * and nothing hides it in dst; so keep no more rows than weigh anything, and protect none that is hidden.  No counterpart in the
+ * reference. */
 VLAB200_API int32_t vlab200_kv_evict(const vlab200_kv_store *src, const vlab200_kv_store *dst, const float *mass, const int32_t *lens,
                                      int32_t max_len, int32_t keep, int32_t sink, int32_t recent, int32_t *kept, float *mass_out,
                                      int32_t *lens_out, void *stream);

@@ -37,3 +37,31 @@ def test_attention_over_what_was_kept(B, P, S, n_q, n_kv, hd, keep):
     assert bool((err <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * size).all()), (err / size).max().item()
     z, lse = vb.cross_attention(small, 0, q, lens=left)
     check_attention(torch, small, 0, q, left, None, z, lse)
+
+
+@pytest.mark.parametrize("hd,n_q,n_kv,S", [(64, 6, 2, 20), (256, 8, 1, 1)])
+def test_hidden_rows_go_where_enough_others_weigh_something(hd, n_q, n_kv, S):
+    """Hidden rows weigh nothing: with no more rows kept than are visible, and none of the protected ones hidden, none of them is left."""
+    torch = require_cuda()
+    import vla_cpp_b200 as vb
+
+    B, P, keep = 4, 180, 100
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    st, small = vb.KvStore(1, B, n_kv, hd, 0, P), vb.KvStore(1, B, n_kv, hd, keep, 0)
+    st.k.normal_(0, 1, generator=g)
+    st.v.normal_(0, 1, generator=g)
+    lens = torch.tensor([P, 150, 170, 130], dtype=torch.int32, device="cuda")
+    pads = torch.tensor([[60, 100], [4, 54], [120, 130], [50, 80]], dtype=torch.int32, device="cuda")  # 140, 100, 160 and 100 visible rows
+    for b, (lo, hi) in enumerate(pads.tolist()):
+        st.k[:, b, :, lo:hi] = float("nan")
+        st.v[:, b, :, lo:hi] = float("nan")
+    q = torch.randn(B, n_q, S, hd, device="cuda", generator=g).bfloat16()
+    _, lse = vb.cross_attention(st, 0, q, lens=lens, pad_ranges=pads)
+    mass = vb.key_mass(st, 0, q, lse, lens=lens, pad_ranges=pads)
+    left, kept, _ = vb.kv_evict(st, small, mass[None], keep, lens=lens, sink=4, recent=8)
+    rows = kept[0].long()
+    assert left.tolist() == [keep] * B
+    assert not ((rows >= pads[:, None, :1]) & (rows < pads[:, None, 1:])).any()
+    out, lse = vb.cross_attention(small, 0, q, lens=left)
+    check_attention(torch, small, 0, q, left, None, out, lse)
+    assert vb.device_status() == 0

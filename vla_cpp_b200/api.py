@@ -414,7 +414,8 @@ def cross_attention(store, layer, q, lens=None, max_len=None, pad_ranges=None, s
 
     q: bf16 [n_obs, n_q, S, hd]; lens: int32 [n_obs] rows of every observation or None (max_len, by default the store's cap);
     pad_ranges: int32 [n_obs, 2] hidden rows [lo, hi) or None.  out: bf16 [n_obs, S, n_q * hd], lse: f32 [n_obs, n_q, S] (0 and -inf for a
-    row that sees nothing).  split=False takes no workspace: work is cut at whole units only."""
+    row that sees nothing).  split=False takes no workspace: work is cut at whole units only.  Work is dealt by max_len, not by lens: give a
+    bound near the longest where the pages have much room."""
     import torch
 
     dev, S, n_q, max_len = _ragged_args(store, q, lens, max_len, pad_ranges)
@@ -467,6 +468,8 @@ def kv_evict(src, dst, mass, keep, lens=None, max_len=None, sink=0, recent=0, ma
     mass: f32 [n_layers, n_obs, n_kv, src.cap] (key_mass per layer); lens: int32 [n_obs] rows of every observation or None (max_len, by
     default src.cap); the first `sink` and last `recent` rows stay in any case.  mass_out: f32 [n_layers, n_obs, n_kv, dst.cap], kept: int32
     [n_layers, n_obs, n_kv, keep] (indices in src, then -1) and lens_out: int32 [n_obs] are allocated where they are None.
+    Rows that pad_ranges hid from the other calls have weight 0 and no protection from being kept where too few weigh more, or from sink and
+    recent; nothing hides them in dst.
     Returns (lens_out, kept, mass_out)."""
     import torch
 

@@ -21,7 +21,8 @@
 // leaves un-normalised rows with their maximum and sum in the workspace, at most two pieces per CTA, and cross_combine_kernel merges them
 // in order.
 //
-// Measured (cold L2): 4 prompts of 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 rows 199 us = 1,030 TFLOP/s; there the chain of a
+// Measured (graph replay, cold L2): 4 prompts of 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 rows 201 us = 1,020 TFLOP/s (in a stream
+// of calls on changing inputs 214 = 955); there the chain of a
 // tile's block -- S, softmax, P V, some 3,400 clocks -- bounds it, of which the pipe computes 2,048 for the two tiles.  64 x 50 tokens, 15 / 5
 // heads of 64, over 113 to 241 rows 22 us, and 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 rows 35 us: the chain of a unit's blocks
 // (2,400 to 3,000 clocks each), of the first loads (5,000 to 8,000 with the launch) and of the store bounds those.

@@ -15,9 +15,10 @@
 //   16 sum warps     four per lane quarter, 128 columns of every second (heads of 256: fourth) chunk each: p = 2^(s c - lse')
 //
 // One query token: K streams once, HBM bounds it.  Many: the exponentials (16 per clock and SM) at heads of 64 and 128, at 256 their sum
-// with the product's chain.  Measured (cold L2): 4 x 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 keys 145 us, 90 of them the
-// exponential unit's (a polynomial on the FMA pipe for every fourth or eighth of them was slower: the sum warps' issue slots are full);
-// 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 keys 26 us; one token over 16,001 keys 14 us, 10.5 with the pages in L2.
+// with the product's chain.  Measured (graph replay, cold L2): 4 x 816 tokens, 20 / 5 heads of 128, over 4,097 to 8,190 keys 151 us (142 with
+// the pages in L2), 90 of them the exponential unit's; a polynomial on the FMA pipe for every fourth or eighth of them was slower, though
+// 38 % of the issue slots are in use: what held it up was not found.
+// 64 x 51 tokens, 8 / 1 heads of 256, over 304 to 816 keys 26.6 us (20.5); one token over 16,001 keys 14 to 16 us (10.3).
 #include <cuda_bf16.h>
 
 #include "f32x2.cuh"

@@ -5,9 +5,12 @@
 // The keep-th largest key of a page decides -- the weight's bits mapped so that they compare as whole numbers, protected rows on top,
 // no-numbers at the bottom.  Pages of up to 1,024 rows: one kernel, a warp of every block finds it bit by bit with the keys in registers, then
 // the block copies its rows.  Longer pages: a block each finds it 8 bits at a time from histograms, a second kernel copies.  K and V rows go
-// 16 bytes per thread: all there is to move, HBM bounds it.  Measured (cold L2): 1,152 pages of 304 to 816 rows of 256, 387 of them kept,
-// 156 us = 5.8 TB/s of the 6.45 of a copy, 144 of them the copy's; with histograms and a second kernel 184.  16 pages of 241 rows of 64,
-// 120 kept, 10.3 us (14.3).
+// 16 bytes per thread: all there is to move, HBM bounds it.  Measured (graph replay, cold L2): 1,152 pages of 304 to 816 rows of 256, 387 of
+// them kept, 158 us = 5.7 TB/s of the 6.45 of a copy (151 in a stream of calls), 144 of them the copy's; with histograms and a second kernel
+// 184.  16 pages of 241 rows of 64, 120 kept, 10.2 us (14.3).
+// Above 1,024 rows the selection bounds it, a chain of barriers per 256 rows, five times over a page's weights: 80 pages of 16,384 rows of 64,
+// 4,096 kept, 170 us = 1.0 TB/s; 144 pages of 8,192 rows of 256, 2,048 kept, 193 us = 3.2; 1,152 pages of 1,600 rows of 256, 800 kept, 387 us =
+// 4.9.  Call after call without a graph the first two take 351 and 322; why was not looked into.
 #include "host_common.h"
 #include "tc5.cuh"
 

@@ -11,8 +11,8 @@
 // the token's r / 2 of each once and exchanges them through shared memory).  In the half layout a lane holds columns 8 j .. 8 j + 7 and
 // their partners r / 2 further on, so the rotation needs no exchange.  Few tokens: a token's heads are dealt over several warps.
 //
-// Measured (cold L2): 33 prefixes of 306 to 816 tokens, 8 + 2 heads of 256 in bf16, 53 us = 4.2 TB/s of the 6.45 of a copy (an elementwise
-// kernel of torch moves as many bytes in 41).  Loads and stores alone take 47 us, arithmetic alone 40: 16 warps of 128 registers issue half
+// Measured (graph replay, cold L2): 33 prefixes of 306 to 816 tokens, 8 + 2 heads of 256 in bf16, 55 us = 4.1 TB/s of the 6.45 of a copy (49 in a
+// stream of calls; an elementwise kernel of torch moves as many bytes in 41).  Loads and stores alone take 47 us, arithmetic alone 40: 16 warps of 128 registers issue half
 // of the time and hide neither wholly.  A table of the heads' places instead of arithmetic per step 59 -> 53; no change from rows straight to
 // shared memory instead of through registers, nor from equal numbers of live tokens per warp; slower: 24 warps of 80 registers (57), two steps
 // at a time (56); whole rows by bulk copies of a loader warp 51, but 64 x 51 tokens of 15 + 10 heads of 64 in float32 22 instead of 17.
@@ -428,7 +428,9 @@ static int launch_rope_norm(RopeNormParams &p, cudaStream_t stream) {
 template <int HD, bool F32>
 static int dispatch_rope_norm(RopeNormParams &p, int interleaved, cudaStream_t stream) {
     if (interleaved) return launch_rope_norm<HD, ROPE_PAIRS, F32>(p, stream);
-    // chunks of 8 columns and the chunks of their partners
+    // Chunks of 8 columns and the chunks of their partners, in one lane; at other widths the partners lie in the middle of other lanes' chunks and
+    // are read one by one.  33 x 816 tokens, 8 + 2 heads of 256, bf16, 276 MB (graph replay, cold L2): 256 columns rotated 55 us, 250 133, 100 96;
+    // 64 x 51 tokens, 15 + 10 heads of 64, float32: 32 columns 18.4, 20 24.6.
     if (p.rot % 16 == 0) return launch_rope_norm<HD, ROPE_HALF_LANES, F32>(p, stream);
     return launch_rope_norm<HD, ROPE_HALF_ANY, F32>(p, stream);
 }
