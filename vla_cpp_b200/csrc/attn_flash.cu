@@ -437,7 +437,6 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     uint64_t *pair_bar = bars + 32;  // [4] the two softmax warps of a lane quarter meet here (64 arrivals)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 36);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    uint32_t *pv_issued = tmem_slot + 2;  // P V blocks issued so far (even CTA)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -466,7 +465,6 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             mbar_init(&pv_done[i], 1);
         }
         *abort_flag = 0;
-        *pv_issued = 0;
         fence_barrier_init();
     }
     __syncthreads();
@@ -545,25 +543,13 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             // used the same TMEM buffer (jbx - FP_NS) has finished.  This thread issues only the Q K^T MMAs
             // (16 per block, the longer stream); the P V MMAs come from a thread of their own (warp
             // FP_PV_WARP): one thread issuing both spent ~2500 cycles per block, twice the tensor time.
-            // It does not wait for that P V block to COMPLETE: the tensor pipe takes the MMAs of a CTA pair in the order
-            // they were issued, so it is enough that the P V thread has issued them (a counter in shared memory that
-            // it bumps after its last MMA of a block).  Waiting for the commit instead kept the pipe idle for the
-            // ~500 cycles between the block's last MMA and the moment this thread saw the barrier flip.
+            // It waits for that P V block to be COMPLETE, since S lies over its P: the pipe keeps the order of one thread's
+            // MMAs, not of two threads'.  A counter of the P V blocks issued (a fence, a release, an acquire and a fence in
+            // between) was faster -- 456 us instead of 477 at 1,024 observations of 51 tokens over 867 keys, heads of 256 -- but
+            // in the cross-attention kernel of the same structure S overtook the last steps of P V now and then.
             auto ready_s = [&](uint32_t jbx) -> bool {
                 bool r = mbar_wait(&k_full[jbx % FP_STAGES], (jbx / FP_STAGES) & 1u, wc, DEV_TIMEOUT_FULL);
-                if (r && jbx >= FP_NS && ld_acquire_cta(pv_issued) < jbx - FP_NS + 1u) {
-                    const long long t0 = clock64();
-                    for (uint32_t it = 1; ld_acquire_cta(pv_issued) < jbx - FP_NS + 1u; ++it) {
-                        if ((it & 63u) == 0) {
-                            if (*abort_flag) return false;
-                            if (clock64() - t0 > wc.budget) {
-                                *abort_flag = 1;
-                                atomicCAS(p.status, 0, (int)DEV_TIMEOUT_FULL);
-                                return false;
-                            }
-                        }
-                    }
-                }
+                if (r && jbx >= FP_NS) r = mbar_wait(&pv_done[jbx % FP_NS], (jbx / FP_NS & 1u) ^ 1u, wc, DEV_TIMEOUT_FULL);
                 return r;
             };
             for (int unit = cid; ok && unit < n_units; unit += ncl, ++ui) {
@@ -620,8 +606,6 @@ attn_flash_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                         for (int k16 = 0; k16 < FP_BKV / 16; ++k16)
                             mma_f16_tmem_a_pair(tmem_base, p_tmem + (uint32_t)(k16 * 8), v_desc + (uint64_t)(k16 * 128), idesc_o,
                                                 (j | k16) != 0 ? 1u : 0u);
-                        tc_fence_before();
-                        st_release_cta(pv_issued, jb + 1u);
                         tc_commit_pair(&pv_done[sb], 3);
                         tc_commit_pair(&v_free[st], 3);
                     }

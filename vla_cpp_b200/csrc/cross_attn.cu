@@ -500,7 +500,7 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
         uint32_t si = 0, jb = 0;
         uint32_t blk[2] = {0, 0}, seg[2] = {0, 0};  // blocks and segments of each tile so far
         // S of a segment's first block follows the P V of the segment before: by tile where its Q has its own stage, behind both otherwise.
-        // A tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order.
+        // A tile's S buffer held the P of its last block: that P V was issued before, and the pipe keeps the order of one warp's products.
         auto tiles_of = [&](const XaSegment &g) { return p.R > g.mt * 256 + 128 ? 2 : 1; };
         XaSegment after;
         bool here = work.next(s);
@@ -724,8 +724,10 @@ cross_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
 // ------------------------------------------------------------------ heads of 256: CTA pairs --
 // O alone takes 256 columns of TMEM and K, V of 128 rows 64 KB each, so one CTA has room for one tile and no second block.  A pair of CTAs
 // (tcgen05 cta_group::2, M = 256) shares every block: each stages half of K's rows and half of V's columns, and holds one of the
-// unit's two tiles.  Two S buffers lie behind O; two warps of the even CTA issue the products, Q K^T up to a block ahead of P V (the first
-// follows the second by a counter: the pipe keeps their order); the odd CTA tells the even one what has landed.
+// unit's two tiles.  Two S buffers lie behind O; two warps of the even CTA issue the products, Q K^T up to a block ahead of P V; the odd CTA
+// tells the even one what has landed.  P lies over its S, so the S of the block two further on waits for the P V to be complete: the pipe does
+// not keep the order of two warps' products.  With a counter of the blocks issued instead, S overtook the last steps of P V in one call of a thousand
+// behind another kernel with cold caches, and the counter gave nothing: 64 x 51 tokens over 304 to 816 rows 28.9 us, 29.0 so.
 //   8 softmax warps   lane quarter = warp & 3, column half = warp >> 2: the two warps of a row exchange maxima and sums through shared memory
 // A unit's O is drained after the next unit's first block, so the pipe does not wait for it.
 constexpr int XP_THREADS = 384, XP_LOADER = 8, XP_S = 9, XP_PV = 10, XP_CLEANER = 11;
@@ -758,7 +760,6 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     uint64_t *v_raw = bars + 22;                                                               // [ST]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    uint32_t *pv_issued = tmem_slot + 2;  // P V blocks issued so far (even CTA)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const WaitCtx wc{abort_flag, p.status};
@@ -785,7 +786,6 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         }
         for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 64);
         *abort_flag = 0;
-        *pv_issued = 0;
         fence_barrier_init();
     }
     __syncthreads();
@@ -858,25 +858,8 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 ok = warp_wait(q_full, si & 1u, wc, DEV_TIMEOUT_FULL);
                 for (int j = s.j0; ok && j < s.j1; ++j, ++jb) {
                     ok = warp_wait(&k_full[jb % ST], (jb / ST) & 1u, wc, DEV_TIMEOUT_FULL);
-                    // the P V of the block that used this S buffer has to be in the pipe
-                    if (ok && jb >= NS && ld_acquire_cta(pv_issued) < jb - NS + 1u) {
-                        const long long t0 = clock64();
-                        for (uint32_t it = 1; ld_acquire_cta(pv_issued) < jb - NS + 1u; ++it) {
-                            if ((it & 63u) == 0) {
-                                if (*abort_flag) {
-                                    ok = false;
-                                    break;
-                                }
-                                if (clock64() - t0 > wc.budget) {
-                                    *abort_flag = 1;
-                                    atomicCAS(p.status, 0, (int)DEV_TIMEOUT_FULL);
-                                    ok = false;
-                                    break;
-                                }
-                            }
-                        }
-                    }
-                    ok = __all_sync(0xffffffffu, ok) != 0;
+                    // the P V of the block that used this S buffer has read its weights
+                    if (ok && jb >= NS) ok = warp_wait(&pv_done[jb % NS], (jb / NS & 1u) ^ 1u, wc, DEV_TIMEOUT_FULL);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t st = jb % ST, d = tmem_base + HD + (jb % NS) * BKV;
@@ -927,8 +910,6 @@ cross_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                         for (int kk = 0; kk < BKV / 16; ++kk)
                             mma_f16_tmem_a_pair(tmem_base, p_tmem + (uint32_t)(kk * 8), v_desc + (uint64_t)(kk * 128), idesc_o,
                                                 j != s.j0 || kk != 0 ? 1u : 0u);
-                        tc_fence_before();
-                        st_release_cta(pv_issued, jb + 1u);
                         tc_commit_pair(&pv_done[sb], 3);
                         tc_commit_pair(&v_free[st], 3);
                         if (j + 1 == s.j1) tc_commit_pair(o_done, 3);

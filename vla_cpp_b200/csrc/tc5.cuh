@@ -127,17 +127,6 @@ __device__ __forceinline__ void stage_release(uint64_t *bar, float consumed, int
         asm volatile("{\n.reg .b64 t;\nmbarrier.arrive.shared::cta.b64 t, [%0];\n}" ::"r"(smem_u32(bar) + (done & 0u)) : "memory");
 }
 
-// A counter in shared memory by which a warp that issues products follows another one that does.  The order of their instructions in the tensor
-// pipe is that of  issue, tc_fence_before, st_release_cta  and  ld_acquire_cta, tc_fence_after, issue.
-__device__ __forceinline__ void st_release_cta(uint32_t *p, uint32_t v) {
-    asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_acquire_cta(const uint32_t *p) {
-    uint32_t v;
-    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
-    return v;
-}
-
 // generic-proxy writes to shared memory -> visible to the async proxy (TMA / tcgen05 reads)
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
